@@ -46,6 +46,8 @@ enum {
 
 /* ---- element types (dtype/src: Float32, Float16, BFloat16, Int32, Int64, Bool) ---- */
 enum { SVODB_F32 = 0, SVODB_F16 = 1, SVODB_BF16 = 2, SVODB_I32 = 3, SVODB_I64 = 4, SVODB_U8 = 5 };
+/* Only in paged caches (below): 8-bit floats, and powers of two (code c stands for 2^(c - 127), 255 for NaN). */
+enum { SVODB_E4M3 = 6, SVODB_E8M0 = 7 };
 
 /* ---- `kernels::Act` (tk/src/kernels/mod.rs:272-280); GELU_TANH is the extra
  * `Tensor::gelu` form (tensor/src/activation.rs:198-230). GELU is the exact (erf)
@@ -246,6 +248,50 @@ int svodb_attention_packed(const svodb_tensor* qkv, int32_t heads, int32_t kv_he
  * f32 partials o_part [S,B,T,H,D], m_part/l_part [S,B,T,H] (m in log2 units). */
 int svodb_combine_splits(const svodb_tensor* o_part, const svodb_tensor* m_part, const svodb_tensor* l_part,
                          svodb_tensor* o, void* stream);
+
+/* ---- a paged key/value cache ------------------------------------------------
+ * No counterpart in the reference, whose caches (`ops::Cache`) are rows of one length.
+ * Position p of sequence b lies in slot p % page_size of page table[b, p / page_size];
+ * entries of `table` behind a sequence's last page are never looked at, and two sequences
+ * may share pages (a common prefix) as long as nobody writes them. Pages hold the stream
+ * type, or e4m3 beside one power of two a token and head. A user's view of one layer of a
+ * larger buffer is a cache: any strides do, innermost 1. */
+typedef struct svodb_paged_cache {
+  const svodb_tensor* k;       /* [pages, page_size, kv_heads, D], the stream type or e4m3 */
+  const svodb_tensor* v;
+  const svodb_tensor* k_scale; /* [pages, kv_heads, page_size] e8m0 with e4m3 pages, else NULL */
+  const svodb_tensor* v_scale;
+  const svodb_tensor* table;   /* [B, width] i32 */
+} svodb_paged_cache;
+
+/* Writes a chunk: k, v [B, T, kv_heads, D]; row b's first lens[b] tokens (all T without
+ * `lens`; the count is taken as within 0..T) become positions start[b] and on of sequence b.
+ * With e4m3 pages a token's head row of values x gets the scale 2^e, e the least with
+ * max|x| <= 448 * 2^e (2^-127 for zeros), and holds round(x / 2^e); a row that holds a NaN or an
+ * infinity reads back as NaN. Slots that no token falls into stay as they are; two tokens
+ * of one call that fall into the same slot leave either there. A row whose positions leave
+ * the table and a token whose table entry is no page write nothing, and
+ * `svodb_device_status` says so. */
+int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_paged_cache* cache,
+                      const svodb_tensor* start, const svodb_tensor* lens, void* stream);
+
+/* Reads rows back: k, v [B, L, kv_heads, D] in the stream type (the pages', or any float type
+ * for e4m3 pages: value * scale, rounded once). Positions from lens[b] on are zeros; so are
+ * those without a page, which `svodb_device_status` reports. */
+int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, svodb_tensor* k, svodb_tensor* v,
+                     void* stream);
+
+/* Attention of a chunk over the cache it was written to: q [B, T, H, D] -> o [B, T, H, D].
+ * Query i of row b stands at position start[b] + i and sees keys 0 .. start[b] + lens[b] - 1
+ * (lens = T without `lens`), under `causal` those up to its own position, under a window
+ * those from window_left before to window_right behind it. Rows from lens[b] on and rows
+ * without a key are zeros (lse -inf). Of `opts`: causal, has_window, has_scale, lse,
+ * workspace; any other option is refused. `workspace`: svodb_attention_paged_workspace_bytes
+ * bytes, 16-byte aligned, for this call alone (two calls that may overlap on the GPU, or two
+ * graphs that may be replayed at once, have one each). */
+size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_paged_cache* cache);
+int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache, const svodb_tensor* start,
+                          const svodb_tensor* lens, const svodb_attn_opts* opts, svodb_tensor* o, void* stream);
 
 /* `ops::Qkv` (tk/src/ops/heads.rs:18-32). */
 typedef struct svodb_qkv_opts {

@@ -20,7 +20,7 @@ MAX_RANK = 5
 OK, ERR_SHAPE, ERR_DTYPE, ERR_HEADS, ERR_GRAPH, ERR_LAUNCH, ERR_UNREALIZED, ERR_ALIAS, ERR_TIMEOUT, \
     ERR_POISONED, ERR_WORKSPACE, ERR_UNSUPPORTED = range(12)
 
-F32, F16, BF16, I32, I64, U8 = range(6)
+F32, F16, BF16, I32, I64, U8, E4M3, E8M0 = range(8)
 
 NOALLOC_SCRATCH_BYTES = 8 << 20  # SVODB_NOALLOC_SCRATCH_BYTES
 
@@ -98,6 +98,10 @@ class AttnOpts(C.Structure):
         ("cache_app_v", TensorP),
         ("cache_app_lens", TensorP),
     ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [(n, TensorP) for n in ("k", "v", "k_scale", "v_scale", "table")]
 
 
 class QkvOpts(C.Structure):
@@ -193,6 +197,11 @@ SYMBOLS = [
     ("svodb_attention_splits_noalloc", C.c_int, [TensorP, TensorP, TensorP, C.POINTER(AttnOpts), TensorP, C.c_void_p]),
     ("svodb_attention_packed", C.c_int, [TensorP, C.c_int32, C.c_int32, C.POINTER(AttnOpts), TensorP, C.c_void_p]),
     ("svodb_combine_splits", C.c_int, [TensorP, TensorP, TensorP, TensorP, C.c_void_p]),
+    ("svodb_cache_write", C.c_int, [TensorP, TensorP, C.POINTER(PagedCache), TensorP, TensorP, C.c_void_p]),
+    ("svodb_cache_read", C.c_int, [C.POINTER(PagedCache), TensorP, TensorP, TensorP, C.c_void_p]),
+    ("svodb_attention_paged_workspace_bytes", C.c_size_t, [TensorP, C.POINTER(PagedCache)]),
+    ("svodb_attention_paged", C.c_int, [TensorP, C.POINTER(PagedCache), TensorP, TensorP, C.POINTER(AttnOpts), TensorP,
+                                        C.c_void_p]),
     ("svodb_heads", C.c_int, [TensorP, C.POINTER(QkvOpts), TensorP, TensorP, TensorP, C.c_void_p]),
     ("svodb_layer_norm", C.c_int, [TensorP, TensorP, TensorP, C.c_double, TensorP, C.c_void_p]),
     ("svodb_add_layer_norm", C.c_int, [TensorP, TensorP, TensorP, TensorP, C.c_double, TensorP, TensorP, C.c_void_p]),

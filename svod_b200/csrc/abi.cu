@@ -74,14 +74,14 @@ int check_launch(const char* op) {
 bool is_float(int dt) { return dt == SVODB_F32 || dt == SVODB_F16 || dt == SVODB_BF16; }
 bool is_half(int dt) { return dt == SVODB_F16 || dt == SVODB_BF16; }
 const char* dtype_name(int dt) {
-  static const char* names[] = {"Float32", "Float16", "BFloat16", "Int32", "Int64", "UInt8"};
-  return dt >= 0 && dt <= 5 ? names[dt] : "?";
+  static const char* names[] = {"Float32", "Float16", "BFloat16", "Int32", "Int64", "UInt8", "Float8E4M3", "Float8E8M0"};
+  return dt >= 0 && dt <= 7 ? names[dt] : "?";
 }
 size_t esize(int dt) {
   switch (dt) {
     case SVODB_F32: case SVODB_I32: return 4;
     case SVODB_I64: return 8;
-    case SVODB_U8: return 1;
+    case SVODB_U8: case SVODB_E4M3: case SVODB_E8M0: return 1;
     default: return 2;
   }
 }
@@ -288,7 +288,7 @@ int svodb_device_status(void* stream) {
     cudaMemsetAsync(w, 0, sizeof host, (cudaStream_t)stream);
     cudaStreamSynchronize((cudaStream_t)stream);
     if (host == kStatusBadIndex)
-      return fail(SVODB_ERR_SHAPE, "a device-side index was out of range (a cache row map entry)");
+      return fail(SVODB_ERR_SHAPE, "a device-side index was out of range (a cache row map or page table entry, or a position past the table)");
     return fail(SVODB_ERR_TIMEOUT, "a bounded device wait ran out (code %u)", host);
   }
   return SVODB_OK;
@@ -891,6 +891,266 @@ int svodb_combine_splits(const svodb_tensor* o_part, const svodb_tensor* m_part,
   c.dtype = o->dtype;
   launch_combine(c, (cudaStream_t)stream);
   chose_kernel(OP, "combine_splits", "{br:4}");
+  return check_launch(OP);
+}
+
+// ---------------------------------------------------------------------------
+// paged cache
+// ---------------------------------------------------------------------------
+namespace {
+
+// Checks a cache against a batch and a stream type (-1: whatever its pages hold) and fills `c`.
+int paged_cache(const char* OP, const svodb_paged_cache* p, int64_t batch, int stream_dtype, PagedCache& c) {
+  if (p == nullptr) return fail(SVODB_ERR_UNREALIZED, "%s: the cache is missing", OP);
+  TRY(realized(OP, "cache k", p->k));
+  TRY(realized(OP, "cache v", p->v));
+  TRY(realized(OP, "table", p->table));
+  const svodb_tensor *k = p->k, *v = p->v, *t = p->table;
+  if (k->rank != 4 || k->shape[1] <= 0 || k->shape[2] <= 0 || k->shape[3] <= 0)
+    return shape_err(OP, "cache k", k, "[pages, page_size, kv_heads, D]");
+  if (!same_shape(v, k)) return shape_err(OP, "cache v", v, "the shape of cache k");
+  if (v->dtype != k->dtype)
+    return fail(SVODB_ERR_DTYPE, "%s: cache v is %s, cache k is %s", OP, dtype_name(v->dtype), dtype_name(k->dtype));
+  const bool q8 = k->dtype == SVODB_E4M3;
+  if (!q8 && !is_float(k->dtype)) return fail(SVODB_ERR_DTYPE, "%s: cache k is %s, not a float type", OP, dtype_name(k->dtype));
+  if (!q8 && k->dtype != stream_dtype) return dtype_err(OP, "cache k", k->dtype, stream_dtype);
+  if (k->stride[3] != 1 || v->stride[3] != 1) return fail(SVODB_ERR_GRAPH, "%s: the head dim must be contiguous", OP);
+  if (q8 != (p->k_scale != nullptr) || q8 != (p->v_scale != nullptr))
+    return fail(SVODB_ERR_DTYPE, "%s: scales come with e4m3 pages, for keys and values, and with no others", OP);
+  if (k->shape[0] > INT32_MAX || k->shape[1] > INT32_MAX || k->shape[2] > INT32_MAX || k->shape[3] > INT32_MAX)
+    return shape_err(OP, "cache k", k, "sizes below 2^31");
+  const svodb_tensor* scales[2] = {p->k_scale, p->v_scale};
+  for (int i = 0; q8 && i < 2; ++i) {
+    const char* name = i == 0 ? "k scale" : "v scale";
+    TRY(realized(OP, name, scales[i]));
+    const svodb_tensor* s = scales[i];
+    if (s->rank != 3 || s->shape[0] != k->shape[0] || s->shape[1] != k->shape[2] || s->shape[2] != k->shape[1])
+      return shape_err(OP, name, s, "[pages, kv_heads, page_size]");
+    if (s->dtype != SVODB_E8M0) return fail(SVODB_ERR_DTYPE, "%s: %s is %s, expected Float8E8M0", OP, name, dtype_name(s->dtype));
+    if (s->shape[2] > 1 && s->stride[2] != 1) return fail(SVODB_ERR_GRAPH, "%s: a page's scales must be contiguous", OP);
+  }
+  if (t->rank != 2 || t->shape[0] != batch) return shape_err(OP, "table", t, "[B, width]");
+  if (t->dtype != SVODB_I32) return fail(SVODB_ERR_DTYPE, "%s: table is %s, expected Int32", OP, dtype_name(t->dtype));
+  if (t->shape[1] > 1 && t->stride[1] != 1) return fail(SVODB_ERR_GRAPH, "%s: a table row must be contiguous", OP);
+  if (t->shape[1] * k->shape[1] > 0x7fffff00LL) return shape_err(OP, "table", t, "a reach below 2^31 positions");
+  // a negative stride would leave the spans that the alias checks and the kernels' maps go by
+  for (const svodb_tensor* x : {k, v, p->k_scale, p->v_scale, t})
+    for (int i = 0; x != nullptr && i < x->rank; ++i)
+      if (x->stride[i] < 0) return fail(SVODB_ERR_GRAPH, "%s: a cache with negative strides", OP);
+  c = PagedCache{};
+  c.k = k->data, c.v = v->data;
+  c.k_sp = k->stride[0], c.k_ss = k->stride[1], c.k_sh = k->stride[2];
+  c.v_sp = v->stride[0], c.v_ss = v->stride[1], c.v_sh = v->stride[2];
+  if (q8) {
+    c.k_scale = (uint8_t*)p->k_scale->data, c.v_scale = (uint8_t*)p->v_scale->data;
+    c.ks_sp = p->k_scale->stride[0], c.ks_sh = p->k_scale->stride[1];
+    c.vs_sp = p->v_scale->stride[0], c.vs_sh = p->v_scale->stride[1];
+  }
+  c.table = (const int32_t*)t->data;
+  c.table_sb = t->stride[0];
+  c.width = t->shape[1], c.pages = k->shape[0];
+  c.page_size = (int)k->shape[1], c.kv_heads = (int)k->shape[2], c.d = (int)k->shape[3];
+  c.dtype = k->dtype;
+  return SVODB_OK;
+}
+
+// `[B]` i32, contiguous.
+int row_counts(const char* OP, const char* name, const svodb_tensor* t, int64_t batch) {
+  TRY(realized(OP, name, t));
+  if (t->rank != 1 || t->shape[0] != batch) return shape_err(OP, name, t, "[B]");
+  if (t->dtype != SVODB_I32) return fail(SVODB_ERR_DTYPE, "%s: %s is %s, expected Int32", OP, name, dtype_name(t->dtype));
+  if (batch > 1 && t->stride[0] != 1) return fail(SVODB_ERR_GRAPH, "%s: %s must be contiguous", OP, name);
+  return SVODB_OK;
+}
+
+// A `[B, T, heads, D]` operand beside a cache.
+int chunk_rows(const char* OP, const char* name, const svodb_tensor* t, int64_t heads, int64_t d, const char* expected) {
+  if (t->rank != 4 || t->shape[2] != heads || t->shape[3] != d) return shape_err(OP, name, t, expected);
+  if (!is_float(t->dtype)) return fail(SVODB_ERR_GRAPH, "%s: %s is %s, not a float type", OP, name, dtype_name(t->dtype));
+  if (t->stride[3] != 1) return fail(SVODB_ERR_GRAPH, "%s: the head dim must be contiguous", OP);
+  if (t->shape[1] > 0x7fffff00LL) return shape_err(OP, name, t, "a chunk below 2^31 tokens");
+  for (int i = 0; i < 3; ++i)
+    if (t->stride[i] < 0) return fail(SVODB_ERR_GRAPH, "%s: %s has negative strides", OP, name);
+  return SVODB_OK;
+}
+
+// No two elements of a written tensor in one place, by strides that leave no room for it.
+bool apart(const svodb_tensor* t) {
+  int64_t reach[SVODB_MAX_RANK], step[SVODB_MAX_RANK];
+  int n = 0;
+  for (int i = 0; i < t->rank; ++i)
+    if (t->shape[i] > 1) step[n] = t->stride[i], reach[n++] = (t->shape[i] - 1) * t->stride[i];
+  int64_t covered = 0;  // by the dims taken so far, smallest stride first
+  for (int taken = 0; taken < n; ++taken) {
+    int at = taken;
+    for (int i = taken; i < n; ++i)
+      if (step[i] < step[at]) at = i;
+    if (step[at] <= covered) return false;
+    covered += reach[at];
+    const int64_t s = step[at], r = reach[at];
+    step[at] = step[taken], reach[at] = reach[taken];
+    step[taken] = s, reach[taken] = r;
+  }
+  return true;
+}
+
+}  // namespace
+
+int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_paged_cache* cache,
+                      const svodb_tensor* start, const svodb_tensor* lens, void* stream) {
+  static const char* OP = "cache_write";
+  GUARD(OP);
+  if (active_rows() != nullptr) return rows_unsupported(OP);
+  TRY(realized(OP, "k", k));
+  TRY(realized(OP, "v", v));
+  if (k->rank != 4) return shape_err(OP, "k", k, "[B, T, kv_heads, D]");
+  CacheWriteArgs a{};
+  TRY(paged_cache(OP, cache, k->shape[0], k->dtype, a.c));
+  TRY(chunk_rows(OP, "k", k, a.c.kv_heads, a.c.d, "[B, T, kv_heads, D] of the cache"));
+  TRY(chunk_rows(OP, "v", v, a.c.kv_heads, a.c.d, "[B, T, kv_heads, D] of the cache"));
+  if (!same_shape(v, k)) return shape_err(OP, "v", v, "the shape of k");
+  if (v->dtype != k->dtype) return dtype_err(OP, "v", v->dtype, k->dtype);
+  const int64_t B = k->shape[0], T = k->shape[1];
+  TRY(row_counts(OP, "start", start, B));
+  if (lens != nullptr) TRY(row_counts(OP, "lens", lens, B));
+  const svodb_tensor* outs[4] = {cache->k, cache->v, cache->k_scale, cache->v_scale};
+  for (int i = 0; i < 4; ++i) {
+    if (outs[i] == nullptr) continue;
+    if (!apart(outs[i])) return fail(SVODB_ERR_GRAPH, "%s: a cache whose slots overlap", OP);
+    TRY(no_alias(OP, outs[i], {k, v, start, lens, cache->table}));
+    for (int j = 0; j < i; ++j)
+      // k and v of one buffer [.., 2, ..] interleave: their spans overlap, their slots do not
+      if (outs[j] != nullptr && outs[j]->data == outs[i]->data)
+        return fail(SVODB_ERR_ALIAS, "%s: keys, values and scales share storage", OP);
+  }
+  if (B * T == 0 || a.c.pages == 0) {
+    chose_graph(OP, "shape");
+    return SVODB_OK;
+  }
+  if (B * T * a.c.kv_heads > (int64_t)1 << 32) return fail(SVODB_ERR_UNSUPPORTED, "%s: more than 2^32 head rows a call", OP);
+  a.k = k->data, a.v = v->data;
+  a.k_sb = k->stride[0], a.k_st = k->stride[1], a.k_sh = k->stride[2];
+  a.v_sb = v->stride[0], a.v_st = v->stride[1], a.v_sh = v->stride[2];
+  a.batch = B, a.t = T, a.dtype = k->dtype;
+  a.start = (const int32_t*)start->data;
+  a.lens = lens != nullptr ? (const int32_t*)lens->data : nullptr;
+  a.status = device_status_word();
+  const int vec = launch_cache_write(a, (cudaStream_t)stream);
+  if (vec) chose_kernel(OP, "cache_write", a.c.dtype == SVODB_E4M3 ? "{e4m3}" : "{copy}");
+  else chose_graph(OP, "shape");
+  return check_launch(OP);
+}
+
+int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, svodb_tensor* k, svodb_tensor* v,
+                     void* stream) {
+  static const char* OP = "cache_read";
+  GUARD(OP);
+  if (active_rows() != nullptr) return rows_unsupported(OP);
+  TRY(realized(OP, "k", k));
+  TRY(realized(OP, "v", v));
+  if (k->rank != 4) return shape_err(OP, "k", k, "[B, L, kv_heads, D]");
+  CacheReadArgs a{};
+  TRY(paged_cache(OP, cache, k->shape[0], k->dtype, a.c));
+  TRY(chunk_rows(OP, "k", k, a.c.kv_heads, a.c.d, "[B, L, kv_heads, D] of the cache"));
+  TRY(chunk_rows(OP, "v", v, a.c.kv_heads, a.c.d, "[B, L, kv_heads, D] of the cache"));
+  if (!same_shape(v, k)) return shape_err(OP, "v", v, "the shape of k");
+  if (v->dtype != k->dtype) return dtype_err(OP, "v", v->dtype, k->dtype);
+  const int64_t B = k->shape[0], T = k->shape[1];
+  TRY(row_counts(OP, "lens", lens, B));
+  if (!apart(k) || !apart(v)) return fail(SVODB_ERR_GRAPH, "%s: an output whose elements overlap", OP);
+  TRY(no_alias(OP, k, {cache->k, cache->v, cache->k_scale, cache->v_scale, cache->table, lens, v}));
+  TRY(no_alias(OP, v, {cache->k, cache->v, cache->k_scale, cache->v_scale, cache->table, lens}));
+  if (B * T == 0) {
+    chose_graph(OP, "shape");
+    return SVODB_OK;
+  }
+  if (B * T * a.c.kv_heads > (int64_t)1 << 32) return fail(SVODB_ERR_UNSUPPORTED, "%s: more than 2^32 head rows a call", OP);
+  a.k = k->data, a.v = v->data;
+  a.k_sb = k->stride[0], a.k_st = k->stride[1], a.k_sh = k->stride[2];
+  a.v_sb = v->stride[0], a.v_st = v->stride[1], a.v_sh = v->stride[2];
+  a.batch = B, a.len = T, a.dtype = k->dtype;
+  a.lens = (const int32_t*)lens->data;
+  a.status = device_status_word();
+  const int vec = launch_cache_read(a, (cudaStream_t)stream);
+  if (vec) chose_kernel(OP, "cache_read", a.c.dtype == SVODB_E4M3 ? "{e4m3}" : "{copy}");
+  else chose_graph(OP, "shape");
+  return check_launch(OP);
+}
+
+size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_paged_cache* cache) {
+  (void)q, (void)cache;
+  return 0;
+}
+
+int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache, const svodb_tensor* start,
+                          const svodb_tensor* lens, const svodb_attn_opts* opts, svodb_tensor* o, void* stream) {
+  static const char* OP = "attention_paged";
+  GUARD(OP);
+  if (active_rows() != nullptr) return rows_unsupported(OP);
+  svodb_attn_opts none{};
+  if (opts == nullptr) opts = &none;
+  TRY(realized(OP, "q", q));
+  TRY(realized(OP, "o", o));
+  if (q->rank != 4) return shape_err(OP, "q", q, "[B, T, H, D]");
+  PagedAttnArgs a{};
+  TRY(paged_cache(OP, cache, q->shape[0], q->dtype, a.c));
+  const int64_t B = q->shape[0], T = q->shape[1], H = q->shape[2], D = q->shape[3];
+  TRY(chunk_rows(OP, "q", q, H, a.c.d, "[B, T, H, D], D of the cache"));
+  if (H > INT32_MAX || H % a.c.kv_heads != 0)
+    return fail(SVODB_ERR_HEADS, "%s: %lld query heads are not a multiple of %d key/value heads", OP, (long long)H, a.c.kv_heads);
+  if (!same_shape(o, q)) return shape_err(OP, "o", o, "[B, T, H, D]");
+  if (o->dtype != q->dtype) return dtype_err(OP, "o", o->dtype, q->dtype);
+  if (o->stride[3] != 1) return fail(SVODB_ERR_GRAPH, "%s: the head dim must be contiguous", OP);
+  for (int i = 0; i < 3; ++i)
+    if (o->stride[i] < 0) return fail(SVODB_ERR_GRAPH, "%s: o has negative strides", OP);
+  TRY(row_counts(OP, "start", start, B));
+  if (lens != nullptr) TRY(row_counts(OP, "lens", lens, B));
+  if (opts->key_lens != nullptr || opts->key_mask != nullptr)
+    return fail(SVODB_ERR_UNSUPPORTED, "%s: start and lens say which keys there are, no key mask does", OP);
+  if (opts->has_chunk || opts->seg_start != nullptr || opts->bias != nullptr || opts->has_cache || opts->splits > 1)
+    return fail(SVODB_ERR_UNSUPPORTED, "%s: chunks, segments, a bias, cache rows and key splits are not covered", OP);
+  if (opts->has_window && (opts->window_left < 0 || opts->window_right < 0))
+    return fail(SVODB_ERR_GRAPH, "%s: a window reaches 0 or more keys to either side", OP);
+  if (opts->lse != nullptr) {
+    TRY(realized(OP, "lse", opts->lse));
+    const svodb_tensor* l = opts->lse;
+    if (l->rank != 3 || l->shape[0] != B || l->shape[1] != H || l->shape[2] != T || !contiguous(l))
+      return shape_err(OP, "lse", l, "[B, H, T]");
+    if (l->dtype != SVODB_F32) return dtype_err(OP, "lse", l->dtype, SVODB_F32);
+  }
+  if (!apart(o)) return fail(SVODB_ERR_GRAPH, "%s: an output whose elements overlap", OP);
+  for (const svodb_tensor* out : {(const svodb_tensor*)o, (const svodb_tensor*)opts->lse})
+    TRY(no_alias(OP, out, {q, cache->k, cache->v, cache->k_scale, cache->v_scale, cache->table, start, lens}));
+  TRY(no_alias(OP, o, {opts->lse}));
+  if (B * T * H == 0) {
+    chose_graph(OP, "shape");
+    return SVODB_OK;
+  }
+  if (D > 256) return fail(SVODB_ERR_UNSUPPORTED, "%s: head dim %lld is above 256", OP, (long long)D);
+  if (B * T * H > INT32_MAX) return fail(SVODB_ERR_UNSUPPORTED, "%s: more than 2^31 query rows a call", OP);
+  a.q = q->data, a.o = o->data;
+  a.q_sb = q->stride[0], a.q_st = q->stride[1], a.q_sh = q->stride[2];
+  a.o_sb = o->stride[0], a.o_st = o->stride[1], a.o_sh = o->stride[2];
+  a.batch = B, a.t = T, a.heads = (int)H, a.dtype = q->dtype;
+  a.scale = opts->has_scale ? opts->scale : 1.0f / sqrtf((float)D);
+  a.causal = opts->causal;
+  a.has_window = opts->has_window;
+  // no position is 2^31 away: a wider window is none, and sums with it stay in range
+  a.win_left = opts->window_left > INT32_MAX ? INT32_MAX : opts->window_left;
+  a.win_right = opts->window_right > INT32_MAX ? INT32_MAX : opts->window_right;
+  a.start = (const int32_t*)start->data;
+  a.lens = lens != nullptr ? (const int32_t*)lens->data : nullptr;
+  a.lse = opts->lse ? (float*)opts->lse->data : nullptr;
+  a.status = device_status_word();
+  char cfg[128];
+  if (config_lookup("attention|exact") == 0 && attention_paged_decode_covers(a)) {
+    const int rc = launch_attention_paged_decode(a, (cudaStream_t)stream, cfg, sizeof cfg);
+    if (rc != 0) return fail(SVODB_ERR_LAUNCH, "%s: the tensor map or kernel attributes were rejected", OP);
+    chose_kernel(OP, "paged_decode", cfg);
+    return check_launch(OP);
+  }
+  launch_attention_paged_exact(a, (cudaStream_t)stream);
+  chose_graph(OP, is_half(a.dtype) ? "shape" : "dtype");
   return check_launch(OP);
 }
 

@@ -18,7 +18,7 @@ namespace svodb {
 enum : uint32_t {
   kStatusOk = 0,
   kStatusWaitTimeout = 1,
-  kStatusBadIndex = 2,  // a device-side index (a cache row map entry) was out of range
+  kStatusBadIndex = 2,  // a device-side index (a cache row map or page table entry) was out of range
 };
 
 // ---- dtype traits ----------------------------------------------------------

@@ -220,6 +220,73 @@ struct CombineArgs {
 };
 void launch_combine(const CombineArgs& a, cudaStream_t s);
 
+// ---- paged cache ----------------------------------------------------------------
+// A cache in pages (paged.cuh). Strides in elements; `sp` a page, `ss` a slot, `sh` a head.
+struct PagedCache {
+  void* k;
+  void* v;
+  int64_t k_sp, k_ss, k_sh;
+  int64_t v_sp, v_ss, v_sh;
+  uint8_t* k_scale;  // [pages, kv_heads, page_size], null without 8-bit pages; slots lie side by side
+  uint8_t* v_scale;
+  int64_t ks_sp, ks_sh, vs_sp, vs_sh;
+  const int32_t* table;  // [B, width]
+  int64_t table_sb;
+  int64_t width, pages;
+  int page_size, kv_heads, d;
+  int dtype;  // of the pages: SVODB_E4M3 or the stream type
+};
+struct CacheWriteArgs {
+  PagedCache c;
+  const void* k;  // [B, T, kv_heads, D]
+  const void* v;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  int64_t batch, t;
+  int dtype;
+  const int32_t* start;
+  const int32_t* lens;  // nullable
+  uint32_t* status;
+};
+// Returns 1 when the vector kernel ran, 0 when the one for every width and alignment did.
+int launch_cache_write(const CacheWriteArgs& a, cudaStream_t s);
+struct CacheReadArgs {
+  PagedCache c;
+  void* k;  // [B, L, kv_heads, D]
+  void* v;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  int64_t batch, len;
+  int dtype;
+  const int32_t* lens;
+  uint32_t* status;
+};
+int launch_cache_read(const CacheReadArgs& a, cudaStream_t s);
+struct PagedAttnArgs {
+  PagedCache c;
+  const void* q;  // [B, T, H, D]
+  void* o;
+  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+  int64_t batch, t;
+  int heads;
+  int dtype;
+  float scale;
+  int causal;
+  int has_window;
+  int64_t win_left, win_right;
+  const int32_t* start;
+  const int32_t* lens;  // nullable
+  float* lse;           // [B, H, T], nullable
+  uint32_t* status;
+};
+// Every float type, head width up to 256, page size and alignment.
+int launch_attention_paged_exact(const PagedAttnArgs& a, cudaStream_t s);
+// What the tensor-core kernels over pages take in common.
+bool attention_paged_tiles(const PagedAttnArgs& a);
+// Up to 64 query rows a KV head: keys as the M of both MMAs.
+bool attention_paged_decode_covers(const PagedAttnArgs& a);
+int launch_attention_paged_decode(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len);
+// Keys of the largest run that divides a page and `most`: no box of that many straddles pages.
+int page_box(int page_size, int most);
+
 // ---- GEMM ---------------------------------------------------------------------
 struct GemmArgs {
   const void* a;  // [M,K], row stride lda

@@ -1,0 +1,420 @@
+// A paged key/value cache: new tokens written into its pages (as they are or in 8 bits),
+// pages read back into rows, and attention over the pages for every type, width and page
+// size (`attention_paged_exact`; the tensor-core kernels are in their own files).
+//
+// Write and read move every byte once and are bound by HBM, or by the chain
+// start -> table -> page of dependent loads where there is little to move. A lane owns 16
+// elements of a head row: two 16-byte accesses on the 16-bit side, one on the 8-bit side;
+// a row's D / 16 lanes find its largest value among themselves.
+#include <math.h>
+
+#include <initializer_list>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.h"
+#include "paged.cuh"
+#include "svodb.h"
+
+namespace svodb {
+
+namespace {
+
+using namespace paged;
+
+constexpr int kThreadsPaged = 256;
+
+// The slot of position `pos` of row b: {page, slot}; page < 0 when the table's entry is none.
+__device__ __forceinline__ int64_t page_of(const PagedCache& c, int64_t b, int64_t page, uint32_t* status) {
+  const int32_t id = c.table[b * c.table_sb + page];
+  if (id < 0 || id >= c.pages) {
+    atomicExch(status, (uint32_t)kStatusBadIndex);
+    return -1;
+  }
+  return id;
+}
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, uint4 (&u)[2]) {
+  u[0] = ldg128(p);
+  u[1] = ldg128(p + 8);
+}
+template <typename T>
+__device__ __forceinline__ void widen16(const uint4 (&u)[2], float (&f)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w = i < 4 ? (i == 0 ? u[0].x : i == 1 ? u[0].y : i == 2 ? u[0].z : u[0].w)
+                             : (i == 4 ? u[1].x : i == 5 ? u[1].y : i == 6 ? u[1].z : u[1].w);
+    const float2 v = Elem<T>::unpack(w);
+    f[2 * i] = v.x, f[2 * i + 1] = v.y;
+  }
+}
+
+// One token's head row a group of LPR lanes; blockIdx.y: keys or values.
+template <typename T, bool Q8, int LPR>
+__global__ void __launch_bounds__(kThreadsPaged) cache_write_kernel(const CacheWriteArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const bool is_v = blockIdx.y != 0;
+  const int64_t g = (int64_t)blockIdx.x * kThreadsPaged + threadIdx.x;
+  const int64_t rows = a.batch * a.t * a.c.kv_heads;
+  const int64_t row = g / LPR;
+  const int sub = (int)(g % LPR);
+  const bool live = row < rows;
+  const int64_t token = live ? row / a.c.kv_heads : 0;
+  const int h = live ? (int)(row % a.c.kv_heads) : 0;
+  const int64_t b = token / a.t, i = token % a.t;
+  const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
+  const bool real = live && i < r.n;
+  uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  int64_t page = -1;
+  int slot = 0;
+  if (real) {
+    load16<T>(is_v ? (const T*)a.v + b * a.v_sb + i * a.v_st + h * a.v_sh + sub * 16
+                   : (const T*)a.k + b * a.k_sb + i * a.k_st + h * a.k_sh + sub * 16, u);
+    const int64_t pos = r.start + i;
+    const int64_t at = pos / a.c.page_size;
+    slot = (int)(pos - at * a.c.page_size);
+    page = page_of(a.c, b, at, a.status);
+  }
+  if (r.bad && live && i == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  const int64_t to = is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh;
+  if constexpr (!Q8) {
+    if (page < 0) return;
+    T* dst = (T*)(is_v ? a.c.v : a.c.k) + to + sub * 16;
+    stg128(dst, u[0]);
+    stg128(dst + 8, u[1]);
+  } else {
+    float f[16];
+    widen16<T>(u, f);
+    // the largest as an integer: a NaN's bits are above every number's, and stay so
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (page < 0) return;
+    const uint32_t code = scale_code(__uint_as_float(top));
+    const float inv = code == 255u ? 0.f : scale_inverse(code);
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t lo = to_e4m3x2(f[4 * e] * inv, f[4 * e + 1] * inv), hi = to_e4m3x2(f[4 * e + 2] * inv, f[4 * e + 3] * inv);
+      w[e] = code == 255u ? 0u : lo | (hi << 16);
+    }
+    stg128((uint8_t*)(is_v ? a.c.v : a.c.k) + to + sub * 16, make_uint4(w[0], w[1], w[2], w[3]));
+    if (sub == 0) {
+      if (is_v) a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] = (uint8_t)code;
+      else a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot] = (uint8_t)code;
+    }
+  }
+}
+
+// The same for every width and alignment: a warp a head row.
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(kThreadsPaged) cache_write_any_kernel(const CacheWriteArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const bool is_v = blockIdx.y != 0;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * (kThreadsPaged / 32) + (threadIdx.x >> 5);
+  if (row >= a.batch * a.t * a.c.kv_heads) return;
+  const int64_t token = row / a.c.kv_heads;
+  const int h = (int)(row % a.c.kv_heads);
+  const int64_t b = token / a.t, i = token % a.t;
+  const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
+  if (r.bad && i == 0 && lane == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (i >= r.n) return;
+  const int64_t pos = r.start + i, at = pos / a.c.page_size;
+  const int slot = (int)(pos - at * a.c.page_size);
+  const int64_t page = page_of(a.c, b, at, a.status);
+  if (page < 0) return;
+  const T* src = is_v ? (const T*)a.v + b * a.v_sb + i * a.v_st + h * a.v_sh : (const T*)a.k + b * a.k_sb + i * a.k_st + h * a.k_sh;
+  const int64_t to = is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh;
+  void* base = is_v ? a.c.v : a.c.k;
+  if constexpr (!Q8) {
+    for (int e = lane; e < a.c.d; e += 32) ((T*)base)[to + e] = src[e];
+  } else {
+    uint32_t top = 0;
+    for (int e = lane; e < a.c.d; e += 32) top = max(top, __float_as_uint(Elem<T>::to_f(src[e])) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t code = scale_code(__uint_as_float(top));
+    const float inv = code == 255u ? 0.f : scale_inverse(code);
+    for (int e = lane; e < a.c.d; e += 32)
+      ((uint8_t*)base)[to + e] = code == 255u ? 0 : (uint8_t)(to_e4m3x2(Elem<T>::to_f(src[e]) * inv, 0.f) & 0xffu);
+    if (lane == 0) {
+      if (is_v) a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] = (uint8_t)code;
+      else a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot] = (uint8_t)code;
+    }
+  }
+}
+
+// Sixteen e4m3 values times their scale, rounded to the stream type.
+template <typename T>
+__device__ __forceinline__ void widen_e4m3(uint4 u, float scale, uint32_t (&w)[8]) {
+  const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 lo = from_e4m3x2(in[e] & 0xffffu), hi = from_e4m3x2(in[e] >> 16);
+    w[2 * e] = Elem<T>::pack(lo.x * scale, lo.y * scale);
+    w[2 * e + 1] = Elem<T>::pack(hi.x * scale, hi.y * scale);
+  }
+}
+
+template <typename T, bool Q8, int LPR>
+__global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheReadArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const bool is_v = blockIdx.y != 0;
+  const int64_t g = (int64_t)blockIdx.x * kThreadsPaged + threadIdx.x;
+  const int64_t row = g / LPR;
+  const int sub = (int)(g % LPR);
+  if (row >= a.batch * a.len * a.c.kv_heads) return;
+  const int64_t token = row / a.c.kv_heads;
+  const int h = (int)(row % a.c.kv_heads);
+  const int64_t b = token / a.len, pos = token % a.len;
+  const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
+  if (r.bad && pos == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  uint32_t w[8] = {};
+  if (pos < r.n) {
+    const int64_t at = pos / a.c.page_size;
+    const int slot = (int)(pos - at * a.c.page_size);
+    const int64_t page = page_of(a.c, b, at, a.status);
+    if (page >= 0) {
+      const int64_t from = (is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh) + sub * 16;
+      if constexpr (Q8) {
+        const uint4 u = ldg128((const uint8_t*)(is_v ? a.c.v : a.c.k) + from);
+        const uint32_t code = is_v ? a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] : a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot];
+        widen_e4m3<T>(u, scale_value(code), w);
+      } else {
+        uint4 u[2];
+        load16<T>((const T*)(is_v ? a.c.v : a.c.k) + from, u);
+        w[0] = u[0].x, w[1] = u[0].y, w[2] = u[0].z, w[3] = u[0].w;
+        w[4] = u[1].x, w[5] = u[1].y, w[6] = u[1].z, w[7] = u[1].w;
+      }
+    }
+  }
+  T* dst = is_v ? (T*)a.v + b * a.v_sb + pos * a.v_st + h * a.v_sh + sub * 16 : (T*)a.k + b * a.k_sb + pos * a.k_st + h * a.k_sh + sub * 16;
+  stg128(dst, make_uint4(w[0], w[1], w[2], w[3]));
+  stg128(dst + 8, make_uint4(w[4], w[5], w[6], w[7]));
+}
+
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(kThreadsPaged) cache_read_any_kernel(const CacheReadArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const bool is_v = blockIdx.y != 0;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * (kThreadsPaged / 32) + (threadIdx.x >> 5);
+  if (row >= a.batch * a.len * a.c.kv_heads) return;
+  const int64_t token = row / a.c.kv_heads;
+  const int h = (int)(row % a.c.kv_heads);
+  const int64_t b = token / a.len, pos = token % a.len;
+  const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
+  if (r.bad && pos == 0 && lane == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  int64_t page = -1, from = 0;
+  float scale = 0.f;
+  if (pos < r.n) {
+    const int64_t at = pos / a.c.page_size;
+    const int slot = (int)(pos - at * a.c.page_size);
+    page = page_of(a.c, b, at, a.status);
+    if (page >= 0) {
+      from = is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh;
+      if constexpr (Q8) scale = scale_value(is_v ? a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] : a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot]);
+    }
+  }
+  T* dst = is_v ? (T*)a.v + b * a.v_sb + pos * a.v_st + h * a.v_sh : (T*)a.k + b * a.k_sb + pos * a.k_st + h * a.k_sh;
+  const void* base = is_v ? a.c.v : a.c.k;
+  for (int e = lane; e < a.c.d; e += 32) {
+    if (page < 0) dst[e] = Elem<T>::from_f(0.f);
+    else if constexpr (Q8) dst[e] = Elem<T>::from_f(from_e4m3x2(((const uint8_t*)base)[from + e]).x * scale);
+    else dst[e] = ((const T*)base)[from + e];
+  }
+}
+
+// ---- exact attention -------------------------------------------------------------
+// A block a query row and head; its four warps take every fourth visible key, lanes hold
+// the head's elements d = lane + 32 i, and the four running states meet in shared memory.
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedAttnArgs a) {
+  constexpr int kMaxD = 256, kPer = kMaxD / 32, kWarps = 4;
+  __shared__ float o_s[kWarps][kMaxD];
+  __shared__ float m_s[kWarps], l_s[kWarps];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t item = blockIdx.x;
+  const int h = (int)(item % a.heads);
+  const int64_t i = item / a.heads % a.t, b = item / a.heads / a.t;
+  const int hk = h / (a.heads / a.c.kv_heads), d = a.c.d;
+  const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
+  if (r.bad && i == 0 && h == 0 && threadIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  const int64_t pos = r.start + i;
+  int64_t lo = 0, hi = r.start + r.n;
+  if (a.causal && pos + 1 < hi) hi = pos + 1;
+  if (a.has_window) {
+    if (pos - a.win_left > lo) lo = pos - a.win_left;
+    if (pos + a.win_right + 1 < hi) hi = pos + a.win_right + 1;
+  }
+  if (i >= r.n) hi = lo;
+  float q[kPer], o[kPer];
+  const T* qp = (const T*)a.q + b * a.q_sb + i * a.q_st + h * a.q_sh;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    q[e] = lane + 32 * e < d ? Elem<T>::to_f(qp[lane + 32 * e]) : 0.f;
+    o[e] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  for (int64_t j = lo + warp; j < hi; j += kWarps) {
+    const int64_t at = j / a.c.page_size;
+    const int slot = (int)(j - at * a.c.page_size);
+    const int64_t page = page_of(a.c, b, at, a.status);
+    if (page < 0) continue;
+    const int64_t fk = page * a.c.k_sp + slot * a.c.k_ss + hk * a.c.k_sh, fv = page * a.c.v_sp + slot * a.c.v_ss + hk * a.c.v_sh;
+    float ks = 1.f, vs = 1.f;
+    if constexpr (Q8) {
+      ks = scale_value(a.c.k_scale[page * a.c.ks_sp + hk * a.c.ks_sh + slot]);
+      vs = scale_value(a.c.v_scale[page * a.c.vs_sp + hk * a.c.vs_sh + slot]);
+    }
+    float s = 0.f, v[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int c = lane + 32 * e;
+      v[e] = 0.f;
+      if (c < d) {
+        if constexpr (Q8) {
+          s = fmaf(q[e], from_e4m3x2(((const uint8_t*)a.c.k)[fk + c]).x * ks, s);
+          v[e] = from_e4m3x2(((const uint8_t*)a.c.v)[fv + c]).x * vs;
+        } else {
+          s = fmaf(q[e], Elem<T>::to_f(((const T*)a.c.k)[fk + c]), s);
+          v[e] = Elem<T>::to_f(((const T*)a.c.v)[fv + c]);
+        }
+      }
+    }
+    s = warp_sum(s) * a.scale;
+    const float m_new = fmaxf(m, s), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float corr = m == -INFINITY ? 0.f : expf(m - m_use), p = expf(s - m_use);
+    l = fmaf(l, m == -INFINITY ? 1.f : corr, p);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = fmaf(o[e], m == -INFINITY ? 1.f : corr, p * v[e]);
+    m = m_new;
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) o_s[warp][lane + 32 * e] = o[e];
+  if (lane == 0) m_s[warp] = m, l_s[warp] = l;
+  __syncthreads();
+  float top = -INFINITY, total = 0.f, w[kWarps];
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) top = fmaxf(top, m_s[k]);
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) {
+    w[k] = l_s[k] == 0.f ? 0.f : m_s[k] == -INFINITY ? 1.f : expf(m_s[k] - top);
+    total = fmaf(w[k], l_s[k], total);
+  }
+  T* op = (T*)a.o + b * a.o_sb + i * a.o_st + h * a.o_sh;
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  for (int c = threadIdx.x; c < d; c += 128) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k)
+      if (l_s[k] != 0.f) x = fmaf(w[k], o_s[k][c], x);
+    op[c] = Elem<T>::from_f(x * inv);
+  }
+  if (a.lse != nullptr && threadIdx.x == 0) a.lse[(b * a.heads + h) * a.t + i] = total == 0.f ? -INFINITY : top + logf(total);
+}
+
+int lanes_a_row(int d) {
+  if (d % 16 != 0 || d > 512) return 0;
+  const int l = d / 16;
+  return (l & (l - 1)) == 0 ? l : 0;
+}
+bool on_grid(const void* p, std::initializer_list<int64_t> strides, int64_t size) {
+  if (!aligned16(p)) return false;
+  for (int64_t s : strides)
+    if (s * size % 16 != 0) return false;
+  return true;
+}
+bool pages_on_grid(const PagedCache& c) {
+  const int64_t size = c.dtype == SVODB_E4M3 ? 1 : c.dtype == SVODB_F32 ? 4 : 2;
+  return on_grid(c.k, {c.k_sp, c.k_ss, c.k_sh}, size) && on_grid(c.v, {c.v_sp, c.v_ss, c.v_sh}, size);
+}
+
+unsigned blocks_of(int64_t n, int64_t per) { return (unsigned)((n + per - 1) / per); }
+
+template <typename T, bool Q8>
+int run_write(const CacheWriteArgs& a, cudaStream_t s) {
+  const int64_t rows = a.batch * a.t * a.c.kv_heads;
+  const int lpr = lanes_a_row(a.c.d);
+  if constexpr (!std::is_same<T, float>::value) {
+    if (lpr != 0 && pages_on_grid(a.c) && on_grid(a.k, {a.k_sb, a.k_st, a.k_sh}, 2) && on_grid(a.v, {a.v_sb, a.v_st, a.v_sh}, 2)) {
+      const dim3 grid(blocks_of(rows * lpr, kThreadsPaged), 2), block(kThreadsPaged);
+      const int64_t pdl = a.batch * a.t;
+      switch (lpr) {
+        case 1: launch_pdl(cache_write_kernel<T, Q8, 1>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 2: launch_pdl(cache_write_kernel<T, Q8, 2>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 4: launch_pdl(cache_write_kernel<T, Q8, 4>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 8: launch_pdl(cache_write_kernel<T, Q8, 8>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 16: launch_pdl(cache_write_kernel<T, Q8, 16>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 32: launch_pdl(cache_write_kernel<T, Q8, 32>, grid, block, 0, s, 1, pdl, a); return 1;
+      }
+    }
+  }
+  launch_pdl(cache_write_any_kernel<T, Q8>, dim3(blocks_of(rows, kThreadsPaged / 32), 2), dim3(kThreadsPaged), 0, s, 1, a.batch * a.t, a);
+  return 0;
+}
+
+template <typename T, bool Q8>
+int run_read(const CacheReadArgs& a, cudaStream_t s) {
+  const int64_t rows = a.batch * a.len * a.c.kv_heads;
+  const int lpr = lanes_a_row(a.c.d);
+  if constexpr (!std::is_same<T, float>::value) {
+    if (lpr != 0 && pages_on_grid(a.c) && on_grid(a.k, {a.k_sb, a.k_st, a.k_sh}, 2) && on_grid(a.v, {a.v_sb, a.v_st, a.v_sh}, 2)) {
+      const dim3 grid(blocks_of(rows * lpr, kThreadsPaged), 2), block(kThreadsPaged);
+      const int64_t pdl = a.batch * a.len;
+      switch (lpr) {
+        case 1: launch_pdl(cache_read_kernel<T, Q8, 1>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 2: launch_pdl(cache_read_kernel<T, Q8, 2>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 4: launch_pdl(cache_read_kernel<T, Q8, 4>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 8: launch_pdl(cache_read_kernel<T, Q8, 8>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 16: launch_pdl(cache_read_kernel<T, Q8, 16>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 32: launch_pdl(cache_read_kernel<T, Q8, 32>, grid, block, 0, s, 1, pdl, a); return 1;
+      }
+    }
+  }
+  launch_pdl(cache_read_any_kernel<T, Q8>, dim3(blocks_of(rows, kThreadsPaged / 32), 2), dim3(kThreadsPaged), 0, s, 1, a.batch * a.len, a);
+  return 0;
+}
+
+// `f` with the stream type and whether the pages hold 8 bits.
+template <typename F>
+int by_type(int dtype, bool q8, F&& f) {
+  switch (dtype) {
+    case SVODB_BF16: return q8 ? f(__nv_bfloat16{}, std::true_type{}) : f(__nv_bfloat16{}, std::false_type{});
+    case SVODB_F16: return q8 ? f(__half{}, std::true_type{}) : f(__half{}, std::false_type{});
+    default: return q8 ? f(float{}, std::true_type{}) : f(float{}, std::false_type{});
+  }
+}
+
+}  // namespace
+
+int launch_cache_write(const CacheWriteArgs& a, cudaStream_t s) {
+  return by_type(a.dtype, a.c.dtype == SVODB_E4M3,
+                 [&](auto t, auto q8) { return run_write<decltype(t), decltype(q8)::value>(a, s); });
+}
+
+int launch_cache_read(const CacheReadArgs& a, cudaStream_t s) {
+  return by_type(a.dtype, a.c.dtype == SVODB_E4M3,
+                 [&](auto t, auto q8) { return run_read<decltype(t), decltype(q8)::value>(a, s); });
+}
+
+int launch_attention_paged_exact(const PagedAttnArgs& a, cudaStream_t s) {
+  return by_type(a.dtype, a.c.dtype == SVODB_E4M3, [&](auto t, auto q8) {
+    launch_pdl(attention_paged_exact_kernel<decltype(t), decltype(q8)::value>, dim3((unsigned)(a.batch * a.t * a.heads)),
+               dim3(128), 0, s, 1, a.batch * a.t, a);
+    return 0;
+  });
+}
+
+}  // namespace svodb

@@ -38,6 +38,7 @@ bool make_tmap(CUtensorMap* map, const void* base, int dtype, int rank, const ui
     case SVODB_BF16: dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, esize = 2; break;
     case SVODB_F16: dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT16, esize = 2; break;
     case SVODB_F32: dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT32, esize = 4; break;
+    case SVODB_E4M3: dt = CU_TENSOR_MAP_DATA_TYPE_UINT8, esize = 1; break;
     default: return false;
   }
   cuuint64_t gdim[5], gstride[4];

@@ -7,7 +7,7 @@
 
 namespace svodb {
 
-// A tiled map over a dense tensor of 16-bit (or 32-bit) elements with the
+// A tiled map over a dense tensor of 16-bit (or 32-bit, or e4m3) elements with the
 // 128-byte shared-memory swizzle. `dims` are innermost first; `strides` are the
 // element strides of dims 1..rank-1 (dim 0 is contiguous); out-of-bounds
 // elements read as zero. Returns false (with `svodb_last_error` set by the
@@ -19,5 +19,9 @@ bool make_tmap(CUtensorMap* map, const void* base, int dtype, int rank, const ui
 // [rows, inner] row-major with `row_stride` elements between rows; box = box_rows x box_inner.
 bool make_tmap_2d(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t row_stride,
                   uint32_t box_inner, uint32_t box_rows);
+
+struct PagedCache;  // kernels.h
+// The keys' (or values') pages [pages, page_size, kv_heads, D]: boxes of `rows` slots x `cols` elements of a head.
+bool page_map(CUtensorMap* map, const PagedCache& c, bool values, uint32_t cols, uint32_t rows);
 
 }  // namespace svodb

@@ -146,21 +146,22 @@ _DTYPES = {
     torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16,
     torch.int32: L.I32, torch.int64: L.I64, torch.uint8: L.U8, torch.bool: L.U8,
 }
+_PAGE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: L.E4M3, torch.float8_e8m0fnu: L.E8M0}
 
 
-def _desc(t: Optional[torch.Tensor]):
+def _desc(t: Optional[torch.Tensor], dtypes=_DTYPES):
     """The `svodb_tensor` of a CUDA tensor, or a null pointer."""
     if t is None:
         return None
     if not t.is_cuda:
         raise OpsError(L.ERR_UNREALIZED, "operand is not a realized device buffer")
-    if t.dtype not in _DTYPES:
+    if t.dtype not in dtypes:
         raise OpsError(L.ERR_DTYPE, f"unsupported element type {t.dtype}")
     if t.dim() > L.MAX_RANK:
         raise OpsError(L.ERR_SHAPE, f"rank {t.dim()} is above {L.MAX_RANK}")
     d = L.Tensor()
     d.data = t.data_ptr()
-    d.dtype = _DTYPES[t.dtype]
+    d.dtype = dtypes[t.dtype]
     d.rank = t.dim()
     for i, (s, st) in enumerate(zip(t.shape, t.stride())):
         d.shape[i] = s
@@ -420,6 +421,132 @@ def combine_splits(o_part: torch.Tensor, m_part: torch.Tensor, l_part: torch.Ten
     a, b, c, d = _desc(o_part), _desc(m_part), _desc(l_part), _desc(out)
     _check(L.load().svodb_combine_splits(_p(a), _p(b), _p(c), _p(d), _stream()))
     return out
+
+
+# ---------------------------------------------------------------------- paged cache
+@dataclass
+class PagedCache:
+    """Keys and values in pages (no counterpart in the reference, whose caches are rows of
+    one length): `k`, `v` `[pages, page_size, kv_heads, D]` in the stream type, or in
+    `float8_e4m3fn` beside one power of two a token and head, `k_scale`, `v_scale`
+    `[pages, kv_heads, page_size]` `float8_e8m0fnu`. Position `p` of sequence `b` lies in
+    slot `p % page_size` of page `table[b, p // page_size]`; the ops take the `[B, width]`
+    i32 `table` of the batch at hand, whose entries behind a sequence's last page mean
+    nothing. Any view with a contiguous head dim will do (one layer of a larger buffer)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def empty(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16, quantized: bool = False,
+              device="cuda") -> "PagedCache":
+        """Pages with nothing in them, in 8 bits where `quantized`."""
+        mk = lambda: torch.zeros(pages, page_size, kv_heads, head_dim, device=device,
+                                 dtype=torch.float8_e4m3fn if quantized else dtype)
+        scale = lambda: (torch.zeros(pages, kv_heads, page_size, dtype=torch.uint8, device=device)
+                         .view(torch.float8_e8m0fnu) if quantized else None)
+        return PagedCache(mk(), mk(), scale(), scale())
+
+
+def _i32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+
+
+def _paged(cache: PagedCache, table: torch.Tensor, keep: list):
+    c = L.PagedCache()
+    if table.dtype != torch.int32 or (table.dim() == 2 and table.shape[1] > 1 and table.stride(1) != 1):
+        table = table.to(torch.int32).contiguous()
+    keep.append(table)
+    for name, t in (("k", cache.k), ("v", cache.v), ("k_scale", cache.k_scale), ("v_scale", cache.v_scale), ("table", table)):
+        if t is not None:
+            keep.append(_desc(t, _PAGE_DTYPES))
+            setattr(c, name, C.pointer(keep[-1]))
+    return c
+
+
+def _one_device(first: torch.Tensor, *others) -> int:
+    """The device of all operands of a call: kernels run there, on its current stream,
+    whatever the thread's current device is."""
+    if not first.is_cuda:
+        raise OpsError(L.ERR_UNREALIZED, "operand is not a realized device buffer")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise OpsError(L.ERR_UNREALIZED, f"operands on {first.device} and {t.device}")
+    return first.device.index
+
+
+def cache_write(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, table: torch.Tensor, start: torch.Tensor,
+                lens: Optional[torch.Tensor] = None) -> None:
+    """Writes a chunk `k`, `v` `[B, T, kv_heads, D]` into the pages: row `b`'s first
+    `lens[b]` tokens (all T without `lens`) become positions `start[b]` and on of sequence
+    `b`. 8-bit pages: a token's head row gets the scale `2^e`, `e` the least with
+    `max|x| <= 448 * 2^e`, and holds `round(x / 2^e)`; a row with a NaN or an infinity reads
+    back as NaN. Other slots stay as they are; two tokens of one call in the same slot leave
+    either. Rows that leave the table and entries that are no page write nothing, and
+    `device_status()` raises."""
+    dev = _one_device(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, table, start, lens)
+    with torch.cuda.device(dev):
+        keep: list = []
+        start, lens = _i32(start), _i32(lens)
+        c = _paged(cache, table, keep)
+        kd, vd, sd, ld = _desc(k), _desc(v), _desc(start), _desc(lens)
+        _check(L.load().svodb_cache_write(_p(kd), _p(vd), C.byref(c), _p(sd), _p(ld), _stream()))
+
+
+def cache_read(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, length: Optional[int] = None, dtype=None):
+    """`(k, v)` `[B, length, kv_heads, D]` of the sequences under `table`: the first
+    `lens[b]` positions of row `b`, zeros behind them. `length` defaults to what the table
+    reaches; `dtype` is the pages' own, for 8-bit pages any float type (bf16 by default;
+    value times scale, rounded once)."""
+    dev = _one_device(cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens)
+    if cache.k.dim() != 4 or table.dim() != 2:
+        raise OpsError(L.ERR_SHAPE, f"cache_read: cache k has shape {list(cache.k.shape)}, table {list(table.shape)}, expected "
+                                    "[pages, page_size, kv_heads, D] and [B, width]")
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
+    if length is None:
+        length = table.shape[1] * cache.k.shape[1]
+    with torch.cuda.device(dev):
+        keep: list = []
+        lens = _i32(lens)
+        c = _paged(cache, table, keep)
+        k = torch.empty(table.shape[0], length, *cache.k.shape[2:], dtype=dtype, device=cache.k.device)
+        v = torch.empty_like(k)
+        ld, kd, vd = _desc(lens), _desc(k), _desc(v)
+        _check(L.load().svodb_cache_read(C.byref(c), _p(ld), _p(kd), _p(vd), _stream()))
+    return k, v
+
+
+def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, start: torch.Tensor,
+                    lens: Optional[torch.Tensor] = None, opts: Optional[Attn] = None):
+    """Attention of a chunk over the pages it was written to: `q [B,T,H,D]` -> `[B,T,H,D]`
+    (and `lse` when `opts.want_lse`). Query `i` of row `b` stands at position `start[b] + i`
+    and sees the `start[b] + lens[b]` keys of its sequence (T without `lens`), under
+    `opts.causal` (the default without `opts`) those up to its own position, under
+    `opts.window` those near it. One token a row is a decoding step, `start` zeros a prompt.
+    Rows from `lens[b]` on and rows that see no key are zeros. Other options are refused."""
+    dev = _one_device(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, start, lens)
+    if q.dim() != 4:
+        raise OpsError(L.ERR_SHAPE, f"attention_paged: q has shape {list(q.shape)}, expected [B, T, H, D]")
+    opts = opts or Attn(causal=True)
+    with torch.cuda.device(dev):
+        keep: list = []
+        start, lens = _i32(start), _i32(lens)
+        c = _paged(cache, table, keep)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if opts.splits is not None and opts.splits > 1:
+            raise OpsError(L.ERR_UNSUPPORTED, "attention_paged: the split of the keys is the kernel's own")
+        o, lse = _attn_opts(opts, q.shape, q.dtype, q.device, keep)
+        qd, sd, ld, od = _desc(q), _desc(start), _desc(lens), _desc(out)
+        lib = L.load()
+        need = lib.svodb_attention_paged_workspace_bytes(_p(qd), C.byref(c))
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            keep.append(ws)
+            o.workspace, o.workspace_bytes = ws.data_ptr(), need
+        _check(lib.svodb_attention_paged(_p(qd), C.byref(c), _p(sd), _p(ld), C.byref(o), _p(od), _stream()))
+    return (out, lse) if opts.want_lse else out
 
 
 # ---------------------------------------------------------------------------- heads

@@ -1,0 +1,444 @@
+"""The paged cache on the GPU: writing, reading back and attention over the pages against
+64 bits, at the sizes, masks and layouts where they can go wrong. Slots that hold no token
+are NaN throughout, table entries that mean nothing name no page."""
+import math
+
+import pytest
+import torch
+
+from svod_b200 import ops
+from svod_b200 import _lib as L
+from tests.paged_reference import Case, EPS, quantise, stored
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [(BF16, False), (BF16, True), (F16, False), (F16, True)]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def cache_of(c):
+    up = lambda t: None if t is None else t.cuda()
+    return ops.PagedCache(up(c.k), up(c.v), up(c.ks), up(c.vs))
+
+
+def raw(t):
+    return t.view(torch.uint8) if t.element_size() == 1 else t.view(torch.int16 if t.element_size() == 2 else torch.int32)
+
+
+def attend(c, opts=None, cache=None, q=None, lens=True):
+    return ops.attention_paged(c.q.cuda() if q is None else q, cache or cache_of(c), c.table.cuda(), i32(c.held),
+                               i32(c.new) if lens else None, opts)
+
+
+def check(got, c, **mask):
+    ops.device_status()
+    want, lse, bound = c.attention(**mask)
+    off = (got.double().cpu() - want).abs()
+    assert torch.isfinite(got.float()).all()
+    worst = (off / bound.clamp(min=2.0 ** -40)).max() if off.numel() else 0.0
+    assert worst <= 1.0, float(worst)
+    for b, n in enumerate(c.new):
+        assert (got[b, n:] == 0).all()
+    return lse
+
+
+# ------------------------------------------------------------------------------ write, read
+@pytest.mark.parametrize("dtype,quantized", TYPES + [(F32, False), (F32, True)])
+@pytest.mark.parametrize("heads,d,page", [(2, 128, 16), (3, 64, 32), (1, 80, 48), (2, 40, 7), (1, 256, 1), (5, 16, 128),
+                                          (1, 13, 5), (2, 512, 8)])
+def test_write_is_the_definition(dtype, quantized, heads, d, page):
+    c = Case(d + page, 4, 9, [0, 5, page, 3 * page + 1], [9, 0, 4, 1], heads, heads, d, page, dtype, quantized)
+    cache = cache_of(c)
+    fill = lambda xs: torch.stack([torch.nn.functional.pad(x[h:h + n], (0, 0, 0, 0, 0, 9 - n)) for x, h, n in zip(xs, c.held, c.new)]).cuda()
+    ops.cache_write(fill(c.keys), fill(c.values), cache, c.table.cuda(), i32(c.held), i32(c.new))
+    ops.device_status()
+    c.put(c.held, [h + n for h, n in zip(c.held, c.new)])
+    for got, want in ((cache.k, c.k), (cache.v, c.v), (cache.k_scale, c.ks), (cache.v_scale, c.vs)):
+        if want is not None:
+            assert torch.equal(raw(got.cpu()), raw(want))  # every other slot as it was, to the bit
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_write_8_bits_of_odd_values(dtype):
+    """Rows of zeros, of one value, at the borders of a power of two, tiny, huge, with NaN
+    and infinities; -0.0 and values that round to the smallest step."""
+    d = 64
+    top = torch.finfo(dtype).max
+    rows = [torch.zeros(d), torch.full((d,), 448.0), torch.full((d,), -449.0 if dtype == F16 else -450.0),
+            torch.linspace(-1, 1, d), torch.full((d,), torch.finfo(dtype).tiny), torch.linspace(0, top, d),
+            torch.tensor([1.0] * 63 + [math.nan]), torch.tensor([1.0] * 63 + [math.inf]), torch.tensor([-math.inf] + [0.0] * 63),
+            torch.tensor([448.0] + [2.0 ** -k for k in range(1, 64)]), torch.tensor([1.75] + [-0.0] * 63),
+            torch.tensor([1.7578125] + [0.25] * 63), torch.full((d,), 2.0 ** -24)]
+    x = torch.stack(rows).to(dtype).view(1, len(rows), 1, d)
+    cache = ops.PagedCache.empty(2, 16, 1, d, dtype, quantized=True)
+    ops.cache_write(x.cuda(), x.flip(1).cuda(), cache, i32([[1]]), i32([2]))
+    ops.device_status()
+    v, e = quantise(x[0, :, 0])
+    assert torch.equal(cache.k_scale.cpu()[1, 0, 2:2 + len(rows)].view(torch.uint8).double(), e + 127)
+    got = cache.k.cpu()[1, 2:2 + len(rows), 0].double()
+    assert torch.equal(got, v)
+    assert torch.equal(cache.v.cpu()[1, 2:2 + len(rows), 0].double(), v.flip(0))
+    k, _ = ops.cache_read(cache, i32([[1]]), i32([2 + len(rows)]), dtype=dtype)
+    want = stored(x[0, :, 0], dtype, True).to(dtype)
+    assert torch.equal(k[0, 2:, 0].cpu()[:len(rows)].nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES + [(F32, False), (F32, True)])
+@pytest.mark.parametrize("heads,d,page", [(2, 128, 16), (3, 64, 32), (1, 80, 48), (2, 40, 7), (1, 256, 1), (1, 13, 5)])
+def test_read_is_the_definition(dtype, quantized, heads, d, page):
+    held = [0, 1, page, 2 * page + 3]
+    c = Case(page + d, 4, 1, held, [0] * 4, heads, heads, d, page, dtype, quantized)
+    c.put([0] * 4, held)
+    length = max(held) + 5
+    k, v = ops.cache_read(cache_of(c), c.table.cuda(), i32(held), length, dtype)
+    ops.device_status()
+    assert k.dtype == dtype and k.shape == (4, length, heads, d)
+    for b, n in enumerate(held):
+        assert torch.equal(k[b, :n].cpu(), stored(c.keys[b], dtype, quantized).to(dtype))
+        assert torch.equal(v[b, :n].cpu(), stored(c.values[b], dtype, quantized).to(dtype))
+        assert (k[b, n:] == 0).all() and (v[b, n:] == 0).all()
+
+
+def test_layers_of_one_buffer_and_views():
+    """A layer, a slice of the heads and keys beside values of one buffer; strided new rows."""
+    big = torch.full((3, 10, 16, 2, 6, 64), math.nan, dtype=BF16, device="cuda")  # layer, page, slot, k | v, head
+    view = ops.PagedCache(big[1, :, :, 0, 2:5], big[1, :, :, 1, 2:5])
+    qkv = torch.randn(2, 20, 12 * 64, device="cuda").to(BF16).view(2, 20, 12, 64)
+    table = i32([[9, 3, 0, 0, 0, 1], [4, 5, 0, 0, 0, 1]])[:, :2]
+    before = big.clone()
+    ops.cache_write(qkv[:, :, 6:9], qkv[:, :, 9:12], view, table, i32([1, 0]))
+    k, v = ops.cache_read(view, table, i32([21, 20]), 21)
+    ops.device_status()
+    assert torch.equal(k[1, :20], qkv[1, :, 6:9]) and torch.equal(v[0, 1:], qkv[0, :, 9:12])
+    before[1, 9, 1:, :, 2:5] = torch.stack([qkv[0, :15, 6:9], qkv[0, :15, 9:12]], 1)
+    before[1, 3, :5, :, 2:5] = torch.stack([qkv[0, 15:, 6:9], qkv[0, 15:, 9:12]], 1)
+    before[1, 4, :, :, 2:5] = torch.stack([qkv[1, :16, 6:9], qkv[1, :16, 9:12]], 1)
+    before[1, 5, :4, :, 2:5] = torch.stack([qkv[1, 16:, 6:9], qkv[1, 16:, 9:12]], 1)
+    assert torch.equal(raw(big), raw(before))
+    q = qkv[:, :, :6]
+    got = ops.attention_paged(q, view, table, i32([1, 0]), None, ops.Attn(causal=True))
+    # row 1 starts its sequence: the framework's contiguous attention says the same
+    want = ops.attention(q[1:].contiguous(), qkv[1:, :, 6:9].contiguous(), qkv[1:, :, 9:12].contiguous(), ops.Attn(causal=True))
+    assert (got[1:].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
+# -------------------------------------------------------------------------------- attention
+SHAPES = [
+    # heads, kv_heads, d, page
+    (4, 2, 128, 16), (2, 2, 64, 32), (6, 2, 64, 64), (8, 1, 128, 128), (3, 1, 96, 48), (4, 4, 40, 8), (2, 1, 128, 256),
+    (4, 2, 80, 24), (2, 1, 64, 7), (2, 2, 200, 16), (1, 1, 13, 3), (12, 2, 128, 16),
+]
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("heads,kv,d,page", SHAPES)
+def test_one_token(dtype, quantized, heads, kv, d, page):
+    held = [0, 1, page - 1, page, 127, 128, 129, 700]
+    c = Case(heads + d, len(held), 1, held, [1, 1, 1, 1, 1, 0, 1, 1], heads, kv, d, page, dtype, quantized)
+    c.put([0] * len(held), [h + n for h, n in zip(c.held, c.new)])
+    check(attend(c), c)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("heads,kv,d,page", SHAPES)
+@pytest.mark.parametrize("tokens", [5, 19])
+def test_few_tokens(dtype, quantized, heads, kv, d, page, tokens):
+    held, new = [0, 3, 250, 64], [tokens, 2, tokens - 1, 0]
+    c = Case(heads + d + tokens, 4, tokens, held, new, heads, kv, d, page, dtype, quantized)
+    c.put([0] * 4, [h + n for h, n in zip(held, new)])
+    check(attend(c), c)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("heads,kv,d,page", SHAPES[:8])
+@pytest.mark.parametrize("causal,window", [(True, None), (False, None), (True, (40, 0)), (False, (100, 30)), (True, (0, 0))])
+def test_chunks(dtype, quantized, heads, kv, d, page, causal, window):
+    held, new = [0, 130, 61], [300, 7, 200]
+    c = Case(heads + d, 3, 300, held, new, heads, kv, d, page, dtype, quantized)
+    c.put([0] * 3, [h + n for h, n in zip(held, new)])
+    check(attend(c, ops.Attn(causal=causal, window=window)), c, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("tokens", [1, 4, 40])
+@pytest.mark.parametrize("window", [(0, 0), (200, 0), (1, 64)])
+def test_window_leaves_old_pages_alone(dtype, quantized, tokens, window):
+    """Pages that a window has left behind are somebody else's: their entries may be gone
+    from the table and nothing of them is looked at."""
+    page, held = 16, [900, 333]
+    c = Case(3, 2, tokens, held, [tokens, tokens], 4, 2, 128, page, dtype, quantized)
+    c.put([max(0, h - window[0]) for h in held], [h + tokens for h in held])
+    for b, h in enumerate(held):
+        c.table[b, :max(0, h - window[0]) // page] = -1
+    check(attend(c, ops.Attn(causal=True, window=window)), c, window=window)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("tokens", [1, 3, 150])
+def test_scale_lse_and_loud_scores(dtype, quantized, tokens):
+    held, new = [500, 0], [tokens, max(1, tokens - 1)]
+    c = Case(8, 2, tokens, held, new, 4, 2, 64, 32, dtype, quantized, loud=6.0)
+    c.put([0, 0], [h + n for h, n in zip(held, new)])
+    for scale in (None, 0.7, 0.01):
+        o, lse = attend(c, ops.Attn(causal=True, scale=scale, want_lse=True))
+        want = check(o, c, scale=scale)
+        live = torch.isfinite(want)
+        assert torch.equal(torch.isfinite(lse.cpu()), live)
+        # scores are sums of D products in 32 bits; their largest is below 64 * 25 here
+        assert (lse.cpu().double() - want)[live].abs().max() <= 2.0 ** -24 * 72 * 1600 + 2.0 ** -18
+
+
+def test_other_scales():
+    """Zero and negative scales, which the tensor-core kernels leave to the exact one."""
+    c = Case(9, 2, 3, [20, 0], [3, 3], 2, 1, 64, 16, BF16, False)
+    c.put([0, 0], [23, 3])
+    for scale in (0.0, -0.5):
+        check(attend(c, ops.Attn(causal=True, scale=scale)), c, scale=scale)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_f32(quantized):
+    c = Case(5, 2, 17, [30, 0], [17, 9], 4, 2, 72, 16, F32, quantized)
+    c.put([0, 0], [47, 9])
+    check(attend(c), c)
+    check(attend(c, ops.Attn(causal=False)), c, causal=False)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+def test_one_heavy_key_among_thousands(dtype, quantized):
+    """A key of weight 1 beside 20000 of weight 2^-19 together: what the small ones add up
+    to is not lost, whatever the type of the weights in the product."""
+    n, d = 20001, 128
+    c = Case(1, 1, 1, [n - 1], [1], 2, 1, d, 64, dtype, quantized)
+    c.keys[0].zero_()
+    c.keys[0][0, 0, 0] = 19 * math.log(2.0) * math.sqrt(d) / 4
+    c.q.zero_()
+    c.q[..., 0] = 4.0
+    c.values[0].fill_(1.0)
+    c.values[0][0] = 0.0
+    c.put([0], [n])
+    check(attend(c), c)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_long_cache(dtype, quantized, tokens):
+    held = [9000, 40, 5000]
+    c = Case(2, 3, tokens, held, [tokens] * 3, 4, 2, 128, 16, dtype, quantized)
+    c.put([0] * 3, [h + tokens for h in held])
+    check(attend(c, lens=False), c)
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^32 bytes, the tokens in its last pages."""
+    pages, page, h, d = 9000, 256, 8, 128
+    c = Case(4, 1, 130, [300], [130], 8, 8, d, page, BF16, False)
+    c.put([0], [430])
+    big = [torch.empty(pages, page, h, d, dtype=BF16, device="cuda") for _ in "kv"]
+    moved = pages - c.pages
+    for x, src in zip(big, (c.k, c.v)):
+        x[moved:] = src.cuda()
+    table = c.table.clone()
+    table[0, :2] += moved
+    cache = ops.PagedCache(*big)
+    got = ops.attention_paged(c.q.cuda(), cache, table.cuda(), i32(c.held))
+    check(got, c)
+    one = ops.attention_paged(c.q[:, -1:].cuda(), cache, table.cuda(), i32([429]))
+    assert (one.double() - got[:, -1:].double()).abs().max() <= 2 * c.attention()[2][:, -1:].max()
+    k, _ = ops.cache_read(cache, table.cuda(), i32([430]), 430)
+    assert torch.equal(k[0].cpu(), c.keys[0])
+    ops.cache_write(k + 1, k, cache, table.cuda(), i32([0]))
+    assert torch.equal(big[0][table[0, 0].item()], (k + 1)[0, :256]) and torch.equal(big[1][table[0, 1].item(), :174], k[0, 256:])
+
+
+# ------------------------------------------------------------------------ bad rows, refusals
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("tokens", [1, 200])
+def test_bad_rows_are_reported(dtype, quantized, tokens):
+    """A table entry that names no page, a start below zero, a row that leaves its table:
+    the status word says so, rows beside them are what they are, nothing is touched."""
+    held = [40, 60, 30, 50]
+    c = Case(6, 4, tokens, held, [tokens] * 4, 4, 2, 128, 16, dtype, quantized)
+    c.put([0] * 4, [h + tokens for h in held])
+    good = attend(c)
+    ops.device_status()
+    for what in ("entry", "start", "reach"):
+        table, start = c.table.clone(), i32(held)
+        if what == "entry":
+            table[1, 1] = c.pages
+        elif what == "start":
+            start[1] = -1
+        else:
+            start[1] = 16 * table.shape[1] - tokens + 1
+        cache = cache_of(c)
+        got = ops.attention_paged(c.q.cuda(), cache, table.cuda(), start)
+        with pytest.raises(ops.OpsError, match="out of range"):
+            ops.device_status()
+        for b in (0, 2, 3):
+            assert torch.equal(got[b], good[b])
+        if what != "entry":
+            assert (got[1] == 0).all()
+            kept = cache_of(c)
+            new = torch.ones(4, tokens, 2, 128, dtype=dtype, device="cuda")
+            ops.cache_write(new, new, cache, table.cuda(), start)
+            with pytest.raises(ops.OpsError, match="out of range"):
+                ops.device_status()
+            mine = c.table[1, :-(-(held[1] + tokens) // 16)].long()
+            assert torch.equal(raw(cache.k)[mine.cuda()], raw(kept.k)[mine.cuda()])
+    ops.device_status()
+
+
+def test_refusals():
+    q = torch.zeros(2, 3, 4, 64, dtype=BF16, device="cuda")
+    cache = ops.PagedCache.empty(4, 16, 2, 64)
+    q8 = ops.PagedCache.empty(4, 16, 2, 64, quantized=True)
+    table, start = i32([[0, 1], [2, 3]]), i32([0, 0])
+    kv = torch.zeros(2, 3, 2, 64, dtype=BF16, device="cuda")
+
+    def refused(kind, f, *a):
+        with pytest.raises(ops.OpsError) as e:
+            f(*a)
+        assert e.value.kind == kind, e.value
+
+    A = ops.attention_paged
+    refused("Shape", A, q[0], cache, table, start)
+    refused("Shape", A, q, cache, table[:1], start)
+    refused("Shape", A, q, cache, table, start[:1])
+    refused("Shape", A, q, cache, table, start, i32([1, 1, 1]))
+    refused("Shape", A, q[..., :32], cache, table, start)
+    refused("Heads", A, q[:, :, :3], cache, table, start)
+    refused("Dtype", A, q.half(), cache, table, start)
+    refused("Dtype", A, q, ops.PagedCache(q8.k, q8.v), table, start)
+    refused("Dtype", A, q, ops.PagedCache(cache.k, cache.v, q8.k_scale, q8.v_scale), table, start)
+    refused("Dtype", A, q, ops.PagedCache(q8.k, q8.v, q8.k_scale.float(), q8.v_scale), table, start)
+    refused("Shape", A, q, ops.PagedCache(q8.k, q8.v, q8.k_scale[:3], q8.v_scale), table, start)
+    refused("Shape", A, q, ops.PagedCache(cache.k, cache.v[:3]), table, start)
+    refused("Unrealized", A, q.cpu(), cache, table, start)
+    refused("Unrealized", A, q, cache, table.cpu(), start)
+    for opts in (ops.Attn(bias=torch.zeros(2, 4, 3, 32, dtype=BF16, device="cuda")), ops.Attn(chunk=ops.Chunk(4)),
+                 ops.Attn(splits=2), ops.Attn(keys=ops.KeyMask.Lens(start)), ops.Attn(seg_start=torch.zeros(2, 3, dtype=torch.int32, device="cuda")),
+                 ops.Attn(window=(-1, 0))):
+        refused("Graph", A, q, cache, table, start, None, opts)
+    W = ops.cache_write
+    refused("Shape", W, kv[0], kv[0], cache, table, start)
+    refused("Shape", W, kv, kv[:, :2], cache, table, start)
+    refused("Shape", W, kv[:, :, :1], kv[:, :, :1], cache, table, start)
+    refused("Dtype", W, kv.half(), kv.half(), cache, table, start)
+    refused("Launch", W, cache.k[:2, :3], kv, cache, table, start)
+    refused("Launch", W, kv, kv, ops.PagedCache(cache.k, cache.k), table, start)
+    refused("Graph", W, kv, kv, ops.PagedCache(cache.k[:1].expand(4, -1, -1, -1), cache.v), table, start)
+    refused("Unrealized", W, kv.cpu(), kv, cache, table, start)
+    R = ops.cache_read
+    refused("Shape", R, cache, table, start[:1])
+    refused("Dtype", R, cache, table, start, 4, F16)
+    refused("Graph", R, q8, table, start, 4, torch.int32)
+    ops.device_status()
+
+
+def test_empty_calls():
+    cache = ops.PagedCache.empty(4, 16, 2, 64)
+    mk = lambda *s: torch.zeros(*s, dtype=BF16, device="cuda")
+    assert ops.attention_paged(mk(0, 3, 4, 64), cache, i32([[]]).view(0, 0), i32([])).shape == (0, 3, 4, 64)
+    assert ops.attention_paged(mk(2, 0, 4, 64), cache, i32([[0], [1]]), i32([0, 0])).shape == (2, 0, 4, 64)
+    got = ops.attention_paged(mk(2, 3, 4, 64) + 1, cache, i32([[], []]).view(2, 0), i32([0, 0]), i32([0, 0]))
+    assert (got == 0).all()
+    none = ops.PagedCache.empty(0, 16, 2, 64)
+    got = ops.attention_paged(mk(2, 3, 4, 64) + 1, none, i32([[], []]).view(2, 0), i32([0, 0]), i32([0, 0]))
+    assert (got == 0).all()
+    ops.cache_write(mk(2, 0, 2, 64), mk(2, 0, 2, 64), cache, i32([[0], [1]]), i32([0, 0]))
+    k, v = ops.cache_read(cache, i32([[0], [1]]), i32([3, 0]), 0)
+    assert k.shape == (2, 0, 2, 64)
+    ops.device_status()
+
+
+# ------------------------------------------------------------------ as they are used together
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+def test_a_prompt_by_chunks_and_then_token_by_token(dtype, quantized):
+    """Write, attend, write, attend: what comes out is the attention of the whole, however
+    the sequence was cut."""
+    total, cuts = 150, [0, 70, 140, 141, 142, 150]
+    c = Case(11, 2, total, [0, 0], [total, total - 8], 8, 2, 64, 16, dtype, quantized)
+    cache = cache_of(c)
+    pad = torch.nn.functional.pad
+    k, v = (torch.stack([pad(x, (0, 0, 0, 0, 0, total - x.shape[0])) for x in xs]).cuda() for xs in (c.keys, c.values))
+    q, table, got = c.q.cuda(), c.table.cuda(), []
+    for lo, hi in zip(cuts, cuts[1:]):
+        start, lens = i32([lo, lo]), i32([hi - lo, max(0, min(hi, total - 8) - lo)])
+        ops.cache_write(k[:, lo:hi], v[:, lo:hi], cache, table, start, lens)
+        got.append(ops.attention_paged(q[:, lo:hi], cache, table, start, lens))
+    check(torch.cat(got, 1), c)
+    back, _ = ops.cache_read(cache, table, i32([total, total - 8]), total, dtype)
+    for b in range(2):
+        assert torch.equal(back[b, :c.new[b]].cpu(), stored(c.keys[b], dtype, quantized).to(dtype))
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_shared_prefix(quantized):
+    """Two sequences over the same first pages."""
+    c = Case(12, 1, 60, [0], [60], 4, 2, 128, 16, BF16, quantized).put([0], [60])
+    cache = cache_of(c)
+    table = c.table.cuda().repeat(2, 1)
+    table[1, 3] = c.table[0].new_tensor([p for p in range(c.pages) if p not in c.table[0, :4].tolist()])[0].item()
+    new = torch.randn(2, 12, 2, 128, device="cuda").to(BF16)
+    ops.cache_write(new[1:], new[1:], cache, table[1:], i32([48]))
+    a = ops.attention_paged(c.q[:, 48:].cuda().repeat(2, 1, 1, 1), cache, table, i32([48, 48]))
+    check(torch.cat([ops.attention_paged(c.q[:, :48].cuda(), cache, table[:1], i32([0])), a[:1]], 1), c)
+    d = Case(12, 1, 60, [0], [60], 4, 2, 128, 16, BF16, quantized)
+    for xs in (d.keys, d.values):
+        xs[0][48:] = new[1].cpu()
+    want, _, bound = d.attention()
+    assert ((a[1].double().cpu() - want[0, 48:]).abs() <= bound[0, 48:]).all()
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+def test_graphs_streams_and_repeats(dtype, quantized):
+    """Two captured decoding steps replayed at once on two streams, with lengths that move
+    on between replays; results are the eager call's to the bit, twice over."""
+    made = []
+    for seed, tokens in ((21, 1), (22, 90)):
+        held = [700, 90, 0, 301]
+        c = Case(seed, 4, tokens, held, [tokens] * 4, 8, 2, 128, 16, dtype, quantized)
+        c.put([0] * 4, [h + tokens for h in held])
+        cache, q, table, start = cache_of(c), c.q.cuda(), c.table.cuda(), i32(held)
+        eager = ops.attention_paged(q, cache, table, start)
+        short = ops.attention_paged(q, cache, table, start // 2)
+        assert torch.equal(eager, ops.attention_paged(q, cache, table, start))
+        check(eager, c)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                ops.attention_paged(q, cache, table, start)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = ops.attention_paged(q, cache, table, start)
+        made.append((g, s, out, start, eager, short, cache, q, table))  # a graph reads them where they are
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for g, s, *_ in made:
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    g.replay()
+        torch.cuda.synchronize()
+        for _, _, out, start, eager, short, *_ in made:
+            assert torch.equal(out, short if turn == 1 else eager)
+            out.zero_()
+            start.copy_(start // 2) if turn == 0 else start.copy_(i32([700, 90, 0, 301]))
+        torch.cuda.synchronize()
+    ops.device_status()
+    made.clear()
+
+
+def test_refused_inside_packed_rows():
+    lens = i32([40, 64])
+    cache = ops.PagedCache.empty(4, 16, 2, 64)
+    q = torch.zeros(2, 64, 2, 64, dtype=BF16, device="cuda")
+    with ops.PackedRows(lens, 64):
+        with pytest.raises(ops.OpsError) as e:
+            ops.attention_paged(q, cache, i32([[0], [1]]), i32([0, 0]))
+        assert e.value.code == ops.ERR_UNSUPPORTED
