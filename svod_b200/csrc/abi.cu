@@ -1149,6 +1149,12 @@ int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache,
     chose_kernel(OP, "paged_decode", cfg);
     return check_launch(OP);
   }
+  if (config_lookup("attention|exact") == 0 && attention_paged_tc_covers(a)) {
+    const int rc = launch_attention_paged_tc(a, (cudaStream_t)stream, cfg, sizeof cfg);
+    if (rc != 0) return fail(SVODB_ERR_LAUNCH, "%s: the tensor map or kernel attributes were rejected", OP);
+    chose_kernel(OP, "paged_flash_attention", cfg);
+    return check_launch(OP);
+  }
   launch_attention_paged_exact(a, (cudaStream_t)stream);
   chose_graph(OP, is_half(a.dtype) ? "shape" : "dtype");
   return check_launch(OP);

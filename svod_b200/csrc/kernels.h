@@ -284,6 +284,9 @@ bool attention_paged_tiles(const PagedAttnArgs& a);
 // Up to 64 query rows a KV head: keys as the M of both MMAs.
 bool attention_paged_decode_covers(const PagedAttnArgs& a);
 int launch_attention_paged_decode(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len);
+// Any number of query rows: 128-row tiles of tokens x the heads of a KV head.
+bool attention_paged_tc_covers(const PagedAttnArgs& a);
+int launch_attention_paged_tc(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len);
 // Keys of the largest run that divides a page and `most`: no box of that many straddles pages.
 int page_box(int page_size, int most);
 
