@@ -16,7 +16,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -31,12 +33,16 @@ decltype(&svodb_layer_norm) p_layer_norm = nullptr;
 decltype(&svodb_rms_norm) p_rms_norm = nullptr;
 decltype(&svodb_add_layer_norm) p_add_layer_norm = nullptr;
 decltype(&svodb_add_rms_norm) p_add_rms_norm = nullptr;
+decltype(&svodb_cache_write) p_cache_write = nullptr;
+decltype(&svodb_cache_read) p_cache_read = nullptr;
+decltype(&svodb_attention_paged) p_attention_paged = nullptr;
+decltype(&svodb_attention_paged_workspace_bytes) p_attention_paged_workspace_bytes = nullptr;
 
 // Attribute names of the option dataclasses.
 #define NAMES(X)                                                                                                      \
   X(bias) X(act) X(gated) X(residual) X(scale) X(rope) X(into) X(qkv) X(k_splits) X(w_static) X(cos) X(sin) X(heads)  \
   X(head_dim) X(kv_heads) X(q_norm) X(k_norm) X(eps) X(causal) X(keys) X(window) X(chunk) X(seg_start) X(splits)      \
-  X(cache) X(want_lse) X(lens) X(mask) X(head_start) X(row_map) X(appended) X(app_lens)
+  X(cache) X(want_lse) X(lens) X(mask) X(head_start) X(row_map) X(appended) X(app_lens) X(k) X(v) X(k_scale) X(v_scale)
 #define DECL(n) PyObject* s_##n = nullptr;
 NAMES(DECL)
 
@@ -66,6 +72,19 @@ bool desc(PyObject* o, svodb_tensor& d) {
     case at::kByte: case at::kBool: d.dtype = SVODB_U8; break;
     default: return false;
   }
+  d.data = t.data_ptr();
+  d.rank = (int32_t)t.dim();
+  for (int i = 0; i < d.rank; ++i) d.shape[i] = t.size(i), d.stride[i] = t.stride(i);
+  return true;
+}
+// The same for what pages hold: 8-bit floats and their scales too.
+bool page_desc(PyObject* o, svodb_tensor& d) {
+  if (o == nullptr || !THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  const bool e4m3 = t.scalar_type() == at::kFloat8_e4m3fn, e8m0 = t.scalar_type() == at::kFloat8_e8m0fnu;
+  if (!e4m3 && !e8m0) return desc(o, d);
+  if (!t.is_cuda() || t.dim() > SVODB_MAX_RANK || t.layout() != at::kStrided) return false;
+  d.dtype = e4m3 ? SVODB_E4M3 : SVODB_E8M0;
   d.data = t.data_ptr();
   d.rank = (int32_t)t.dim();
   for (int i = 0; i < d.rank; ++i) d.shape[i] = t.size(i), d.stride[i] = t.stride(i);
@@ -333,15 +352,120 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A `PagedCache` and its table, every operand on the current device (the general path goes to
+// another one's). `keep` holds the descriptors the struct points at.
+struct PagedKeep {
+  svodb_tensor k{}, v{}, ks{}, vs{}, table{}, start{}, lens{};
+};
+bool here(PyObject* o) {
+  return THPVariable_Unpack(o).get_device() == c10::cuda::current_device();
+}
+bool paged(PyObject* cache, PyObject* table, svodb_paged_cache& c, PagedKeep& keep) {
+  Ref k = attr(cache, s_k), v = attr(cache, s_v), ks = attr(cache, s_k_scale), vs = attr(cache, s_v_scale);
+  if (!page_desc(k.o, keep.k) || !page_desc(v.o, keep.v) || !here(k.o) || !here(v.o)) return false;
+  c.k = &keep.k, c.v = &keep.v;
+  if (!ks.none()) {
+    if (!page_desc(ks.o, keep.ks) || !here(ks.o)) return false;
+    c.k_scale = &keep.ks;
+  }
+  if (!vs.none()) {
+    if (!page_desc(vs.o, keep.vs) || !here(vs.o)) return false;
+    c.v_scale = &keep.vs;
+  }
+  if (!desc(table, keep.table) || keep.table.dtype != SVODB_I32 || keep.table.rank != 2 || !here(table)) return false;
+  if (keep.table.shape[1] > 1 && keep.table.stride[1] != 1) return false;
+  c.table = &keep.table;
+  return !PyErr_Occurred();
+}
+bool counts(PyObject* o, svodb_tensor& d) { return i32(o, d) && here(o); }
+
+// cache_write(k, v, cache, table, start, lens | None): True
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || p_cache_write == nullptr) return none();
+  svodb_tensor k{}, v{};
+  svodb_paged_cache c{};
+  PagedKeep keep;
+  if (!desc(args[0], k) || !desc(args[1], v) || !here(args[0]) || !here(args[1]) || !paged(args[2], args[3], c, keep) ||
+      !counts(args[4], keep.start) || (args[5] != Py_None && !counts(args[5], keep.lens)))
+    return none();
+  void* st = stream();
+  const svodb_tensor* lens = args[5] != Py_None ? &keep.lens : nullptr;
+  if (unlocked([&] { return p_cache_write(&k, &v, &c, &keep.start, lens, st); }) != SVODB_OK) return none();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read(cache, table, lens, length, like): (k, v) in the type of `like`, a tensor, or in the pages' own
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || p_cache_read == nullptr) return none();
+  svodb_paged_cache c{};
+  PagedKeep keep;
+  if (!paged(args[0], args[1], c, keep) || !counts(args[2], keep.lens) || keep.k.rank != 4) return none();
+  const long long length = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred() || length < 0 || !THPDtype_Check(args[4])) return none();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+  int code;
+  switch (type) {
+    case at::kFloat: code = SVODB_F32; break;
+    case at::kHalf: code = SVODB_F16; break;
+    case at::kBFloat16: code = SVODB_BF16; break;
+    default: return none();
+  }
+  Ref pages = attr(args[0], s_k);
+  const auto options = THPVariable_Unpack(pages.o).options().dtype(type);
+  at::Tensor k = at::empty({keep.table.shape[0], (int64_t)length, keep.k.shape[2], keep.k.shape[3]}, options), v = at::empty_like(k);
+  svodb_tensor kd{}, vd{};
+  desc_of(k, kd, code);
+  desc_of(v, vd, code);
+  void* st = stream();
+  if (unlocked([&] { return p_cache_read(&c, &keep.lens, &kd, &vd, st); }) != SVODB_OK) return none();
+  return with_lse(std::move(k), std::move(v), true);
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_paged(q, cache, table, start, lens | None, opts): opts is an `Attn`
+PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || p_attention_paged == nullptr) return none();
+  svodb_tensor q{}, y{};
+  svodb_paged_cache c{};
+  PagedKeep keep;
+  if (!desc(args[0], q) || q.rank != 4 || !here(args[0]) || !paged(args[1], args[2], c, keep) || !counts(args[3], keep.start) ||
+      (args[4] != Py_None && !counts(args[4], keep.lens)))
+    return none();
+  svodb_attn_opts o{};
+  AttnKeep ak;
+  bool want = false;
+  if (args[5] == Py_None || !attn_opts(args[5], o, ak, want)) return none();
+  const at::Tensor& qt = THPVariable_Unpack(args[0]);
+  at::Tensor out = at::empty(qt.sizes(), qt.options()), lse, ws;
+  desc_of(out, y, q.dtype);
+  if (want) lse = lse_for(qt, q.shape[0], q.shape[2], q.shape[1], o, ak);
+  const size_t need = p_attention_paged_workspace_bytes(&q, &c);
+  if (need > 0) {
+    ws = at::empty({(int64_t)need}, qt.options().dtype(at::kByte));
+    o.workspace = ws.data_ptr(), o.workspace_bytes = need;
+  }
+  void* st = stream();
+  const svodb_tensor* lens = args[4] != Py_None ? &keep.lens : nullptr;
+  if (unlocked([&] { return p_attention_paged(&q, &c, &keep.start, lens, &o, &y, st); }) != SVODB_OK) return none();
+  return with_lse(std::move(out), std::move(lse), want);
+  END_HANDLE_TH_ERRORS
+}
+
 // init(address of svodb_linear, svodb_attention, svodb_attention_packed, svodb_layer_norm,
-// svodb_rms_norm, svodb_add_layer_norm, svodb_add_rms_norm)
+// svodb_rms_norm, svodb_add_layer_norm, svodb_add_rms_norm, svodb_cache_write, svodb_cache_read,
+// svodb_attention_paged, svodb_attention_paged_workspace_bytes)
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "seven entry point addresses");
+  constexpr int kEntries = 11;
+  if (n != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "eleven entry point addresses");
     return nullptr;
   }
-  void* p[7];
-  for (int i = 0; i < 7; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  void* p[kEntries];
+  for (int i = 0; i < kEntries; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
   p_linear = (decltype(p_linear))p[0];
   p_attention = (decltype(p_attention))p[1];
@@ -350,13 +474,18 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   p_rms_norm = (decltype(p_rms_norm))p[4];
   p_add_layer_norm = (decltype(p_add_layer_norm))p[5];
   p_add_rms_norm = (decltype(p_add_rms_norm))p[6];
+  p_cache_write = (decltype(p_cache_write))p[7];
+  p_cache_read = (decltype(p_cache_read))p[8];
+  p_attention_paged = (decltype(p_attention_paged))p[9];
+  p_attention_paged_workspace_bytes = (decltype(p_attention_paged_workspace_bytes))p[10];
 #define INTERN(n) s_##n = PyUnicode_InternFromString(#n);
   NAMES(INTERN)
   Py_RETURN_NONE;
 }
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {FAST(init), FAST(linear), FAST(attention), FAST(attention_packed), FAST(norm), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {FAST(init), FAST(linear), FAST(attention), FAST(attention_packed), FAST(norm), FAST(cache_write),
+                          FAST(cache_read), FAST(attention_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastops", "compiled call path of svod_b200.ops", -1, kMethods};
 
 }  // namespace

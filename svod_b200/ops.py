@@ -184,7 +184,7 @@ def _fast():
     return _call
 
 
-# The compiled forms of linear, attention and the norms (csrc/fastops.cpp): they return None,
+# The compiled forms of linear, attention, the norms and the paged cache's ops (csrc/fastops.cpp): they return None,
 # with nothing launched, for any call out of the ordinary, which then takes the general
 # path below (and is converted or reported there).
 _call = None
@@ -485,6 +485,10 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, table: torc
     back as NaN. Other slots stay as they are; two tokens of one call in the same slot leave
     either. Rows that leave the table and entries that are no page write nothing, and
     `device_status()` raises."""
+    global launches
+    if (_call or _fast()).cache_write(k, v, cache, table, start, lens):
+        launches += 1
+        return
     dev = _one_device(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, table, start, lens)
     with torch.cuda.device(dev):
         keep: list = []
@@ -499,6 +503,12 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, lengt
     `lens[b]` positions of row `b`, zeros behind them. `length` defaults to what the table
     reaches; `dtype` is the pages' own, for 8-bit pages any float type (bf16 by default;
     value times scale, rounded once)."""
+    global launches
+    if length is not None and dtype is not None:
+        r = (_call or _fast()).cache_read(cache, table, lens, length, dtype)
+        if r is not None:
+            launches += 1
+            return r
     dev = _one_device(cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens)
     if cache.k.dim() != 4 or table.dim() != 2:
         raise OpsError(L.ERR_SHAPE, f"cache_read: cache k has shape {list(cache.k.shape)}, table {list(table.shape)}, expected "
@@ -526,10 +536,15 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, sta
     `opts.causal` (the default without `opts`) those up to its own position, under
     `opts.window` those near it. One token a row is a decoding step, `start` zeros a prompt.
     Rows from `lens[b]` on and rows that see no key are zeros. Other options are refused."""
+    global launches
+    opts = opts or Attn(causal=True)
+    r = (_call or _fast()).attention_paged(q, cache, table, start, lens, opts)
+    if r is not None:
+        launches += 1
+        return r
     dev = _one_device(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, start, lens)
     if q.dim() != 4:
         raise OpsError(L.ERR_SHAPE, f"attention_paged: q has shape {list(q.shape)}, expected [B, T, H, D]")
-    opts = opts or Attn(causal=True)
     with torch.cuda.device(dev):
         keep: list = []
         start, lens = _i32(start), _i32(lens)
