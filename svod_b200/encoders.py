@@ -233,6 +233,44 @@ class Qwen3Embedder:
             x = ops.linear(g, lp["down_w"], Linear(residual=h, w_static=w_static))
         return x
 
+    def paged_caches(self, pages: int, page_size: int = 64, quantized: bool = False, device="cuda") -> List[ops.PagedCache]:
+        """Empty pages for `extend`, one cache a layer, in 8 bits where `quantized`."""
+        c = self.cfg
+        return [ops.PagedCache.empty(pages, page_size, c.num_key_value_heads, c.head_dim, c.dtype, quantized, device)
+                for _ in range(c.num_hidden_layers)]
+
+    def extend(self, ids: torch.Tensor, caches: List[ops.PagedCache], table: torch.Tensor, start: torch.Tensor,
+               lens: Optional[torch.Tensor] = None, out=None) -> torch.Tensor:
+        """Embeds the next chunk of every row behind what its pages hold: `ids [B,T]`, of which
+        row `b`'s first `lens[b]` (all T without `lens`, one at least) are real and stand at
+        positions `start[b]` and on. Their keys and values go into `caches` (one a layer, all
+        under `table [B, width]`) and the embedding `[B, D]` f32 of each row's last real token
+        comes back. An instruction that many queries share is embedded once and its pages
+        listed in every query's row; a document longer than memory allows goes in by chunks.
+        Nothing in the reference does this: its stack sees a row's tokens at once."""
+        c, p = self.cfg, self.p
+        H, Hkv, hd = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+        if len(caches) != c.num_hidden_layers:
+            raise ValueError(f"extend: {len(caches)} caches for {c.num_hidden_layers} layers")
+        B, T = ids.shape
+        at = (start[:, None] + torch.arange(T, dtype=torch.int32, device=start.device)).to(torch.int32)
+        cos, sin = ops.rope_table(c.rope_theta, at, hd, c.dtype, ids.device)
+        rope = (cos.view(B, T, 1, hd // 2), sin.view(B, T, 1, hd // 2))
+        x = ops.embed(ids, p["embed"])
+        for lp, cache in zip(p["layers"], caches):
+            xn = ops.rms_norm(x, lp["in_w"], c.rms_norm_eps)
+            qkv = ops.linear(xn, lp["qkv_w"], Linear(qkv=Qkv(H, Hkv, hd, lp["qn_w"], lp["kn_w"], c.rms_norm_eps, rope), w_static=True))
+            # q, k and v are read in place from the packed projection
+            heads = qkv.view(B, T, H + 2 * Hkv, hd)
+            ops.cache_write(heads[:, :, H:H + Hkv], heads[:, :, H + Hkv:], cache, table, start, lens)
+            a = ops.attention_paged(heads[:, :, :H], cache, table, start, lens, Attn(causal=True)).view(B, T, H * hd)
+            h = ops.linear(a, lp["o_w"], Linear(residual=x, w_static=True))
+            hn = ops.rms_norm(h, lp["post_w"], c.rms_norm_eps)
+            g = ops.linear(hn, lp["gu_w"], Linear(act=Act.SILU, gated=True, w_static=True))
+            x = ops.linear(g, lp["down_w"], Linear(residual=h, w_static=True))
+        last = lens if lens is not None else torch.full((B,), T, dtype=torch.int32, device=ids.device)
+        return ops.norm_pool(x, p["norm_w"], None, c.rms_norm_eps, layer=False, aux=last, mode=ops.POOL_LAST, out=out)
+
     def forward(self, ids, lengths, out=None, gather=None):
         def run(lengths):
             # final RMSNorm of the pooled (last real) tokens alone, pooling and L2: one kernel
