@@ -1078,8 +1078,14 @@ int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, s
 }
 
 size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_paged_cache* cache) {
-  (void)q, (void)cache;
-  return 0;
+  if (q == nullptr || q->rank != 4 || cache == nullptr || cache->k == nullptr || cache->v == nullptr || cache->table == nullptr)
+    return 0;  // the call itself says what is wrong
+  PagedAttnArgs a{};
+  if (paged_cache("attention_paged", cache, q->shape[0], q->dtype, a.c) != SVODB_OK) return 0;
+  if (numel(q) == 0 || q->shape[3] != a.c.d || q->shape[2] % a.c.kv_heads != 0 || !is_half(q->dtype) || a.c.d > 128) return 0;
+  a.batch = q->shape[0], a.t = q->shape[1], a.heads = (int)q->shape[2];
+  // the few-row kernel merges on the chip
+  return a.t <= 64 && a.t * (a.heads / a.c.kv_heads) <= 64 ? 0 : attention_paged_tc_workspace(a);
 }
 
 int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache, const svodb_tensor* start,
@@ -1150,6 +1156,10 @@ int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache,
     return check_launch(OP);
   }
   if (config_lookup("attention|exact") == 0 && attention_paged_tc_covers(a)) {
+    const size_t need = attention_paged_tc_workspace(a);
+    if (opts->workspace == nullptr || opts->workspace_bytes < need || !aligned16(opts->workspace))
+      return fail(SVODB_ERR_WORKSPACE, "%s: this call needs %zu workspace bytes, 16-byte aligned", OP, need);
+    a.workspace = opts->workspace;
     const int rc = launch_attention_paged_tc(a, (cudaStream_t)stream, cfg, sizeof cfg);
     if (rc != 0) return fail(SVODB_ERR_LAUNCH, "%s: the tensor map or kernel attributes were rejected", OP);
     chose_kernel(OP, "paged_flash_attention", cfg);

@@ -1,9 +1,10 @@
 // Attention of a chunk of new tokens over a paged cache on tcgen05: many query rows a KV head.
 //
-// The arithmetic is attention_tc.cu's: base-2 online softmax in f32 with the lazy rescale,
-// weights rounded to the stream type before P.V while their sum is taken in f32, scores one
-// block of 64 keys ahead of the softmax, two 128-row tiles a CTA whose softmax warps take
-// turns on the MUFU unit. What differs:
+// The arithmetic is attention_tc.cu's and the pipeline attention_tc_p.cu's: base-2 online
+// softmax in f32 with the lazy rescale, weights rounded to the stream type before P.V while
+// their sum is taken in f32, scores one block of 64 keys ahead of the softmax, two 128-row
+// tiles whose softmax warps take turns on the MUFU unit, one CTA an SM that walks its items
+// behind a two-slot ring of `Work`. What differs:
 //
 // Rows: the query heads that share a KV head lie in one tile, 128 / group tokens x group heads
 // (one TMA box [tokens, group, 64 columns]), so that a KV head's keys are fetched once for all
@@ -15,23 +16,24 @@
 // pages hold beside visible keys may be NaN: the issuers clear those rows of V before they
 // take them (K needs none of it, hidden scores are replaced).
 //
+// Work split: the batch's lengths are device memory, so the CTAs share the work out themselves.
+// Every one adds up the blocks of all items (a fixed cost of kItemCost blocks each) and takes
+// its equal run of them, in the order rows, KV heads, tiles. A run may begin and end inside an
+// item: such a part leaves its f32 state in the workspace and a second kernel merges an item's
+// parts. Rows of 0 to 6000 held keys and 128 to 512 new ones then take what their sum takes,
+// not what the longest does. No atomics, the same parts in every run.
+//
 // 8-bit pages: a fourth warpgroup widens each block from a ring of raw e4m3 blocks into the
 // 16-bit rings, value * 2^e, exact in bf16 (a value is 4 bits) and rounded once in f16's
 // subnormals. A thread moves half a key's row: the e4m3 fields are shifted to where the 16-bit
 // type has them and one packed multiply puts exponent bias and scale right, 5 instructions a
-// pair of values (a conversion through f32 is 6, on slower pipes). A block costs its warps 360
-// issue slots beside the two softmax warps' 700 on the same scheduler.
+// pair of values (a conversion through f32 is 6, on slower pipes).
 //
-// Keys split over a cluster: where there are fewer items than SMs, C CTAs take equal shares of
-// an item's blocks and merge their f32 states through distributed shared memory: one launch,
-// no workspace.
-//
-// Every mbarrier wait is bounded; a warp that gave up walks on as in attention_tc.cu.
+// Every mbarrier wait is bounded; a warp that gave up walks on as in attention_tc_p.cu.
 #include <cuda.h>
 #include <math.h>
 #include <stdio.h>
 
-#include "attention_decode_parts.cuh"
 #include "attention_parts.cuh"
 #include "common.cuh"
 #include "kernels.h"
@@ -46,8 +48,9 @@ namespace {
 
 using namespace fa_parts;
 using namespace paged;
-using dec_parts::cluster_at;
-using dec_parts::ld_cluster_f32;
+
+constexpr int kItemCost = 2;   // what an item costs beside its blocks, in blocks
+constexpr int kLeastShare = 8; // blocks a CTA takes at least, where there are few
 
 template <bool Q8, int D>
 struct PagedTcCfg {
@@ -58,18 +61,64 @@ struct PagedTcCfg {
   static constexpr int kQTile = 128 * D * 2;
   static constexpr int kKv = kBKV * D * 2;
   static constexpr size_t kSmem = 1024 + (size_t)2 * kQTile + (size_t)2 * kStages * kKv + (Q8 ? kRawStages * kRawBytes : 0) +
-                                  512;  // the barriers
+                                  768;  // the barriers and the items
   static_assert(kSmem <= 232448, "beyond the 227 KiB a CTA may hold");
-  static_assert(256 * D * 4 <= 2 * kQTile + kStages * kKv, "a share's output is laid over the tiles of q and k");
-  static_assert(2 * 256 * 4 <= kStages * kKv, "and its m and l over those of v");
 };
 
 struct PagedTcParams {
   PagedAttnArgs a;
   int group, tile_tokens;  // tokens of a 128-row tile: 128 / group
   int box;
+  int n_qt;                // items of two tiles a (row, KV head)
   float scale_log2;
+  int* heads_of_split;     // [grid][kSplitInts]: the split item whose first part a CTA has
+  float* parts;            // [grid][2][part floats]
 };
+
+// What a CTA says about the item it has the first part of, where others have the rest.
+constexpr int kSplitInts = 8;
+struct SplitItem {
+  int valid, b, hk, t0, n_live, last_cta;
+};
+// A part's state: O [D][256] by columns, then m and l of its 256 rows.
+template <int D>
+constexpr int64_t kPartFloats = (int64_t)D * 256 + 512;
+
+struct PagedWork {
+  int valid, b, hk, t0, n_live, start;
+  int key_lo, key_hi;  // of the item
+  Range r0, r1;        // this part's blocks, per tile
+  int u_lo, u_hi;
+  int part;            // -1: the whole item, else the slot that the state goes to
+};
+
+// Keys [first, last) that the query token at position `pos` sees in a row of `end` keys; both
+// grow with the position.
+__device__ __forceinline__ int first_key(const PagedAttnArgs& a, int64_t pos) {
+  const int64_t x = a.has_window ? pos - a.win_left : 0;
+  return (int)(x > 0 ? x : 0);
+}
+__device__ __forceinline__ int last_key(const PagedAttnArgs& a, int64_t pos, int64_t end) {
+  int64_t x = end;
+  if (a.causal && pos + 1 < x) x = pos + 1;
+  if (a.has_window && pos + a.win_right + 1 < x) x = pos + a.win_right + 1;
+  return (int)x;
+}
+
+// The keys of item q of a row.
+__device__ __forceinline__ void item_keys(const PagedTcParams& p, const Row& r, int q, int& lo, int& hi) {
+  const int t = q * 2 * p.tile_tokens, t_last = min(t + 2 * p.tile_tokens, r.n) - 1;
+  lo = first_key(p.a, r.start + t);
+  hi = last_key(p.a, r.start + t_last, r.start + r.n);
+}
+__device__ __forceinline__ int item_blocks(const PagedTcParams& p, const Row& r, int q) {
+  int lo, hi;
+  item_keys(p, r, q, lo, hi);
+  return (hi + kBKV - 1) / kBKV - lo / kBKV;
+}
+__device__ __forceinline__ int live_items(const PagedTcParams& p, const Row& r) {
+  return (r.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+}
 
 // Two e4m3 values, bytes 0 and 1 (or 2 and 3) of `w`, as a 16-bit pair whose exponent bias is
 // still e4m3's; the multiply by `up` (2^120 or 2^8 times the row's scale) puts it right.
@@ -116,35 +165,36 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
   uint8_t* k_s = q_s + 2 * QB;       // [S][KB]
   uint8_t* v_s = k_s + S * KB;       // [S][KB]
   uint8_t* raw_s = v_s + S * KB;     // [R][kRawBytes] (8-bit pages)
-  float* ml_s = reinterpret_cast<float*>(v_s);  // [2][256]: m and l of a share, once its blocks are done
   uint64_t* bars = reinterpret_cast<uint64_t*>(raw_s + (Q8 ? R * C::kRawBytes : 0));
-  uint64_t* q_full = bars;           // [2]
-  uint64_t* k_full = bars + 2;       // [S]
+  uint64_t* q_full = bars;            // [2]
+  uint64_t* q_empty = bars + 2;       // [2]
+  uint64_t* k_full = bars + 4;        // [S]
   uint64_t* k_empty = k_full + S;
   uint64_t* v_full = k_empty + S;
   uint64_t* v_empty = v_full + S;
-  uint64_t* s_full = v_empty + S;    // [2 tiles][2 buffers]
-  uint64_t* p_full = s_full + 4;     // [2 tiles][2 buffers]
-  uint64_t* tail_done = p_full + 4;  // [2 tiles]: the last two P.V of a tile
-  uint64_t* raw_full = tail_done + 2;  // [R]
+  uint64_t* s_full = v_empty + S;     // [2 tiles][2 buffers]
+  uint64_t* p_full = s_full + 4;      // [2 tiles][2 buffers]
+  uint64_t* tail_done = p_full + 4;   // [2 tiles]: the last two P.V of a tile
+  uint64_t* o_empty = tail_done + 2;  // [2 tiles]
+  uint64_t* item_full = o_empty + 2;  // [2 slots]
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* raw_full = item_empty + 2;  // [R]
   uint64_t* raw_empty = raw_full + R;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + R);
+  PagedWork* item_ring = reinterpret_cast<PagedWork*>(tmem_slot + 2);  // [2]
+  static_assert((4 + 4 * S + 18 + 2 * R) * 8 + 8 + 2 * sizeof(PagedWork) <= 768, "the barriers and the items fit");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  uint32_t rank, csize;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
-  // Later query tiles, heavier under a causal mask, come first for every row and head.
-  const int qt = (int)gridDim.y - 1 - (int)blockIdx.y;
-  const int pair = blockIdx.x / csize;
-  const int b = pair / a.c.kv_heads, hk = pair % a.c.kv_heads;
-  const int t0 = qt * 2 * p.tile_tokens;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&tail_done[i], 1);
+      mbar_init(&o_empty[i], 4);                // the tile's four softmax warps
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], Q8 ? 14 : 10);  // two issuers, eight softmax warps, four widening ones
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -169,176 +219,279 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  __syncthreads();
-  pdl_trigger();
-  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
+  pdl_wait();
   const uint32_t tmem_base = *tmem_slot;
-
-  const Row row_b = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (row_b.bad && threadIdx.x == 0 && qt == 0 && hk == 0 && rank == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
-  const int64_t end = row_b.start + row_b.n;
-  // Keys [first, last) that query token t sees; both grow with t.
-  auto first_of = [&](int t) {
-    const int64_t x = a.has_window ? row_b.start + t - a.win_left : 0;
-    return (int)(x > 0 ? x : 0);
-  };
-  auto last_of = [&](int t) {
-    int64_t x = end;
-    if (a.causal && row_b.start + t + 1 < x) x = row_b.start + t + 1;
-    if (a.has_window && row_b.start + t + a.win_right + 1 < x) x = row_b.start + t + a.win_right + 1;
-    return (int)x;
-  };
-  // What the live tokens [t, t + tile_tokens) of a tile see: all its keys, and those that every token sees.
-  const int n_live = row_b.n;
-  const int ta = t0, tb = t0 + p.tile_tokens;
-  auto last_token = [&](int t) { return min(t + p.tile_tokens, n_live) - 1; };
-  const bool has0 = ta < n_live, has1 = tb < n_live;
-  const int lo0 = has0 ? first_of(ta) : 0, hi0 = has0 ? last_of(last_token(ta)) : 0;
-  const int lo1 = has1 ? first_of(tb) : lo0, hi1 = has1 ? last_of(last_token(tb)) : hi0;
-  const int key_lo = lo0, key_hi = hi1 > hi0 ? hi1 : hi0;  // of the item
-  const int blk_lo = key_lo / kBKV, blk_n = key_hi > key_lo ? (key_hi + kBKV - 1) / kBKV - blk_lo : 0;
-  // this CTA's share of the item's blocks
-  const int per = (blk_n + (int)csize - 1) / (int)csize;
-  const int sh_lo = blk_lo + min((int)rank * per, blk_n), sh_hi = min(sh_lo + per, blk_lo + blk_n);
-  auto range = [&](bool has, int lo, int hi) {
-    Range r{0, 0};
-    if (!has || hi <= lo) return r;
-    const int x = max(lo / kBKV, sh_lo), y = min((hi + kBKV - 1) / kBKV, sh_hi);
-    if (y > x) r.lo = x, r.hi = y;
-    return r;
-  };
-  const Range r0 = range(has0, lo0, hi0), r1 = range(has1, lo1, hi1);
-  const bool live0 = r0.hi > r0.lo, live1 = r1.hi > r1.lo;
-  int u_lo = 0, u_hi = 0;
-  if (live0 && live1) {
-    u_lo = r0.lo < r1.lo ? r0.lo : r1.lo;
-    u_hi = r0.hi > r1.hi ? r0.hi : r1.hi;
-  } else if (live0) {
-    u_lo = r0.lo, u_hi = r0.hi;
-  } else if (live1) {
-    u_lo = r1.lo, u_hi = r1.hi;
-  }
-  // the first and the last block hold slots beside the item's keys
-  const bool ragged_lo = key_lo % kBKV != 0, ragged_hi = key_hi % kBKV != 0;
-  const int32_t* table = a.c.table + (int64_t)b * a.c.table_sb;
+  const int64_t capacity = a.c.width * a.c.page_size;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
-      // ---------------- TMA loader: the lanes issue a block's boxes side by side ----------------
-      if (u_hi > u_lo) {
-        const int nb = kBKV / p.box;
-        constexpr int kCols = Q8 ? 1 : D / 64;
-        const int my_box = lane % nb, my_col = lane / nb;
-        const bool mine = my_col < kCols;
-        if (lane == 0) {
-          const uint32_t bytes = (uint32_t)(p.tile_tokens * p.group * 128 * (D / 64));
-          for (int i = 0; i < 2; ++i) {
-            if (i == 0 ? live0 : live1) {
-              mbar_expect_tx(&q_full[i], bytes);
+      // ---------------- the CTA's run of the work, and the TMA loads ----------------
+      // What a row's items weigh, for one KV head.
+      auto weigh = [&](const Row& r) -> int64_t {
+        int64_t w = 0;
+        for (int q = 0; q < live_items(p, r); ++q) w += item_blocks(p, r, q) + kItemCost;
+        return w;
+      };
+      auto row_at = [&](int b) { return row_of(a.start, a.lens, b, a.t, capacity); };
+      const int batch = (int)a.batch;
+      int64_t total = 0;
+      for (int b = lane; b < batch; b += 32) {
+        const Row r = row_at(b);
+        if (r.bad && blockIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+        total += weigh(r);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      total *= a.c.kv_heads;
+      int64_t quota = (total + gridDim.x - 1) / gridDim.x;
+      if (quota < kLeastShare) quota = kLeastShare;
+      const int64_t c0 = quota * blockIdx.x, c1 = c0 + quota < total ? c0 + quota : total;
+      // Where the run begins: row b, KV head hk, item q, whose weight lies at [x, x + weight).
+      int b = 0, hk = 0, q = 0;
+      int64_t x = 0;
+      Row row{0, 0, false};
+      int64_t row_weight = 0;
+      if (c0 < c1) {
+        int64_t base = 0;
+        for (int b0 = 0; b0 < batch; b0 += 32) {
+          const int64_t w = b0 + lane < batch ? weigh(row_at(b0 + lane)) * a.c.kv_heads : 0;
+          int64_t upto = w;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+          }
+          const uint32_t past = __ballot_sync(0xffffffffu, base + upto > c0);
+          if (past != 0u) {
+            const int l = __ffs((int)past) - 1;
+            b = b0 + l;
+            row_weight = __shfl_sync(0xffffffffu, w, l) / a.c.kv_heads;
+            x = base + __shfl_sync(0xffffffffu, upto - w, l);
+            break;
+          }
+          base += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        row = row_at(b);
+        hk = (int)((c0 - x) / row_weight);
+        x += hk * row_weight;
+        for (int64_t w = item_blocks(p, row, 0) + kItemCost; x + w <= c0; w = item_blocks(p, row, q) + kItemCost) x += w, ++q;
+      }
+      SplitItem split{0, 0, 0, 0, 0, 0};
+      const int nb = kBKV / p.box;
+      constexpr int kCols = Q8 ? 1 : D / 64;
+      const int my_box = lane % nb, my_col = lane / nb;
+      const bool mine = my_col < kCols;
+      int s = 0;  // ring slot of the next block (16-bit pages) or copy (8-bit)
+      uint32_t ph = 0;
+      uint32_t q_items[2] = {0, 0};  // live items so far, per tile
+      bool ok = true;
+      auto wait_by_lane0 = [&](uint64_t* bar, uint32_t parity) {
+        bool done = true;
+        if (lane == 0) done = mbar_wait(bar, parity, a.status);
+        ok = __shfl_sync(0xffffffffu, (int)done, 0) != 0;
+        return ok;
+      };
+      uint32_t n_it = 0;
+      // (a CTA whose run would begin behind the last item has none)
+      while (c0 < c1 && x < c1 && ok) {
+        PagedWork w;
+        w.valid = 1, w.b = b, w.hk = hk, w.t0 = q * 2 * p.tile_tokens, w.n_live = row.n, w.start = (int)row.start;
+        item_keys(p, row, q, w.key_lo, w.key_hi);
+        const int blk_lo = w.key_lo / kBKV, blk_n = (w.key_hi + kBKV - 1) / kBKV - blk_lo;
+        const int64_t weight = blk_n + kItemCost;
+        // this run's part of the item's blocks: its first kItemCost units stand for the fixed cost
+        const int64_t u0 = (c0 > x ? c0 - x : 0) - kItemCost, u1 = (c1 < x + weight ? c1 - x : weight) - kItemCost;
+        const int from = u0 > 0 ? (int)u0 : 0, to = u1 > 0 ? (int)u1 : 0;
+        if (to > from) {
+          w.part = from == 0 && to == blk_n ? -1 : from == 0 ? 1 : 0;
+          if (w.part == 1) split = SplitItem{1, b, hk, w.t0, row.n, (int)((x + weight - 1) / quota)};
+          auto range = [&](int t) {
+            Range r{0, 0};
+            if (t >= row.n) return r;
+            const int t_last = min(t + p.tile_tokens, row.n) - 1;
+            const int lo = first_key(a, row.start + t) / kBKV;
+            const int hi = (last_key(a, row.start + t_last, row.start + row.n) + kBKV - 1) / kBKV;
+            const int y = max(lo, blk_lo + from), z = min(hi, blk_lo + to);
+            if (z > y) r.lo = y, r.hi = z;
+            return r;
+          };
+          w.r0 = range(w.t0);
+          w.r1 = range(w.t0 + p.tile_tokens);
+          const bool live0 = w.r0.hi > w.r0.lo, live1 = w.r1.hi > w.r1.lo;
+          w.u_lo = w.u_hi = 0;
+          if (live0 && live1) {
+            w.u_lo = w.r0.lo < w.r1.lo ? w.r0.lo : w.r1.lo;
+            w.u_hi = w.r0.hi > w.r1.hi ? w.r0.hi : w.r1.hi;
+          } else if (live0) {
+            w.u_lo = w.r0.lo, w.u_hi = w.r0.hi;
+          } else if (live1) {
+            w.u_lo = w.r1.lo, w.u_hi = w.r1.hi;
+          }
+          const int slot = (int)(n_it & 1);
+          if (!wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1)) break;
+          if (lane == 0) {
+            item_ring[slot] = w;
+            __threadfence_block();
+            mbar_arrive(&item_full[slot]);
+          }
+          ++n_it;
+          const int32_t* table = a.c.table + (int64_t)b * a.c.table_sb;
+          auto look_up = [&](int blk, int& at) -> int {
+            const int j = blk * kBKV + my_box * p.box;
+            at = 0;
+            if (!mine || blk >= w.u_hi || j + p.box <= w.key_lo || j >= w.key_hi) return (int)a.c.pages;
+            const int page = j / a.c.page_size;
+            at = j - page * a.c.page_size;
+            const int id = table[page];
+            if (id < 0 || id >= a.c.pages) {
+              atomicExch(a.status, (uint32_t)kStatusBadIndex);
+              return (int)a.c.pages;
+            }
+            return id;
+          };
+          int next_at;
+          int next_id = look_up(w.u_lo, next_at);
+          for (int i = 0; i < 2 && ok; ++i) {
+            if (!(i == 0 ? live0 : live1)) continue;
+            // the issuer's last QK of the tile's previous live item has read this Q tile
+            if (!wait_by_lane0(&q_empty[i], (q_items[i] & 1) ^ 1)) break;
+            ++q_items[i];
+            if (lane == 0) {
+              mbar_expect_tx(&q_full[i], (uint32_t)(p.tile_tokens * p.group * 128 * (D / 64)));
               for (int c = 0; c < D / 64; ++c)
                 tma_load_4d(q_s + i * QB + c * (128 * 128), &tmap_q, &q_full[i], c * 64, hk * p.group,
-                            t0 + i * p.tile_tokens, b);
+                            w.t0 + i * p.tile_tokens, b);
             }
           }
-        }
-        auto look_up = [&](int blk, int& slot) -> int {
-          const int j = blk * kBKV + my_box * p.box;
-          slot = 0;
-          if (!mine || j + p.box <= key_lo || j >= key_hi) return (int)a.c.pages;
-          const int page = j / a.c.page_size;
-          slot = j - page * a.c.page_size;
-          const int id = table[page];
-          if (id < 0 || id >= a.c.pages) {
-            atomicExch(a.status, (uint32_t)kStatusBadIndex);
-            return (int)a.c.pages;
-          }
-          return id;
-        };
-        int slot, next_slot;
-        int next_id = look_up(u_lo, next_slot);
-        bool ok = true;
-        auto wait_free = [&](uint64_t* bar, uint32_t parity) {
-          bool free = true;
-          if (lane == 0) free = mbar_wait(bar, parity, a.status);
-          ok = __shfl_sync(0xffffffffu, (int)free, 0) != 0;
-          return ok;
-        };
-        int s = 0;       // ring slot of the next block (16-bit pages), or copy count of the raw ring
-        uint32_t ph = 0;
-        for (int j = u_lo; j < u_hi; ++j) {
-          const int id = next_id;
-          slot = next_slot;
-          if (j + 1 < u_hi) next_id = look_up(j + 1, next_slot);
-          for (int kv = 0; kv < 2; ++kv) {
-            const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
-            if constexpr (Q8) {
-              if (!wait_free(&raw_empty[s], ph ^ 1)) break;
-              if (lane == 0) mbar_expect_tx(&raw_full[s], C::kRawBytes);
-              __syncwarp();
-              if (mine) tma_load_4d(raw_s + s * C::kRawBytes + my_box * p.box * 128, map, &raw_full[s], 0, hk, slot, id);
-              if (++s == R) s = 0, ph ^= 1;
-            } else {
-              uint64_t* full = kv ? v_full : k_full;
-              if (!wait_free(kv ? &v_empty[s] : &k_empty[s], ph ^ 1)) break;
-              if (lane == 0) mbar_expect_tx(&full[s], KB);
-              __syncwarp();
-              if (mine)
-                tma_load_4d((kv ? v_s : k_s) + s * KB + my_col * KBOX + my_box * p.box * 128, map, &full[s], my_col * 64, hk,
-                            slot, id);
+          for (int j = w.u_lo; j < w.u_hi && ok; ++j) {
+            const int id = next_id, at = next_at;
+            next_id = look_up(j + 1, next_at);
+            for (int kv = 0; kv < 2; ++kv) {
+              const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
+              if constexpr (Q8) {
+                if (!wait_by_lane0(&raw_empty[s], ph ^ 1)) break;
+                if (lane == 0) mbar_expect_tx(&raw_full[s], C::kRawBytes);
+                __syncwarp();
+                if (mine) tma_load_4d(raw_s + s * C::kRawBytes + my_box * p.box * 128, map, &raw_full[s], 0, hk, at, id);
+                if (++s == R) s = 0, ph ^= 1;
+              } else {
+                uint64_t* full = kv ? v_full : k_full;
+                if (!wait_by_lane0(kv ? &v_empty[s] : &k_empty[s], ph ^ 1)) break;
+                if (lane == 0) mbar_expect_tx(&full[s], KB);
+                __syncwarp();
+                if (mine)
+                  tma_load_4d((kv ? v_s : k_s) + s * KB + my_col * KBOX + my_box * p.box * 128, map, &full[s], my_col * 64, hk,
+                              at, id);
+              }
             }
+            if (!Q8 && ok && ++s == S) s = 0, ph ^= 1;
           }
-          if (!ok) break;
-          if (!Q8 && ++s == S) s = 0, ph ^= 1;
         }
-        if (!ok)
-          for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA's memory goes
+        // the next item
+        x += weight;
+        if (++q == live_items(p, row)) {
+          q = 0;
+          if (++hk == a.c.kv_heads) {
+            hk = 0;
+            do row = ++b < batch ? row_at(b) : Row{0, 0, false};
+            while (b < batch && row.n == 0);
+            if (b >= batch) break;
+          }
+        }
       }
-    } else if (warp == 1 || warp == 3) {
-      // ---------------- MMA issuers: warp 1 drives tile 0, warp 3 tile 1 (attention_tc.cu) ----------------
+      if (lane == 0) {
+        int* h = p.heads_of_split + (int64_t)blockIdx.x * kSplitInts;
+        h[0] = split.valid, h[1] = split.b, h[2] = split.hk, h[3] = split.t0, h[4] = split.n_live, h[5] = split.last_cta;
+      }
+      const int slot = (int)(n_it & 1);
+      if (ok && wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1) && lane == 0) {
+        item_ring[slot].valid = 0;
+        __threadfence_block();
+        mbar_arrive(&item_full[slot]);
+      }
+      if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA's memory goes
+    } else if (warp == 2) {
+      // ---------------- rows behind a chunk's real tokens that no item has: zeros ----------------
+      const int step = 2 * p.tile_tokens;
+      for (int64_t u = blockIdx.x; u < a.batch * p.n_qt; u += gridDim.x) {
+        const int64_t b = u / p.n_qt;
+        const int t0 = (int)(u % p.n_qt) * step;
+        const Row r = row_of(a.start, a.lens, b, a.t, capacity);
+        if (t0 < r.n) continue;
+        const int pieces = a.c.d / 8, rows = (int)(a.t - t0 < step ? a.t - t0 : step) * a.heads;
+        for (int i = lane; i < rows * pieces; i += 32) {
+          const int rw = i / pieces, t = t0 + rw / a.heads, h = rw % a.heads;
+          stg128((T*)a.o + b * a.o_sb + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + (i % pieces) * 8, make_uint4(0, 0, 0, 0));
+          if (a.lse != nullptr && i % pieces == 0) a.lse[(b * a.heads + h) * a.t + t] = -INFINITY;
+        }
+      }
+    } else {
+      // ---------------- MMA issuers: warp 1 drives tile 0, warp 3 tile 1 (attention_tc_p.cu) ----------------
       const int i = warp == 1 ? 0 : 1;
-      const Range r = i == 0 ? r0 : r1;
       const bool leader = elect_one();
-      if (u_hi > u_lo) {
-        constexpr uint32_t idesc_qk = umma_idesc(Elem<T>::kUmmaFormat, 128, kBKV, 0, 0);
-        constexpr uint32_t idesc_pv = umma_idesc(Elem<T>::kUmmaFormat, 128, D, 0, 1);
-        const uint64_t qa = umma_desc_sw128(smem_u32(q_s) + i * QB, 16, 1024);
-        const uint64_t k_desc0 = umma_desc_sw128(smem_u32(k_s), 16, 1024);
-        const uint64_t v_desc0 = umma_desc_sw128(smem_u32(v_s), KBOX, 1024);
+      constexpr uint32_t idesc_qk = umma_idesc(Elem<T>::kUmmaFormat, 128, kBKV, 0, 0);
+      constexpr uint32_t idesc_pv = umma_idesc(Elem<T>::kUmmaFormat, 128, D, 0, 1);
+      const uint64_t qa = umma_desc_sw128(smem_u32(q_s) + i * QB, 16, 1024);
+      const uint64_t k_desc0 = umma_desc_sw128(smem_u32(k_s), 16, 1024);
+      const uint64_t v_desc0 = umma_desc_sw128(smem_u32(v_s), KBOX, 1024);
+      uint32_t kv_blocks = 0;  // K/V blocks of all earlier items (ring position)
+      uint32_t my_blocks = 0;  // blocks of this tile in all earlier items (S/P buffer and phase)
+      uint32_t my_items = 0;   // live items of this tile so far
+      bool ok = true;
+      for (uint32_t n_it = 0; ok; ++n_it) {
+        const int slot = (int)(n_it & 1);
+        if (!mbar_wait(&item_full[slot], (n_it >> 1) & 1, a.status)) break;
+        const PagedWork w = item_ring[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[slot]);
+        if (!w.valid) break;
+        const Range r = i == 0 ? w.r0 : w.r1;
         const int nblk = r.hi - r.lo;
-        bool ok = true;
+        const bool live = nblk > 0;
+        // blocks that hold slots beside the item's keys
+        const int edge_lo = w.key_lo % kBKV != 0 ? w.key_lo / kBKV : -1;
+        const int edge_hi = w.key_hi % kBKV != 0 ? w.key_hi / kBKV : -1;
         bool q_ready = false;
-        for (int t = u_lo - 1; t <= u_hi && ok; ++t) {
+        for (int t = w.u_lo - 1; t <= w.u_hi && ok; ++t) {
           const int jq = t + 1;  // block whose scores are issued this step
           const int jp = t - 1;  // block whose P.V is issued this step
-          const bool have_k = jq >= u_lo && jq < u_hi;
-          const bool have_v = jp >= u_lo && jp < u_hi;
-          const int ks_slot = have_k ? (jq - u_lo) % S : 0;
-          const int vs_slot = have_v ? (jp - u_lo) % S : 0;
+          const bool have_k = jq >= w.u_lo && jq < w.u_hi;
+          const bool have_v = jp >= w.u_lo && jp < w.u_hi;
+          const uint32_t kpos = kv_blocks + (uint32_t)(have_k ? jq - w.u_lo : 0);
+          const uint32_t vpos = kv_blocks + (uint32_t)(have_v ? jp - w.u_lo : 0);
+          const int ks_slot = (int)(kpos % S), vs_slot = (int)(vpos % S);
           const bool do_pv = have_v && jp >= r.lo && jp < r.hi;
           const bool do_qk = have_k && jq >= r.lo && jq < r.hi;
           // Every slot is waited for and released by both issuers, used or not.
-          if ((have_k && !mbar_wait(&k_full[ks_slot], (uint32_t)(((jq - u_lo) / S) & 1), a.status)) ||
-              (have_v && !mbar_wait(&v_full[vs_slot], (uint32_t)(((jp - u_lo) / S) & 1), a.status))) {
+          if ((have_k && !mbar_wait(&k_full[ks_slot], (kpos / S) & 1, a.status)) ||
+              (have_v && !mbar_wait(&v_full[vs_slot], (vpos / S) & 1, a.status))) {
             ok = false;
             break;
           }
           if (do_pv) {
-            const int n = jp - r.lo;  // this tile's block counter
-            if (!mbar_wait(&p_full[i * 2 + (n & 1)], (uint32_t)((n >> 1) & 1), a.status)) {
+            const uint32_t n = (uint32_t)(jp - r.lo);
+            const uint32_t N = my_blocks + n;  // this tile's running block counter
+            if (n == 0 && !mbar_wait(&o_empty[i], (my_items & 1) ^ 1, a.status)) {
+              ok = false;  // the previous item's O has not been read out
+              break;
+            }
+            if (!mbar_wait(&p_full[i * 2 + (N & 1)], (N >> 1) & 1, a.status)) {
               ok = false;
               break;
             }
             if constexpr (!Q8) {
               // Rows beside the item's keys hold whatever the pages hold there: 0 * NaN must not
               // enter the sum. Both issuers clear them, to the same zeros, before either lets go.
-              if ((ragged_lo && jp == blk_lo) || (ragged_hi && jp == blk_lo + blk_n - 1)) {
-                for (int x = lane; x < kBKV * (D / 8); x += 32) {
-                  const int row = x / (D / 8), c = x % (D / 8), key = jp * kBKV + row;
-                  if (key < key_lo || key >= key_hi)
+              if (jp == edge_lo || jp == edge_hi) {
+                for (int y = lane; y < kBKV * (D / 8); y += 32) {
+                  const int row = y / (D / 8), c = y % (D / 8), key = jp * kBKV + row;
+                  if (key < w.key_lo || key >= w.key_hi)
                     *reinterpret_cast<uint4*>(v_s + vs_slot * KB + (c >> 3) * KBOX + row * 128 + (c & 7) * 16) =
                         make_uint4(0, 0, 0, 0);
                 }
@@ -348,7 +501,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
             }
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + 256 + i * D;
-            const uint32_t a_tmem = tmem_base + (uint32_t)((i * 2 + (n & 1)) * kBKV);
+            const uint32_t a_tmem = tmem_base + (uint32_t)((i * 2 + (N & 1)) * kBKV);
             const uint64_t vb = v_desc0 + (uint64_t)((vs_slot * KB) >> 4);
             const uint32_t first = n != 0 ? 1u : 0u;
 #pragma unroll
@@ -356,19 +509,19 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
               if (leader)
                 umma_ts(d_tmem, a_tmem + ks * 8, vb + (uint64_t)(ks * (2048 >> 4)), idesc_pv,
                         (first | (uint32_t)ks) != 0 ? 1u : 0u);
-            if (leader && n + 2 >= nblk) tc_commit(&tail_done[i]);
+            if (leader && (int)n + 2 >= nblk) tc_commit(&tail_done[i]);
           }
           if (do_qk) {
             if (!q_ready) {
-              if (!mbar_wait(&q_full[i], 0, a.status)) {
+              if (!mbar_wait(&q_full[i], my_items & 1, a.status)) {
                 ok = false;
                 break;
               }
               q_ready = true;
             }
             tc_fence_after();
-            const int n = jq - r.lo;
-            const uint32_t d_tmem = tmem_base + (uint32_t)((i * 2 + (n & 1)) * kBKV);
+            const uint32_t N = my_blocks + (uint32_t)(jq - r.lo);
+            const uint32_t d_tmem = tmem_base + (uint32_t)((i * 2 + (N & 1)) * kBKV);
             const uint64_t kb = k_desc0 + (uint64_t)((ks_slot * KB) >> 4);
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
@@ -376,312 +529,392 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
               const uint64_t koff = (uint64_t)((ks >> 2) * (KBOX >> 4) + (ks & 3) * 2);
               if (leader) umma_ss(d_tmem, qa + qoff, kb + koff, idesc_qk, ks != 0 ? 1u : 0u);
             }
-            if (leader) tc_commit(&s_full[i * 2 + (n & 1)]);
+            if (leader) tc_commit(&s_full[i * 2 + (N & 1)]);
+            // the item's last QK has read the Q tile: the loader may bring the next one
+            if (leader && jq == r.hi - 1) tc_commit(&q_empty[i]);
           }
           if (leader && have_v) tc_commit(&v_empty[vs_slot]);
           if (leader && have_k) tc_commit(&k_empty[ks_slot]);
           __syncwarp();
         }
+        kv_blocks += (uint32_t)(w.u_hi - w.u_lo);
+        if (live) {
+          my_blocks += (uint32_t)nblk;
+          ++my_items;
+        }
       }
     }
   } else if (Q8 && warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ---------------- widening: raw e4m3 blocks into the 16-bit rings ----------------
     if constexpr (Q8) {
       const int tid = threadIdx.x - 384;
       const int r = tid & 63, half = tid >> 6;  // a key of the block, half of its row
       constexpr int kPieces = D / 32;           // 16-byte pieces of half a row
-      // my key's scale codes, its page looked up a block ahead
-      auto key_page = [&](int j) -> int {
-        const int key = j * kBKV + r;
-        return j < u_hi && key >= key_lo && key < key_hi ? table[key / a.c.page_size] : -1;
-      };
-      auto key_codes = [&](int j, int page, uint32_t& kc, uint32_t& vc) {
-        kc = vc = 0u;
-        if (page >= 0 && page < a.c.pages) {
-          const int64_t slot = (j * kBKV + r) % a.c.page_size;
-          kc = a.c.k_scale[page * a.c.ks_sp + hk * a.c.ks_sh + slot];
-          vc = a.c.v_scale[page * a.c.vs_sp + hk * a.c.vs_sh + slot];
-        }
-      };
-      uint32_t codes[2], next_codes[2];
-      key_codes(u_lo, key_page(u_lo), codes[0], codes[1]);
-      int page_next = key_page(u_lo + 1);
+      const int page_size = a.c.page_size;
+      const int pages_on = kBKV / page_size, slots_on = kBKV % page_size;  // from a block to the next
+      // where the pieces of my half row lie: 16-byte piece c of a 128-byte row r at (c ^ r) mod 8
+      const uint32_t src_at = (uint32_t)(r * 128 + (((half * kPieces) ^ (r & 7)) << 4));
+      const uint32_t dst_at = (uint32_t)(r * 128 + ((((half * kPieces * 2) & 7) ^ (r & 7)) << 4) + ((half * kPieces * 2) >> 3) * KBOX);
+      uint32_t pos = 0;  // K/V blocks so far (ring position)
       int rs = 0;
       uint32_t rph = 0;
       bool ok = true;
-      for (int j = u_lo; j < u_hi && ok; ++j) {
-        key_codes(j + 1, page_next, next_codes[0], next_codes[1]);
-        page_next = key_page(j + 2);
-        const int s = (j - u_lo) % S;
-        const uint32_t ph = (uint32_t)(((j - u_lo) / S) & 1);
-        const int key = j * kBKV + r;
-        const bool real = key >= key_lo && key < key_hi;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!mbar_wait(&raw_full[rs], rph, a.status) || !mbar_wait(kv ? &v_empty[s] : &k_empty[s], ph ^ 1, a.status)) {
-            ok = false;
-            break;
+      for (uint32_t n_it = 0; ok; ++n_it) {
+        const int islot = (int)(n_it & 1);
+        if (!mbar_wait(&item_full[islot], (n_it >> 1) & 1, a.status)) break;
+        const PagedWork w = item_ring[islot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[islot]);
+        if (!w.valid) break;
+        const int32_t* table = a.c.table + (int64_t)w.b * a.c.table_sb;
+        const uint8_t* ks_base = a.c.k_scale + (int64_t)w.hk * a.c.ks_sh;
+        const uint8_t* vs_base = a.c.v_scale + (int64_t)w.hk * a.c.vs_sh;
+        // my key's page and slot walk a block at a time; its page id is looked up two blocks
+        // ahead, its scale codes one
+        int page = (w.u_lo * kBKV + r) / page_size, slot = (w.u_lo * kBKV + r) - page * page_size;
+        auto id_of = [&](int key, int pg) -> int { return key >= w.key_lo && key < w.key_hi ? table[pg] : -1; };
+        auto codes_of = [&](int id, int sl, uint32_t& kc, uint32_t& vc) {
+          kc = vc = 0u;
+          if (id >= 0 && id < a.c.pages) {
+            kc = ks_base[id * a.c.ks_sp + sl];
+            vc = vs_base[id * a.c.vs_sp + sl];
           }
-          const uint8_t* src = raw_s + rs * C::kRawBytes + r * 128;
-          uint8_t* dst = (kv ? v_s : k_s) + s * KB + r * 128;
-          const uint32_t up = widen_factor<T>(codes[kv]);
-          const bool plain = up != 0u;
+        };
+        auto step = [&]() {
+          page += pages_on, slot += slots_on;
+          if (slot >= page_size) slot -= page_size, ++page;
+        };
+        int key = w.u_lo * kBKV + r;
+        uint32_t kc, vc;
+        codes_of(id_of(key, page), slot, kc, vc);
+        step();
+        int id_next = w.u_lo + 1 < w.u_hi ? id_of(key + kBKV, page) : -1;
+        for (int j = w.u_lo; j < w.u_hi; ++j, ++pos, key += kBKV) {
+          uint32_t kc_next, vc_next;
+          codes_of(id_next, slot, kc_next, vc_next);
+          step();
+          id_next = j + 2 < w.u_hi ? id_of(key + 2 * kBKV, page) : -1;
+          const int s = (int)(pos % S);
+          const uint32_t ph = (pos / S) & 1;
+          const bool real = key >= w.key_lo && key < w.key_hi;
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const int c = half * kPieces + i;  // 16 columns from 16 c
-            const uint4 u = *reinterpret_cast<const uint4*>(src + ((c ^ (r & 7)) << 4));
-            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-            uint32_t w[8];
-            if (plain) {
+          for (int kv = 0; kv < 2; ++kv) {
+            if (!mbar_wait(&raw_full[rs], rph, a.status) || !mbar_wait(kv ? &v_empty[s] : &k_empty[s], ph ^ 1, a.status)) {
+              ok = false;
+              break;
+            }
+            const uint8_t* src = raw_s + rs * C::kRawBytes;
+            uint8_t* dst = (kv ? v_s : k_s) + s * KB;
+            const uint32_t code = kv ? vc : kc;
+            // a slot beside the item's keys becomes zeros, whatever it holds: every pattern is finite here
+            const uint32_t factor = widen_factor<T>(code), up = real ? factor : 0u;
+            uint4 in[kPieces];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                w[2 * e] = widen_pair<T>(in[e], 0, up);
-                w[2 * e + 1] = widen_pair<T>(in[e], 1, up);
+            for (int i = 0; i < kPieces; ++i) in[i] = *reinterpret_cast<const uint4*>(src + (src_at ^ (uint32_t)(i << 4)));
+            if (!real || factor != 0u) {
+#pragma unroll
+              for (int i = 0; i < kPieces; ++i) {
+                // piece i of 16 values: 32 bytes, the 16-byte pieces 2 i and 2 i + 1 behind dst_at's
+                const uint32_t to = (dst_at ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
+                const uint4 x = make_uint4(widen_pair<T>(in[i].x, 0, up), widen_pair<T>(in[i].x, 1, up),
+                                           widen_pair<T>(in[i].y, 0, up), widen_pair<T>(in[i].y, 1, up));
+                const uint4 y = make_uint4(widen_pair<T>(in[i].z, 0, up), widen_pair<T>(in[i].z, 1, up),
+                                           widen_pair<T>(in[i].w, 0, up), widen_pair<T>(in[i].w, 1, up));
+                *reinterpret_cast<uint4*>(dst + to) = x;
+                *reinterpret_cast<uint4*>(dst + (to ^ 16u)) = y;
               }
             } else {
-              const float scale = scale_value(codes[kv]);
+              // a scale beyond the type's normal numbers, or NaN: through f32
+              const float scale = scale_value(code);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 x = from_e4m3x2(in[e] & 0xffffu), y = from_e4m3x2(in[e] >> 16);
-                w[2 * e] = Elem<T>::pack(x.x * scale, x.y * scale);
-                w[2 * e + 1] = Elem<T>::pack(y.x * scale, y.y * scale);
+              for (int i = 0; i < kPieces; ++i) {
+                const uint32_t to = (dst_at ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
+                const uint32_t word[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  uint32_t o[4];
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const float2 x = from_e4m3x2(word[2 * h + e] & 0xffffu), y = from_e4m3x2(word[2 * h + e] >> 16);
+                    o[2 * e] = Elem<T>::pack(x.x * scale, x.y * scale);
+                    o[2 * e + 1] = Elem<T>::pack(y.x * scale, y.y * scale);
+                  }
+                  *reinterpret_cast<uint4*>(dst + (to ^ (uint32_t)(h << 4))) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
               }
             }
-            if (!real) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = 0u;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(kv ? &v_full[s] : &k_full[s]);
+              mbar_arrive(&raw_empty[rs]);
             }
-            const int c0 = 2 * c;  // two 16-byte pieces of the 16-bit row
-            uint8_t* box = dst + (c0 >> 3) * KBOX;
-            *reinterpret_cast<uint4*>(box + (((c0 & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(box + ((((c0 & 7) + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            if (++rs == R) rs = 0, rph ^= 1;
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(kv ? &v_full[s] : &k_full[s]);
-            mbar_arrive(&raw_empty[rs]);
-          }
-          if (++rs == R) rs = 0, rph ^= 1;
+          if (!ok) break;
+          kc = kc_next, vc = vc_next;
         }
-        codes[0] = next_codes[0], codes[1] = next_codes[1];
       }
     }
   } else {
     if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    // ---------------- softmax + epilogue (attention_tc.cu) ----------------
+    // ---------------- softmax + epilogue (attention_tc_p.cu) ----------------
     const int i = (warp - 4) >> 2;  // query tile
     const int quarter = warp & 3;   // TMEM lane quarter
-    const Range r = i == 0 ? r0 : r1;
     const int tile_row = quarter * 32 + lane;
-    const int t_first = t0 + i * p.tile_tokens;
-    const int t_row = t_first + tile_row / p.group;
-    const int head = hk * p.group + tile_row % p.group;
-    const bool row_ok = tile_row < p.tile_tokens * p.group && t_row < a.t;  // a row of the output
-    const bool row_real = row_ok && t_row < n_live;
+    const int row_token = tile_row / p.group, row_head = tile_row % p.group;
+    const bool in_tile = tile_row < p.tile_tokens * p.group;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t o_tmem = tmem_base + 256 + i * D + lane_addr;
     const float sl2 = p.scale_log2;
-    const int vis_lo = row_real ? first_of(t_row) : 0, vis_hi = row_real ? last_of(t_row) : 0;
-    // keys that every live token of the tile sees
-    const bool has = i == 0 ? has0 : has1;
-    const int all_lo = has ? first_of(last_token(t_first)) : 0, all_hi = has ? last_of(t_first) : 0;
-    auto vis_word = [&](int base) -> uint32_t {
-      int x = vis_lo - base, y = vis_hi - base;
-      x = x < 0 ? 0 : x;
-      y = y > 32 ? 32 : y;
-      uint32_t w = 0;
-      if (y > x) w = (y == 32 ? 0xffffffffu : ((1u << y) - 1u)) & ~((1u << x) - 1u);
-      return w;
-    };
-    float m_run = -INFINITY;  // running maximum, scaled log2 units
-    float l_run = 0.f;
-    bool ok = true;
-    const int nblk = r.hi - r.lo;
-    // turns on the MUFU unit, as in attention_tc.cu
-    const int n_paired = paired_blocks(r0, r1);
     const int my_turn = 1 + i * 4 + quarter;
     const int other_turn = 1 + (1 - i) * 4 + quarter;
-    int turns_done = 0;
-    uint32_t sr[2][32];
-    bool requested = false;
-    for (int j = r.lo; j < r.hi; ++j) {
-      const int n = j - r.lo;
-      const int buf = n & 1;
-      turns_done = n;
-      const uint32_t s_tmem = tmem_base + (uint32_t)((i * 2 + buf) * kBKV) + lane_addr;
-      if (!requested) {
-        if (!mbar_wait(&s_full[i * 2 + buf], (uint32_t)((n >> 1) & 1), a.status)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        tmem_ld32(s_tmem, sr[0]);
-        tmem_ld32(s_tmem + 32, sr[1]);
+    uint32_t my_blocks = 0;   // blocks of this tile in all earlier items
+    uint32_t tail_count = 0;  // tail commits of this tile in all earlier items
+    // Turns on the MUFU unit (attention_tc.cu): tile 0 takes its n-th block that both tiles have,
+    // then tile 1 its own, and so on from item to item. A named barrier counts arrivals and does
+    // not know their turn: were a warp to arrive twice before its partner has waited once, the
+    // two arrivals would complete the barrier between them and the partner would wait for good
+    // (short items, where tile 0 finds its next item before tile 1 has begun this one's last
+    // block). So each side waits for the other's last turn before every one of its own, the
+    // CTA's first excepted, and a warp whose bounded wait ran out walks all turns on.
+    uint32_t turns = 0;       // of all earlier items and this one
+    bool ok = true;           // false once a bounded wait ran out: nothing is computed from then on
+    for (uint32_t n_it = 0;; ++n_it) {
+      const int slot = (int)(n_it & 1);
+      if (!mbar_wait_patient(&item_full[slot], (n_it >> 1) & 1, a.status)) {
+        for (int64_t m = 0; m < 2 * (capacity / kBKV + 2); ++m) named_barrier_arrive(other_turn, 64);
+        break;
       }
-      const int j0 = j * kBKV;
-      const bool need_mask = j0 < all_lo || j0 + kBKV > all_hi;
-      tmem_ld_wait_for(sr[0]);
-      tmem_ld_wait_for(sr[1]);
-      if (need_mask) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t vw = vis_word(j0 + 32 * c);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (((vw >> e) & 1u) == 0) sr[c][e] = 0xff800000u;
+      const PagedWork w = item_ring[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      if (!w.valid) break;
+      const int n_paired = paired_blocks(w.r0, w.r1);
+      int turns_done = 0;     // of this item
+      bool my_turn_now = false;
+      auto take_turn = [&]() {
+        if (i == 1 || turns > 0) named_barrier(my_turn, 64);
+        my_turn_now = true;
+      };
+      auto pass_turn = [&]() {
+        named_barrier_arrive(other_turn, 64);
+        ++turns, ++turns_done;
+        my_turn_now = false;
+      };
+      auto walk_turns = [&]() {
+        while (turns_done < n_paired) {
+          if (!my_turn_now) take_turn();
+          pass_turn();
         }
+      };
+      if (!ok) {
+        walk_turns();
+        continue;
       }
-      float mx;
-      {
-        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+      const Range r = i == 0 ? w.r0 : w.r1;
+      const int nblk = r.hi - r.lo;
+      const int t_first = w.t0 + i * p.tile_tokens, t_row = t_first + row_token;
+      const bool row_ok = in_tile && t_row < a.t;  // a row of the output
+      const bool row_real = row_ok && t_row < w.n_live;
+      const int64_t end = (int64_t)w.start + w.n_live;
+      const int vis_lo = row_real ? first_key(a, (int64_t)w.start + t_row) : 0;
+      const int vis_hi = row_real ? last_key(a, (int64_t)w.start + t_row, end) : 0;
+      // keys that every live token of the tile sees
+      const int t_last = min(t_first + p.tile_tokens, w.n_live) - 1;
+      const int all_lo = first_key(a, (int64_t)w.start + t_last), all_hi = last_key(a, (int64_t)w.start + t_first, end);
+      auto vis_word = [&](int base) -> uint32_t {
+        int x = vis_lo - base, y = vis_hi - base;
+        x = x < 0 ? 0 : x;
+        y = y > 32 ? 32 : y;
+        uint32_t word = 0;
+        if (y > x) word = (y == 32 ? 0xffffffffu : ((1u << y) - 1u)) & ~((1u << x) - 1u);
+        return word;
+      };
+      float m_run = -INFINITY;  // running maximum, scaled log2 units
+      float l_run = 0.f;
+      uint32_t sr[2][32];
+      bool requested = false;
+      for (int j = r.lo; j < r.hi && ok; ++j) {
+        const int n = j - r.lo;
+        const uint32_t N = my_blocks + (uint32_t)n;
+        const int buf = (int)(N & 1);
+        const uint32_t s_tmem = tmem_base + (uint32_t)((i * 2 + buf) * kBKV) + lane_addr;
+        if (!requested) {
+          if (!mbar_wait(&s_full[i * 2 + buf], (N >> 1) & 1, a.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          tmem_ld32(s_tmem, sr[0]);
+          tmem_ld32(s_tmem + 32, sr[1]);
+        }
+        const int j0 = j * kBKV;
+        const bool need_mask = j0 < all_lo || j0 + kBKV > all_hi;
+        tmem_ld_wait_for(sr[0]);
+        tmem_ld_wait_for(sr[1]);
+        if (need_mask) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t vw = vis_word(j0 + 32 * c);
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            m0 = max3(m0, __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
-            m1 = max3(m1, __uint_as_float(sr[c][e + 2]), __uint_as_float(sr[c][e + 3]));
-            m2 = max3(m2, __uint_as_float(sr[c][e + 4]), __uint_as_float(sr[c][e + 5]));
-            m3 = max3(m3, __uint_as_float(sr[c][e + 6]), __uint_as_float(sr[c][e + 7]));
+            for (int e = 0; e < 32; ++e)
+              if (((vw >> e) & 1u) == 0) sr[c][e] = 0xff800000u;
           }
         }
-        mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-      }
-      const float mx_t = mx * sl2;  // scale > 0 on this path
-      float m_new = m_run;
-      if (mx_t > m_run + kRescaleAbove || m_run == -INFINITY) m_new = fmaxf(m_run, mx_t);
-      bool tail0_seen = false;
-      const bool moved = m_new != m_run && m_run != -INFINITY;
-      const float corr = moved ? ex2_approx(m_run - m_new) : 1.0f;
-      if (__any_sync(0xffffffffu, moved)) {
-        const bool landed = n + 1 < nblk
-                                ? mbar_wait(&s_full[i * 2 + ((n + 1) & 1)], (uint32_t)(((n + 1) >> 1) & 1), a.status)
-                                : mbar_wait(&tail_done[i], 0, a.status);
-        if (!landed) {
+        float mx;
+        {
+          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              m0 = max3(m0, __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+              m1 = max3(m1, __uint_as_float(sr[c][e + 2]), __uint_as_float(sr[c][e + 3]));
+              m2 = max3(m2, __uint_as_float(sr[c][e + 4]), __uint_as_float(sr[c][e + 5]));
+              m3 = max3(m3, __uint_as_float(sr[c][e + 6]), __uint_as_float(sr[c][e + 7]));
+            }
+          }
+          mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        }
+        const float mx_t = mx * sl2;  // scale > 0 on this path
+        float m_new = m_run;
+        if (mx_t > m_run + kRescaleAbove || m_run == -INFINITY) m_new = fmaxf(m_run, mx_t);
+        bool tail0_seen = false;
+        const bool moved = m_new != m_run && m_run != -INFINITY;
+        const float corr = moved ? ex2_approx(m_run - m_new) : 1.0f;
+        if (__any_sync(0xffffffffu, moved)) {
+          const uint32_t Nn = N + 1;
+          const bool landed = n + 1 < nblk ? mbar_wait(&s_full[i * 2 + (int)(Nn & 1)], (Nn >> 1) & 1, a.status)
+                                           : mbar_wait(&tail_done[i], tail_count & 1, a.status);
+          if (!landed) {
+            ok = false;
+            break;
+          }
+          tail0_seen = n + 1 == nblk;
+          tc_fence_after();
+          l_run *= corr;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t orr[32];
+            tmem_ld32(o_tmem + c, orr);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * corr);
+            tmem_st32(o_tmem + c, orr);
+          }
+          tmem_st_wait();
+        }
+        m_run = m_new;
+        float m_use = m_run == -INFINITY ? 0.f : m_run;
+        if (n < n_paired) {
+          take_turn();
+          asm volatile("" : "+f"(m_use));  // keeps the exponentials below the barrier
+        }
+        const float2 sl2_2 = make_float2(sl2, sl2), nm_2 = make_float2(-m_use, -m_use);
+        float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+        uint32_t pk[32];
+        constexpr int kLag = 6;
+        float2 xs[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          xs[k] = __ffma2_rn(make_float2(__uint_as_float(sr[k >> 4][2 * (k & 15)]),
+                                         __uint_as_float(sr[k >> 4][2 * (k & 15) + 1])),
+                             sl2_2, nm_2);
+#pragma unroll
+        for (int k = 0; k < 32 + kLag; ++k) {
+          if (k < 32) {
+            xs[k].x = ex2_approx(xs[k].x);
+            xs[k].y = ex2_approx(xs[k].y);
+          }
+          if (k >= kLag) {
+            const int d = k - kLag;
+            if (d & 1) lb = __fadd2_rn(lb, xs[d]);
+            else la = __fadd2_rn(la, xs[d]);
+            pk[d] = Elem<T>::pack(xs[d].x, xs[d].y);
+          }
+        }
+        tmem_st32(s_tmem, pk);
+        if (n < n_paired) pass_turn();
+        l_run += (la.x + la.y) + (lb.x + lb.y);
+        requested = false;
+        if (n + 1 < nblk) {
+          const uint32_t Nn = N + 1;
+          if (mbar_test_wait(&s_full[i * 2 + (int)(Nn & 1)], (Nn >> 1) & 1)) {
+            tc_fence_after();
+            const uint32_t next_tmem = tmem_base + (uint32_t)((i * 2 + (int)(Nn & 1)) * kBKV) + lane_addr;
+            tmem_ld32(next_tmem, sr[0]);
+            tmem_ld32(next_tmem + 32, sr[1]);
+            requested = true;
+          }
+        }
+        tmem_st_wait();
+        if (n + 1 == nblk && nblk >= 2 && !tail0_seen && !mbar_wait(&tail_done[i], tail_count & 1, a.status)) {
           ok = false;
           break;
         }
-        tail0_seen = n + 1 == nblk;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i * 2 + buf]);
+      }
+      if (!ok) {
+        walk_turns();
+        continue;
+      }
+      // ---- epilogue: O / l, zeros in rows without a key; or a part's state ----
+      const int head = w.hk * p.group + row_head;
+      float* part = w.part < 0 ? nullptr : p.parts + ((int64_t)blockIdx.x * 2 + w.part) * kPartFloats<D>;
+      const int row = i * 128 + tile_row;
+      if (!row_real) l_run = 0.f;
+      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+      T* orow = (T*)a.o + (int64_t)w.b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh;
+      if (nblk > 0) {
+        // the last P.V: the item's second tail commit (its only one for a one-block tile)
+        const uint32_t last = tail_count + (nblk >= 2 ? 1u : 0u);
+        if (!mbar_wait(&tail_done[i], last & 1, a.status)) {
+          ok = false;  // the item's hand-over sequence is complete: drain from the next item on
+          continue;
+        }
         tc_fence_after();
-        l_run *= corr;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t orr[32];
           tmem_ld32(o_tmem + c, orr);
           tmem_ld_wait();
+          if (part != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * corr);
-          tmem_st32(o_tmem + c, orr);
-        }
-        tmem_st_wait();
-      }
-      m_run = m_new;
-      float m_use = m_run == -INFINITY ? 0.f : m_run;
-      if (n < n_paired && (i == 1 || n > 0)) {
-        named_barrier(my_turn, 64);
-        asm volatile("" : "+f"(m_use));  // keeps the exponentials below the barrier
-      }
-      const float2 sl2_2 = make_float2(sl2, sl2), nm_2 = make_float2(-m_use, -m_use);
-      float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
-      uint32_t pk[32];
-      constexpr int kLag = 6;
-      float2 xs[32];
-#pragma unroll
-      for (int k = 0; k < 32; ++k)
-        xs[k] = __ffma2_rn(make_float2(__uint_as_float(sr[k >> 4][2 * (k & 15)]),
-                                       __uint_as_float(sr[k >> 4][2 * (k & 15) + 1])),
-                           sl2_2, nm_2);
-#pragma unroll
-      for (int k = 0; k < 32 + kLag; ++k) {
-        if (k < 32) {
-          xs[k].x = ex2_approx(xs[k].x);
-          xs[k].y = ex2_approx(xs[k].y);
-        }
-        if (k >= kLag) {
-          const int d = k - kLag;
-          if (d & 1) lb = __fadd2_rn(lb, xs[d]);
-          else la = __fadd2_rn(la, xs[d]);
-          pk[d] = Elem<T>::pack(xs[d].x, xs[d].y);
-        }
-      }
-      tmem_st32(s_tmem, pk);
-      if (n < n_paired && (i == 0 || n + 1 < n_paired)) named_barrier_arrive(other_turn, 64);
-      turns_done = n + 1;
-      l_run += (la.x + la.y) + (lb.x + lb.y);
-      requested = false;
-      if (n + 1 < nblk && mbar_test_wait(&s_full[i * 2 + (buf ^ 1)], (uint32_t)(((n + 1) >> 1) & 1))) {
-        tc_fence_after();
-        const uint32_t next_tmem = tmem_base + (uint32_t)((i * 2 + (buf ^ 1)) * kBKV) + lane_addr;
-        tmem_ld32(next_tmem, sr[0]);
-        tmem_ld32(next_tmem + 32, sr[1]);
-        requested = true;
-      }
-      tmem_st_wait();
-      if (n + 1 == nblk && nblk >= 2 && !tail0_seen && !mbar_wait(&tail_done[i], 0, a.status)) {
-        ok = false;
-        break;
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[i * 2 + buf]);
-    }
-    if (!ok) {
-      for (int m = turns_done; m < n_paired; ++m)
-        if (i == 0 || m + 1 < n_paired) named_barrier_arrive(other_turn, 64);
-    }
-    // the last P.V: the tail barrier's second phase (its only one for a one-block tile)
-    if (r.hi > r.lo && ok) ok = mbar_wait(&tail_done[i], nblk >= 2 ? 1u : 0u, a.status);
-    tc_fence_after();
-    if (csize == 1) {
-      // ---- epilogue: O / l; zeros where no key reaches a row ----
-      if (!row_real) l_run = 0.f;
-      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-      T* orow = (T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh;
-      const bool any = r.hi > r.lo;
-      if (ok) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t orr[32];
-          if (any) {
-            tmem_ld32(o_tmem + c, orr);
-            tmem_ld_wait();
-          }
-          if (row_ok) {
+            for (int e = 0; e < 32; ++e) part[(c + e) * 256 + row] = __uint_as_float(orr[e]);
+          } else if (row_ok) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               if (c + v * 8 >= a.c.d) break;  // padded head dim: nothing past the real columns
-              uint32_t w[4] = {0u, 0u, 0u, 0u};
-              if (any && l_run != 0.f) {
+              uint32_t o[4] = {0u, 0u, 0u, 0u};
+              if (l_run != 0.f) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  w[e] = Elem<T>::pack(__uint_as_float(orr[v * 8 + 2 * e]) * inv, __uint_as_float(orr[v * 8 + 2 * e + 1]) * inv);
+                  o[e] = Elem<T>::pack(__uint_as_float(orr[v * 8 + 2 * e]) * inv, __uint_as_float(orr[v * 8 + 2 * e + 1]) * inv);
               }
-              stg128(orow + c + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
+              stg128(orow + c + v * 8, make_uint4(o[0], o[1], o[2], o[3]));
             }
           }
         }
+        // O is read out: the next live item's first P.V may overwrite it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[i]);
+        my_blocks += (uint32_t)nblk;
+        tail_count += nblk >= 2 ? 2u : 1u;
+      } else if (part == nullptr && row_ok) {
+        for (int c = 0; c < a.c.d; c += 8) stg128(orow + c, make_uint4(0, 0, 0, 0));
       }
-      if (a.lse != nullptr && row_ok && ok)
-        a.lse[((int64_t)b * a.heads + head) * a.t + t_row] = l_run == 0.f ? -INFINITY : kLn2F * (m_run + log2f(l_run));
-    } else {
-      // ---- this share's state into shared memory, [column][row]: every MMA of both tiles is done ----
-      named_barrier(9, 256);
-      float* op = reinterpret_cast<float*>(smem);
-      const int row = i * 128 + tile_row;
-      if (r.hi > r.lo) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t orr[32];
-          tmem_ld32(o_tmem + c, orr);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) op[(c + e) * 256 + row] = __uint_as_float(orr[e]);
-        }
+      if (part != nullptr) {
+        part[D * 256 + row] = m_run;
+        part[D * 256 + 256 + row] = l_run;
+      } else if (a.lse != nullptr && row_ok) {
+        a.lse[((int64_t)w.b * a.heads + head) * a.t + t_row] = l_run == 0.f ? -INFINITY : kLn2F * (m_run + log2f(l_run));
       }
-      ml_s[row] = m_run;
-      ml_s[256 + row] = r.hi > r.lo ? l_run : 0.f;
     }
   }
 
@@ -692,53 +925,58 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
-  if (csize > 1) {
-    cluster_sync_all();
-    if (warp >= 4 && warp < 12) {
-      const int tid = threadIdx.x - 128;
-      const uint32_t op_addr = smem_u32(smem), ml_addr = smem_u32(ml_s);
-      // a thread: eight columns of a row; a warp 32 rows, so that its reads are whole lines
-      for (int w = (int)rank * 256 + tid; w < 256 * (a.c.d / 8); w += (int)csize * 256) {
-        const int row = w & 255, d0 = (w >> 8) * 8;
-        const int in_tile = row & 127;
-        const int t_row = t0 + (row >> 7) * p.tile_tokens + in_tile / p.group;
-        const int head = hk * p.group + in_tile % p.group;
-        if (in_tile >= p.tile_tokens * p.group || t_row >= a.t) continue;
-        float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (t_row < n_live) {
-          for (uint32_t k = 0; k < csize; ++k) m = fmaxf(m, ld_cluster_f32(cluster_at(ml_addr + row * 4, k)));
-          for (uint32_t k = 0; k < csize; ++k) {
-            const float mr = ld_cluster_f32(cluster_at(ml_addr + row * 4, k));
-            const float lr = ld_cluster_f32(cluster_at(ml_addr + (256 + row) * 4, k));
-            if (lr == 0.f) continue;  // the share saw no key of this row
-            const float f = mr == -INFINITY ? 1.f : ex2_approx(mr - m);
-            l = fmaf(f, lr, l);
-            const uint32_t src = cluster_at(op_addr + (uint32_t)(d0 * 256 + row) * 4, k);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, ld_cluster_f32(src + e * 1024), acc[e]);
-          }
-        }
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        stg128((T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh + d0,
-               make_uint4(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[2] * inv, acc[3] * inv),
-                          Elem<T>::pack(acc[4] * inv, acc[5] * inv), Elem<T>::pack(acc[6] * inv, acc[7] * inv)));
-        if (a.lse != nullptr && d0 == 0)
-          a.lse[((int64_t)b * a.heads + head) * a.t + t_row] = l == 0.f ? -INFINITY : kLn2F * (m + log2f(l));
-      }
-    }
-    cluster_sync_all();  // no CTA leaves while a peer still reads its state
-  }
 }
 
-int sm_count_paged() {
-  static int n = 0;
-  if (n == 0) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (n <= 0) n = 148;
+// The parts of the items that more than one CTA had: block (CTA, eight columns), a thread a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attention_paged_merge_kernel(const __grid_constant__ PagedTcParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const PagedAttnArgs& a = p.a;
+  const int* h = p.heads_of_split + (int64_t)blockIdx.x * kSplitInts;
+  if (h[0] == 0) return;
+  const int b = h[1], hk = h[2], t0 = h[3], n_live = h[4], last = h[5];
+  const int row = threadIdx.x, d0 = blockIdx.y * 8;
+  const int in_tile = row & 127;
+  const int t_row = t0 + (row >> 7) * p.tile_tokens + in_tile / p.group;
+  const int head = hk * p.group + in_tile % p.group;
+  if (in_tile >= p.tile_tokens * p.group || t_row >= a.t) return;
+  float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (t_row < n_live) {
+    // the first part lies in its CTA's second slot, the others in their CTAs' first
+    auto part_of = [&](int k) { return p.parts + ((int64_t)k * 2 + (k == (int)blockIdx.x ? 1 : 0)) * kPartFloats<D>; };
+    for (int k = blockIdx.x; k <= last; ++k) m = fmaxf(m, part_of(k)[D * 256 + row]);
+    for (int k = blockIdx.x; k <= last; ++k) {
+      const float* part = part_of(k);
+      const float mr = part[D * 256 + row], lr = part[D * 256 + 256 + row];
+      if (lr == 0.f) continue;  // no key of this row there (NaN scores leave the maximum at -inf, the sum says so)
+      const float f = mr == -INFINITY ? 1.f : ex2_approx(mr - m);
+      l = fmaf(f, lr, l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, part[(d0 + e) * 256 + row], acc[e]);
+    }
   }
-  return n;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  stg128((T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh + d0,
+         make_uint4(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[2] * inv, acc[3] * inv),
+                    Elem<T>::pack(acc[4] * inv, acc[5] * inv), Elem<T>::pack(acc[6] * inv, acc[7] * inv)));
+  if (a.lse != nullptr && d0 == 0)
+    a.lse[((int64_t)b * a.heads + head) * a.t + t_row] = l == 0.f ? -INFINITY : kLn2F * (m + log2f(l));
+}
+
+// One CTA an SM.
+int grid_of(const PagedAttnArgs&) {
+  static int n[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& sms = n[dev & 63];
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+      cudaGetLastError();
+      sms = 148;
+    }
+  }
+  return sms;
 }
 
 template <typename T, bool Q8, int D>
@@ -750,6 +988,10 @@ int run(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   p.tile_tokens = 128 / p.group;
   p.box = page_box(a.c.page_size, kBKV);
   p.scale_log2 = a.scale * kLog2eF;
+  p.n_qt = (int)((a.t + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens));
+  const int grid = grid_of(a);
+  p.parts = (float*)a.workspace;
+  p.heads_of_split = (int*)(p.parts + (int64_t)grid * 2 * kPartFloats<D>);
   CUtensorMap tq, tk, tv;
   {
     const uint64_t dims[4] = {(uint64_t)a.c.d, (uint64_t)a.heads, (uint64_t)a.t, (uint64_t)a.batch};
@@ -769,20 +1011,13 @@ int run(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
       return -1;
     attr_seen[dev & 63] = true;
   }
-  const int64_t n_qt = (a.t + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-  const int64_t pairs = a.batch * a.c.kv_heads, items = pairs * n_qt;
-  int64_t keys = a.c.width * a.c.page_size;
-  if (a.has_window) {
-    const int64_t w = a.win_left + 2 * p.tile_tokens + (a.causal ? 0 : a.win_right) + kBKV;
-    keys = w < keys ? w : keys;
-  }
-  const int64_t blocks = (keys + kBKV - 1) / kBKV;
-  int csize = 1;
-  while (csize < 8 && items * csize * 2 <= sm_count_paged() && blocks >= 4 * csize * 2) csize *= 2;
-  if (launch_pdl(attention_paged_tc_kernel<T, Q8, D>, dim3((unsigned)(pairs * csize), (unsigned)n_qt), dim3(C::kThreads),
-                 C::kSmem, s, (unsigned)csize, a.batch * a.t, tq, tk, tv, p) != cudaSuccess)
+  if (launch_pdl(attention_paged_tc_kernel<T, Q8, D>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1,
+                 a.batch * a.t, tq, tk, tv, p) != cudaSuccess)
     return -1;
-  snprintf(cfg, cfg_len, "{bq:%d,bkv:%d,d:%d,box:%d,cluster:%d%s}", 2 * kBQ, kBKV, a.c.d, p.box, csize, Q8 ? ",e4m3" : "");
+  if (launch_pdl(attention_paged_merge_kernel<T, D>, dim3((unsigned)grid, (unsigned)(a.c.d / 8)), dim3(256), 0, s, 1,
+                 a.batch * a.t, p) != cudaSuccess)
+    return -1;
+  snprintf(cfg, cfg_len, "{bq:%d,bkv:%d,d:%d,box:%d,grid:%d%s}", 2 * kBQ, kBKV, a.c.d, p.box, grid, Q8 ? ",e4m3" : "");
   return 0;
 }
 
@@ -798,11 +1033,14 @@ int run_type(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) 
 bool attention_paged_tc_covers(const PagedAttnArgs& a) {
   if (!attention_paged_tiles(a)) return false;
   const int64_t group = a.heads / a.c.kv_heads;
-  if (group > 128 || a.batch * a.c.kv_heads > (1 << 26) || a.t > 0x7fffff00LL) return false;
+  if (group > 128 || a.batch > 0x7fffff00LL || a.t > 0x7fffff00LL) return false;
   // the query rows come by a tensor map, which has no stride of zero (an expanded view)
-  if ((a.heads > 1 && a.q_sh == 0) || (a.t > 1 && a.q_st == 0) || (a.batch > 1 && a.q_sb == 0)) return false;
-  const int64_t tokens = 2 * (128 / group);
-  return (a.t + tokens - 1) / tokens <= 65535;
+  return !((a.heads > 1 && a.q_sh == 0) || (a.t > 1 && a.q_st == 0) || (a.batch > 1 && a.q_sb == 0));
+}
+
+size_t attention_paged_tc_workspace(const PagedAttnArgs& a) {
+  const int64_t part = a.c.d > 64 ? kPartFloats<128> : kPartFloats<64>;
+  return (size_t)grid_of(a) * (2 * (size_t)part * sizeof(float) + kSplitInts * sizeof(int));
 }
 
 int launch_attention_paged_tc(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {

@@ -276,6 +276,7 @@ struct PagedAttnArgs {
   const int32_t* lens;  // nullable
   float* lse;           // [B, H, T], nullable
   uint32_t* status;
+  void* workspace;      // what the kernel that takes the call wants of it
 };
 // Every float type, head width up to 256, page size and alignment.
 int launch_attention_paged_exact(const PagedAttnArgs& a, cudaStream_t s);
@@ -286,6 +287,7 @@ bool attention_paged_decode_covers(const PagedAttnArgs& a);
 int launch_attention_paged_decode(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len);
 // Any number of query rows: 128-row tiles of tokens x the heads of a KV head.
 bool attention_paged_tc_covers(const PagedAttnArgs& a);
+size_t attention_paged_tc_workspace(const PagedAttnArgs& a);
 int launch_attention_paged_tc(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len);
 // Keys of the largest run that divides a page and `most`: no box of that many straddles pages.
 int page_box(int page_size, int most);
