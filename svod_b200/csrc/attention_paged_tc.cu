@@ -120,6 +120,15 @@ __device__ __forceinline__ int live_items(const PagedTcParams& p, const Row& r) 
   return (r.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
 // Two e4m3 values, bytes 0 and 1 (or 2 and 3) of `w`, as a 16-bit pair whose exponent bias is
 // still e4m3's; the multiply by `up` (2^120 or 2^8 times the row's scale) puts it right.
 template <typename T>
@@ -194,7 +203,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       mbar_init(&tail_done[i], 1);
       mbar_init(&o_empty[i], 4);                // the tile's four softmax warps
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], Q8 ? 14 : 10);  // two issuers, eight softmax warps, four widening ones
+      mbar_init(&item_empty[i], Q8 ? 15 : 11);  // query loader, two issuers, eight softmax warps, four widening ones
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -288,7 +297,6 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       const bool mine = my_col < kCols;
       int s = 0;  // ring slot of the next block (16-bit pages) or copy (8-bit)
       uint32_t ph = 0;
-      uint32_t q_items[2] = {0, 0};  // live items so far, per tile
       bool ok = true;
       auto wait_by_lane0 = [&](uint64_t* bar, uint32_t parity) {
         bool done = true;
@@ -356,18 +364,6 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
           };
           int next_at;
           int next_id = look_up(w.u_lo, next_at);
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (!(i == 0 ? live0 : live1)) continue;
-            // the issuer's last QK of the tile's previous live item has read this Q tile
-            if (!wait_by_lane0(&q_empty[i], (q_items[i] & 1) ^ 1)) break;
-            ++q_items[i];
-            if (lane == 0) {
-              mbar_expect_tx(&q_full[i], (uint32_t)(p.tile_tokens * p.group * 128 * (D / 64)));
-              for (int c = 0; c < D / 64; ++c)
-                tma_load_4d(q_s + i * QB + c * (128 * 128), &tmap_q, &q_full[i], c * 64, hk * p.group,
-                            w.t0 + i * p.tile_tokens, b);
-            }
-          }
           for (int j = w.u_lo; j < w.u_hi && ok; ++j) {
             const int id = next_id, at = next_at;
             next_id = look_up(j + 1, next_at);
@@ -417,20 +413,35 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       if (!ok)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA's memory goes
     } else if (warp == 2) {
-      // ---------------- rows behind a chunk's real tokens that no item has: zeros ----------------
-      const int step = 2 * p.tile_tokens;
-      for (int64_t u = blockIdx.x; u < a.batch * p.n_qt; u += gridDim.x) {
-        const int64_t b = u / p.n_qt;
-        const int t0 = (int)(u % p.n_qt) * step;
-        const Row r = row_of(a.start, a.lens, b, a.t, capacity);
-        if (t0 < r.n) continue;
-        const int pieces = a.c.d / 8, rows = (int)(a.t - t0 < step ? a.t - t0 : step) * a.heads;
-        for (int i = lane; i < rows * pieces; i += 32) {
-          const int rw = i / pieces, t = t0 + rw / a.heads, h = rw % a.heads;
-          stg128((T*)a.o + b * a.o_sb + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + (i % pieces) * 8, make_uint4(0, 0, 0, 0));
-          if (a.lse != nullptr && i % pieces == 0) a.lse[(b * a.heads + h) * a.t + t] = -INFINITY;
+      // ---------------- query tiles: a warp of its own, so that an item's first keys do not wait ----------------
+      // ---------------- until the last one's last scores have read the tile ----------------
+      if (lane == 0) {
+        uint32_t q_items[2] = {0, 0};  // live items so far, per tile
+        bool ok = true;
+        for (uint32_t n_it = 0; ok; ++n_it) {
+          const int slot = (int)(n_it & 1);
+          if (!mbar_wait(&item_full[slot], (n_it >> 1) & 1, a.status)) break;
+          const PagedWork w = item_ring[slot];
+          mbar_arrive(&item_empty[slot]);
+          if (!w.valid) break;
+          for (int i = 0; i < 2; ++i) {
+            if (i == 0 ? w.r0.hi <= w.r0.lo : w.r1.hi <= w.r1.lo) continue;
+            // the issuer's last QK of the tile's previous live item has read this Q tile
+            if (!mbar_wait(&q_empty[i], (q_items[i] & 1) ^ 1, a.status)) {
+              ok = false;
+              break;
+            }
+            ++q_items[i];
+            mbar_expect_tx(&q_full[i], (uint32_t)(p.tile_tokens * p.group * 128 * (D / 64)));
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(q_s + i * QB + c * (128 * 128), &tmap_q, &q_full[i], c * 64, w.hk * p.group,
+                          w.t0 + i * p.tile_tokens, w.b);
+          }
         }
+        if (!ok)
+          for (int i = 0; i < 64; ++i) __nanosleep(1000);
       }
+      __syncwarp();
     } else {
       // ---------------- MMA issuers: warp 1 drives tile 0, warp 3 tile 1 (attention_tc_p.cu) ----------------
       const int i = warp == 1 ? 0 : 1;
@@ -545,7 +556,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       }
     }
   } else if (Q8 && warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ---------------- widening: raw e4m3 blocks into the 16-bit rings ----------------
     if constexpr (Q8) {
       const int tid = threadIdx.x - 384;
@@ -590,7 +601,10 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         codes_of(id_of(key, page), slot, kc, vc);
         step();
         int id_next = w.u_lo + 1 < w.u_hi ? id_of(key + kBKV, page) : -1;
-        for (int j = w.u_lo; j < w.u_hi; ++j, ++pos, key += kBKV) {
+        // One copy of the code for K and V, the rare path rolled up: with both unrolled the
+        // roles' code no longer stays in the instruction cache and these warps, which run
+        // theirs once a block, wait for every line of it (1100 cycles for 180 instructions).
+        for (int j = w.u_lo; j < w.u_hi && ok; ++j, ++pos, key += kBKV) {
           uint32_t kc_next, vc_next;
           codes_of(id_next, slot, kc_next, vc_next);
           step();
@@ -598,69 +612,86 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
           const int s = (int)(pos % S);
           const uint32_t ph = (pos / S) & 1;
           const bool real = key >= w.key_lo && key < w.key_hi;
-#pragma unroll
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
-            if (!mbar_wait(&raw_full[rs], rph, a.status) || !mbar_wait(kv ? &v_empty[s] : &k_empty[s], ph ^ 1, a.status)) {
+            if (!mbar_wait(&raw_full[rs], rph, a.status) || !mbar_wait((kv ? v_empty : k_empty) + s, ph ^ 1, a.status)) {
               ok = false;
               break;
             }
-            const uint8_t* src = raw_s + rs * C::kRawBytes;
-            uint8_t* dst = (kv ? v_s : k_s) + s * KB;
+            const uint32_t src = smem_u32(raw_s) + rs * C::kRawBytes + src_at;
+            const uint32_t dst = smem_u32(kv ? v_s : k_s) + s * KB + dst_at;
             const uint32_t code = kv ? vc : kc;
             // a slot beside the item's keys becomes zeros, whatever it holds: every pattern is finite here
             const uint32_t factor = widen_factor<T>(code), up = real ? factor : 0u;
-            uint4 in[kPieces];
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) in[i] = *reinterpret_cast<const uint4*>(src + (src_at ^ (uint32_t)(i << 4)));
             if (!real || factor != 0u) {
+              uint4 in[kPieces];
+#pragma unroll
+              for (int i = 0; i < kPieces; ++i) in[i] = lds128(src ^ (uint32_t)(i << 4));
 #pragma unroll
               for (int i = 0; i < kPieces; ++i) {
-                // piece i of 16 values: 32 bytes, the 16-byte pieces 2 i and 2 i + 1 behind dst_at's
-                const uint32_t to = (dst_at ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
-                const uint4 x = make_uint4(widen_pair<T>(in[i].x, 0, up), widen_pair<T>(in[i].x, 1, up),
-                                           widen_pair<T>(in[i].y, 0, up), widen_pair<T>(in[i].y, 1, up));
-                const uint4 y = make_uint4(widen_pair<T>(in[i].z, 0, up), widen_pair<T>(in[i].z, 1, up),
-                                           widen_pair<T>(in[i].w, 0, up), widen_pair<T>(in[i].w, 1, up));
-                *reinterpret_cast<uint4*>(dst + to) = x;
-                *reinterpret_cast<uint4*>(dst + (to ^ 16u)) = y;
+                // piece i of 16 values: 32 bytes, the 16-byte pieces 2 i and 2 i + 1 behind dst's
+                const uint32_t to = (dst ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
+                sts128(to, widen_pair<T>(in[i].x, 0, up), widen_pair<T>(in[i].x, 1, up), widen_pair<T>(in[i].y, 0, up),
+                       widen_pair<T>(in[i].y, 1, up));
+                sts128(to ^ 16u, widen_pair<T>(in[i].z, 0, up), widen_pair<T>(in[i].z, 1, up), widen_pair<T>(in[i].w, 0, up),
+                       widen_pair<T>(in[i].w, 1, up));
               }
             } else {
               // a scale beyond the type's normal numbers, or NaN: through f32
               const float scale = scale_value(code);
-#pragma unroll
+#pragma unroll 1
               for (int i = 0; i < kPieces; ++i) {
-                const uint32_t to = (dst_at ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
-                const uint32_t word[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
-#pragma unroll
+                const uint4 in = lds128(src ^ (uint32_t)(i << 4));
+                const uint32_t to = (dst ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
+#pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
-                  uint32_t o[4];
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    const float2 x = from_e4m3x2(word[2 * h + e] & 0xffffu), y = from_e4m3x2(word[2 * h + e] >> 16);
-                    o[2 * e] = Elem<T>::pack(x.x * scale, x.y * scale);
-                    o[2 * e + 1] = Elem<T>::pack(y.x * scale, y.y * scale);
-                  }
-                  *reinterpret_cast<uint4*>(dst + (to ^ (uint32_t)(h << 4))) = make_uint4(o[0], o[1], o[2], o[3]);
+                  const uint32_t wa = h ? in.z : in.x, wb = h ? in.w : in.y;
+                  const float2 x = from_e4m3x2(wa & 0xffffu), y = from_e4m3x2(wa >> 16);
+                  const float2 z = from_e4m3x2(wb & 0xffffu), u = from_e4m3x2(wb >> 16);
+                  sts128(to ^ (uint32_t)(h << 4), Elem<T>::pack(x.x * scale, x.y * scale), Elem<T>::pack(y.x * scale, y.y * scale),
+                         Elem<T>::pack(z.x * scale, z.y * scale), Elem<T>::pack(u.x * scale, u.y * scale));
                 }
               }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              mbar_arrive(kv ? &v_full[s] : &k_full[s]);
+              mbar_arrive((kv ? v_full : k_full) + s);
               mbar_arrive(&raw_empty[rs]);
             }
             if (++rs == R) rs = 0, rph ^= 1;
           }
-          if (!ok) break;
           kc = kc_next, vc = vc_next;
         }
       }
     }
   } else {
-    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    // (8-bit pages: 4 x 72 + 4 x 72 + 8 x 184 registers a lane are the 512 x 128 of the launch)
+    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- softmax + epilogue (attention_tc_p.cu) ----------------
+    // Rows behind a chunk's real tokens that no item has: zeros. An equal run of the batch's
+    // tokens a CTA and warp, while the first scores are on their way (one warp that clears an
+    // item's 128 tokens x 16 heads alone takes 150 us).
+    {
+      const int step = 2 * p.tile_tokens, pieces = a.c.d / 8;
+      const int64_t tokens = a.batch * a.t, runs = (int64_t)gridDim.x * 8, run = (tokens + runs - 1) / runs;
+      const int64_t me = (int64_t)blockIdx.x * 8 + warp - 4;
+      const int64_t last = run * (me + 1) < tokens ? run * (me + 1) : tokens;
+      for (int64_t u = run * me; u < last;) {
+        const int64_t b = u / a.t, row_lo = b * a.t, row_hi = row_lo + a.t < last ? row_lo + a.t : last;
+        const Row r = row_of(a.start, a.lens, b, a.t, capacity);
+        const int64_t dead = row_lo + (int64_t)live_items(p, r) * step;  // the row's first token without an item
+        for (u = u < dead ? dead : u; u < row_hi; ++u) {
+          T* o = (T*)a.o + b * a.o_sb + (u - row_lo) * a.o_st;
+          for (int x = lane; x < a.heads * pieces; x += 32)
+            stg128(o + (int64_t)(x / pieces) * a.o_sh + (x % pieces) * 8, make_uint4(0, 0, 0, 0));
+          if (a.lse != nullptr)
+            for (int h = lane; h < a.heads; h += 32) a.lse[(b * a.heads + h) * a.t + u - row_lo] = -INFINITY;
+        }
+        u = row_hi;
+      }
+    }
     const int i = (warp - 4) >> 2;  // query tile
     const int quarter = warp & 3;   // TMEM lane quarter
     const int tile_row = quarter * 32 + lane;
@@ -945,15 +976,19 @@ __global__ void __launch_bounds__(256) attention_paged_merge_kernel(const __grid
   if (t_row < n_live) {
     // the first part lies in its CTA's second slot, the others in their CTAs' first
     auto part_of = [&](int k) { return p.parts + ((int64_t)k * 2 + (k == (int)blockIdx.x ? 1 : 0)) * kPartFloats<D>; };
-    for (int k = blockIdx.x; k <= last; ++k) m = fmaxf(m, part_of(k)[D * 256 + row]);
     for (int k = blockIdx.x; k <= last; ++k) {
       const float* part = part_of(k);
       const float mr = part[D * 256 + row], lr = part[D * 256 + 256 + row];
-      if (lr == 0.f) continue;  // no key of this row there (NaN scores leave the maximum at -inf, the sum says so)
-      const float f = mr == -INFINITY ? 1.f : ex2_approx(mr - m);
-      l = fmaf(f, lr, l);
+      float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, part[(d0 + e) * 256 + row], acc[e]);
+      for (int e = 0; e < 8; ++e) x[e] = part[(d0 + e) * 256 + row];
+      if (lr == 0.f) continue;  // no key of this row there (NaN scores leave the maximum at -inf, the sum says so)
+      const float m_new = fmaxf(m, mr);
+      const float f0 = m == -INFINITY ? 1.f : ex2_approx(m - m_new), f1 = mr == -INFINITY ? 1.f : ex2_approx(mr - m_new);
+      l = fmaf(l, f0, f1 * lr);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], f0, f1 * x[e]);
+      m = m_new;
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
