@@ -50,7 +50,7 @@ using namespace fa_parts;
 using namespace paged;
 
 constexpr int kItemCost = 2;   // what an item costs beside its blocks, in blocks
-constexpr int kLeastShare = 8; // blocks a CTA takes at least, where there are few
+constexpr int kLeastShare = 4; // blocks (and items' costs) a CTA takes at least, where there are few
 
 template <bool Q8, int D>
 struct PagedTcCfg {
@@ -248,8 +248,12 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       };
       auto row_at = [&](int b) { return row_of(a.start, a.lens, b, a.t, capacity); };
       const int batch = (int)a.batch;
-      int64_t total = 0;
-      for (int b = lane; b < batch; b += 32) {
+      // lane l keeps row l: a batch of up to 32 rows is read and weighed once
+      const Row my_row = lane < batch ? row_at(lane) : Row{0, 0, false};
+      const int64_t my_weight = weigh(my_row);
+      if (my_row.bad && blockIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+      int64_t total = my_weight;
+      for (int b = lane + 32; b < batch; b += 32) {
         const Row r = row_at(b);
         if (r.bad && blockIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
         total += weigh(r);
@@ -260,6 +264,15 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       int64_t quota = (total + gridDim.x - 1) / gridDim.x;
       if (quota < kLeastShare) quota = kLeastShare;
       const int64_t c0 = quota * blockIdx.x, c1 = c0 + quota < total ? c0 + quota : total;
+      // Row b for the whole warp.
+      auto fetch_row = [&](int b) {
+        if (b >= 32) return row_at(b);
+        Row r;
+        r.start = __shfl_sync(0xffffffffu, my_row.start, b);
+        r.n = __shfl_sync(0xffffffffu, my_row.n, b);
+        r.bad = false;
+        return r;
+      };
       // Where the run begins: row b, KV head hk, item q, whose weight lies at [x, x + weight).
       int b = 0, hk = 0, q = 0;
       int64_t x = 0;
@@ -268,7 +281,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       if (c0 < c1) {
         int64_t base = 0;
         for (int b0 = 0; b0 < batch; b0 += 32) {
-          const int64_t w = b0 + lane < batch ? weigh(row_at(b0 + lane)) * a.c.kv_heads : 0;
+          const int64_t w = (b0 == 0 ? my_weight : b0 + lane < batch ? weigh(row_at(b0 + lane)) : 0) * a.c.kv_heads;
           int64_t upto = w;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -285,7 +298,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
           }
           base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        row = row_at(b);
+        row = fetch_row(b);
         hk = (int)((c0 - x) / row_weight);
         x += hk * row_weight;
         for (int64_t w = item_blocks(p, row, 0) + kItemCost; x + w <= c0; w = item_blocks(p, row, q) + kItemCost) x += w, ++q;
@@ -394,7 +407,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
           q = 0;
           if (++hk == a.c.kv_heads) {
             hk = 0;
-            do row = ++b < batch ? row_at(b) : Row{0, 0, false};
+            do row = ++b < batch ? fetch_row(b) : Row{0, 0, false};
             while (b < batch && row.n == 0);
             if (b >= batch) break;
           }
@@ -976,19 +989,28 @@ __global__ void __launch_bounds__(256) attention_paged_merge_kernel(const __grid
   if (t_row < n_live) {
     // the first part lies in its CTA's second slot, the others in their CTAs' first
     auto part_of = [&](int k) { return p.parts + ((int64_t)k * 2 + (k == (int)blockIdx.x ? 1 : 0)) * kPartFloats<D>; };
-    for (int k = blockIdx.x; k <= last; ++k) {
-      const float* part = part_of(k);
-      const float mr = part[D * 256 + row], lr = part[D * 256 + 256 + row];
-      float x[8];
+    // four parts' loads at a time: one after the other, each waits its microsecond
+    for (int k0 = blockIdx.x; k0 <= last; k0 += 4) {
+      float mr[4], lr[4], x[4][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = part[(d0 + e) * 256 + row];
-      if (lr == 0.f) continue;  // no key of this row there (NaN scores leave the maximum at -inf, the sum says so)
-      const float m_new = fmaxf(m, mr);
-      const float f0 = m == -INFINITY ? 1.f : ex2_approx(m - m_new), f1 = mr == -INFINITY ? 1.f : ex2_approx(mr - m_new);
-      l = fmaf(l, f0, f1 * lr);
+      for (int u = 0; u < 4; ++u) {
+        const bool there = k0 + u <= last;
+        const float* part = part_of(there ? k0 + u : last);
+        mr[u] = part[D * 256 + row];
+        lr[u] = there ? part[D * 256 + 256 + row] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], f0, f1 * x[e]);
-      m = m_new;
+        for (int e = 0; e < 8; ++e) x[u][e] = part[(d0 + e) * 256 + row];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (lr[u] == 0.f) continue;  // no key of this row there (NaN scores leave the maximum at -inf, the sum says so)
+        const float m_new = fmaxf(m, mr[u]);
+        const float f0 = m == -INFINITY ? 1.f : ex2_approx(m - m_new), f1 = mr[u] == -INFINITY ? 1.f : ex2_approx(mr[u] - m_new);
+        l = fmaf(l, f0, f1 * lr[u]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], f0, f1 * x[u][e]);
+        m = m_new;
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
