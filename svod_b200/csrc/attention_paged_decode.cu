@@ -75,15 +75,32 @@ struct PagedDecCfg {
   static constexpr int kTmemCols = 4 * NQ;
   static_assert(kSmem <= 232448, "beyond the 227 KiB a CTA may hold");
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "the CTAs of an SM fit its shared memory");
+  static_assert(kPBufs * kPBytes >= 4 * 1024, "the lengths of kSortedRows rows lie over the weights");
   static_assert(NQ * D * 4 <= kRing, "the partial outputs are laid over the ring");
 };
+
+// Rows of a batch that a CTA puts in order: their lengths fit the smallest weights' buffer.
+constexpr int kSortedRows = 1024;
 
 struct PagedDecParams {
   PagedAttnArgs a;
   int group, rows;  // rows = t * group query rows per KV head
   int box;          // keys of a box
+  int longest_first;  // rows in the order of their visible keys, where the grid does not fit the chip at once
   float scale_log2;
 };
+
+// Keys [lo, hi) that query token t of a row sees; both ends grow with t.
+__device__ __forceinline__ int first_seen(const PagedAttnArgs& a, const Row& r, int t) {
+  const int64_t x = a.has_window ? r.start + t - a.win_left : 0;
+  return (int)(x > 0 ? x : 0);
+}
+__device__ __forceinline__ int last_seen(const PagedAttnArgs& a, const Row& r, int t) {
+  int64_t x = r.start + r.n;
+  if (a.causal && r.start + t + 1 < x) x = r.start + t + 1;
+  if (a.has_window && r.start + t + a.win_right + 1 < x) x = r.start + t + a.win_right + 1;
+  return (int)x;
+}
 
 __device__ __forceinline__ uint32_t to_e5m2x2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E5M2);
@@ -115,7 +132,45 @@ __host__ __device__ constexpr uint32_t umma_idesc_f8(int a_fmt, int b_fmt, int m
          (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
-template <typename T, bool Q8, int D, int NQ>
+// W columns of 32-bit accumulators, in registers when the call returns.
+template <int W>
+__device__ __forceinline__ void tmem_ld_w(uint32_t at, uint32_t (&r)[W]) {
+  if constexpr (W == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+  } else if constexpr (W == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(at)
+                 : "memory");
+  } else {
+    tmem_ld16(at, r);
+  }
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < W; ++i) asm volatile("" : "+r"(r[i]));  // no use moves above the wait
+}
+template <int W>
+__device__ __forceinline__ void tmem_st_w(uint32_t at, const uint32_t (&r)[W]) {
+  if constexpr (W == 4) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3])
+                 : "memory");
+  } else if constexpr (W == 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else {
+    tmem_st16(at, r);
+  }
+}
+
+// NQ: rows of the MMAs; W: the columns of a chunk that softmax threads keep in registers, as
+// few as hold the query rows where these are 16 at most (a register each for scores and sums:
+// three CTAs an SM leave 96).
+template <typename T, bool Q8, int D, int NQ, int W>
 __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerSm))
     attention_paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                                   const __grid_constant__ PagedDecParams p) {
@@ -130,7 +185,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
   float* l_s = reinterpret_cast<float*>(p_s + C::kPBufs * C::kPBytes);  // [NQ][128] (NQ > 16)
   float* red = l_s + C::kLBytes / 4;                              // [NQ][4 warps]
   float* mc = red + NQ * 4;                                       // [2][NQ]: the maximum in use, the rescale factor
-  float* ml = mc + 2 * NQ;                                        // [2][NQ]: this CTA's m and l
+  float* ml = mc + 2 * NQ;                                        // [2][NQ]: this CTA's m (as it runs) and l
   float* fc = ml + 2 * NQ;                                        // [NQ]: log2 units a raw score
   int* lim = reinterpret_cast<int*>(fc + NQ);                     // [2][NQ]: a column's keys [lo, hi)
   int* vred = lim + 2 * NQ;                                       // [4] (8 words kept): per-warp largest V scale code
@@ -150,24 +205,43 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
   uint32_t rank, csize;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
-  const int pair = blockIdx.x / csize;
-  const int b = pair / a.c.kv_heads, hk = pair % a.c.kv_heads;
+  const int pair = blockIdx.x / csize, hk = pair % a.c.kv_heads;
+  int b = pair / a.c.kv_heads;
 
   pdl_wait();
-  const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
+  const int64_t capacity = a.c.width * a.c.page_size;
+  if (p.longest_first) {
+    // This CTA's row is the b-th by visible keys: the chip takes the long ones first and the
+    // short ones fill its last places. (The weights' buffer holds the lengths meanwhile.)
+    int* keys = reinterpret_cast<int*>(p_s);
+    const int batch = (int)a.batch, padded = (batch + 3) & ~3;
+    for (int k = tid; k < padded; k += kThreadsDec) {
+      int n = -1;
+      if (k < batch) {
+        const Row r = row_of(a.start, a.lens, k, a.t, capacity);
+        n = r.n > 0 ? last_seen(a, r, r.n - 1) - first_seen(a, r, 0) : 0;
+      }
+      keys[k] = n;
+    }
+    __syncthreads();
+    for (int k = tid; k < batch; k += kThreadsDec) {
+      const int mine = keys[k];
+      int rank_of = 0;
+      for (int o = 0; o < padded; o += 4) {
+        const int4 n = *reinterpret_cast<const int4*>(keys + o);
+        rank_of += (n.x > mine || (n.x == mine && o < k)) + (n.y > mine || (n.y == mine && o + 1 < k)) +
+                   (n.z > mine || (n.z == mine && o + 2 < k)) + (n.w > mine || (n.w == mine && o + 3 < k));
+      }
+      if (rank_of == b) lim[0] = k;
+    }
+    __syncthreads();
+    b = lim[0];
+    __syncthreads();  // before anything is written over either
+  }
+  const Row r = row_of(a.start, a.lens, b, a.t, capacity);
   if (r.bad && tid == 0 && rank == 0 && hk == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
-  // Keys [lo, hi) that query token t sees; both ends grow with t.
-  const int end = r.n > 0 ? (int)(r.start + r.n) : 0;
-  auto first_of = [&](int t) {
-    const int64_t x = a.has_window ? r.start + t - a.win_left : 0;
-    return (int)(x > 0 ? x : 0);
-  };
-  auto last_of = [&](int t) {
-    int64_t x = end;
-    if (a.causal && r.start + t + 1 < x) x = r.start + t + 1;
-    if (a.has_window && r.start + t + a.win_right + 1 < x) x = r.start + t + a.win_right + 1;
-    return (int)x;
-  };
+  auto first_of = [&](int t) { return first_seen(a, r, t); };
+  auto last_of = [&](int t) { return last_seen(a, r, t); };
   const int lo = r.n > 0 ? first_of(0) : 0, hi = r.n > 0 ? last_of(r.n - 1) : 0;
   // keys that every live query token sees
   const int all_lo = r.n > 0 ? first_of(r.n - 1) : 0, all_hi = r.n > 0 ? last_of(0) : 0;
@@ -400,16 +474,23 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
     // ---------------- softmax: thread = key ----------------
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     const uint32_t o_tmem = tmem_base + 2 * NQ + lane_addr;
+    // `f` on the columns there are: W where the registers hold all of them
+    auto widths = [&](int live, auto&& f) {
+      if constexpr (NQ == 16) f(std::integral_constant<int, W>{});
+      else by_width(live, f);
+    };
     float m_run = -INFINITY;  // of column `tid`: thread c keeps the running maximum of column c
-    float l_lane[16];
+    float l_lane[W];
 #pragma unroll
-    for (int c = 0; c < 16; ++c) l_lane[c] = 0.f;
+    for (int c = 0; c < W; ++c) l_lane[c] = 0.f;
     if (tid < 2 * NQ) mc[tid] = 0.f;
+    // the maxima as they are compared with: nothing is above those of columns that are not there
+    if (tid < NQ) ml[tid] = tid < p.rows ? -INFINITY : INFINITY;
     if (NQ > 16)
       for (int c = 0; c < NQ; ++c) l_s[c * 128 + tid] = 0.f;
     const float my_fc = Q8 ? (tid < NQ ? fc[tid] : 0.f) : p.scale_log2;
     bool live = true;  // false once a bounded wait ran out: barriers are still walked, nothing is waited for
-    uint32_t sr[16];
+    uint32_t sr[W];
     // 8-bit pages: my key's scale codes, its page looked up a block ahead
     uint32_t k_code = 127, v_code = 127;
     int v_top = -1;  // the largest V scale code so far: weights are taken relative to it
@@ -447,87 +528,105 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       const bool edge = base < all_lo || base + kKeys > all_hi;
       const float ks = Q8 ? scale_value(k_code) : 1.f;
       auto load_scores = [&](int q0) {
-        tmem_ld_cols(s_tmem + q0, sr);
+        tmem_ld_w<W>(s_tmem + q0, sr);
         if (Q8) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * ks);
+          for (int c = 0; c < W; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * ks);
         }
         if (edge) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
+          for (int c = 0; c < W; ++c)
             if (key < lim[q0 + c] || key >= lim[NQ + q0 + c]) sr[c] = 0xff800000u;
         }
       };
+      // Most blocks bring no score (and no V scale) above what the running maxima allow: one
+      // barrier says so, and the maxima and the reference stay. The first block sets them.
+      bool over = j == 0;
 #pragma unroll 1
       for (int q0 = 0; q0 < p.rows; q0 += 16) {
         load_scores(q0);
-        float mine_max = 0.f;
-        auto maxima = [&](auto width) {
+        auto compare = [&](auto width) {
 #pragma unroll
-          for (int c = 0; c < decltype(width)::value; ++c) {
-            const float wm = redux_max(__uint_as_float(sr[c]));
-            if (lane == c) mine_max = wm;
-          }
+          for (int c = 0; c < decltype(width)::value; ++c)
+            over = over || __uint_as_float(sr[c]) * (Q8 ? fc[q0 + c] : p.scale_log2) > ml[q0 + c] + kAdoptAbove<Q8>;
         };
-        by_width(p.rows - q0, maxima);
-        if (lane < 16 && q0 + lane < p.rows) red[(q0 + lane) * 4 + warp] = mine_max;
+        widths(p.rows - q0, compare);
         if (NQ == 16) break;
       }
-      if constexpr (Q8) {
-        const int wv = __reduce_max_sync(0xffffffffu, real && v_code != 255u ? (int)v_code : -1);
-        if (lane == 0) vred[warp] = wv;
-      }
-      named_barrier(1, 128);
+      if constexpr (Q8) over = over || (real && v_code != 255u && (int)v_code > v_top);
       bool moved = false;
       float v_corr = 1.f;  // 2^(old - new) of the V scales' reference
-      if constexpr (Q8) {
-        const int v_new = max(v_top, max(max(vred[0], vred[1]), max(vred[2], vred[3])));
-        if (v_new != v_top && v_top >= 0) {
-          v_corr = power_below(v_top - v_new);
-          moved = true;
+      if (barrier_or(2, over)) {
+#pragma unroll 1
+        for (int q0 = 0; q0 < p.rows; q0 += 16) {
+          if (NQ > 16) load_scores(q0);
+          float mine_max = 0.f;
+          auto maxima = [&](auto width) {
+#pragma unroll
+            for (int c = 0; c < decltype(width)::value; ++c) {
+              const float wm = redux_max(__uint_as_float(sr[c]));
+              if (lane == c) mine_max = wm;
+            }
+          };
+          widths(p.rows - q0, maxima);
+          if (lane < 16 && q0 + lane < p.rows) red[(q0 + lane) * 4 + warp] = mine_max;
+          if (NQ == 16) break;
         }
-        v_top = v_new;
-      }
-      if (tid < p.rows) {
-        const float4 w4 = *reinterpret_cast<const float4*>(red + tid * 4);
-        const float mx = fmaxf(fmaxf(w4.x, w4.y), fmaxf(w4.z, w4.w)) * my_fc;
-        float corr = 1.f;
-        if (mx > m_run + kAdoptAbove<Q8> || m_run == -INFINITY) {
-          const float m_new = fmaxf(m_run, mx);
-          if (m_new != m_run && m_run != -INFINITY) {
-            corr = ex2_approx(m_run - m_new);
+        if constexpr (Q8) {
+          const int wv = __reduce_max_sync(0xffffffffu, real && v_code != 255u ? (int)v_code : -1);
+          if (lane == 0) vred[warp] = wv;
+        }
+        named_barrier(1, 128);
+        if constexpr (Q8) {
+          const int v_new = max(v_top, max(max(vred[0], vred[1]), max(vred[2], vred[3])));
+          if (v_new != v_top && v_top >= 0) {
+            v_corr = power_below(v_top - v_new);
             moved = true;
           }
-          m_run = m_new;
+          v_top = v_new;
         }
-        mc[tid] = m_run == -INFINITY ? 0.f : m_run;
-        mc[NQ + tid] = corr;
+        if (tid < p.rows) {
+          const float4 w4 = *reinterpret_cast<const float4*>(red + tid * 4);
+          const float mx = fmaxf(fmaxf(w4.x, w4.y), fmaxf(w4.z, w4.w)) * my_fc;
+          float corr = 1.f;
+          if (mx > m_run + kAdoptAbove<Q8> || m_run == -INFINITY) {
+            const float m_new = fmaxf(m_run, mx);
+            if (m_new != m_run && m_run != -INFINITY) {
+              corr = ex2_approx(m_run - m_new);
+              moved = true;
+            }
+            m_run = m_new;
+          }
+          mc[tid] = m_run == -INFINITY ? 0.f : m_run;
+          mc[NQ + tid] = corr;
+          ml[tid] = m_run;
+        }
+        moved = barrier_or(2, moved);
       }
-      moved = barrier_or(2, moved);
       if (moved && j > 0) {
         // O holds the blocks before this one: rescale it once the last P.V is complete
         if (live && !mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, a.status)) live = false;
         tc_fence_after();
 #pragma unroll 1
         for (int q0 = 0; q0 < p.rows; q0 += 16) {
-          float f[16];
+          float f[W];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) f[c] = mc[NQ + q0 + c];
+          for (int c = 0; c < W; ++c) f[c] = mc[NQ + q0 + c];
 #pragma unroll 1
           for (int half = 0; half < 2; ++half) {
-            uint32_t orr[16];
-            tmem_ld_cols(o_tmem + half * NQ + q0, orr);
+            uint32_t orr[W];
+            tmem_ld_w<W>(o_tmem + half * NQ + q0, orr);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * (f[c] * v_corr));
-            tmem_st16(o_tmem + half * NQ + q0, orr);
+            for (int c = 0; c < W; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * (f[c] * v_corr));
+            tmem_st_w<W>(o_tmem + half * NQ + q0, orr);
           }
           if (NQ == 16) {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) l_lane[c] *= f[c];
+            for (int c = 0; c < W; ++c) l_lane[c] *= f[c];
             break;
           } else {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) l_s[(q0 + c) * 128 + tid] *= f[c];
+            for (int c = 0; c < W; ++c) l_s[(q0 + c) * 128 + tid] *= f[c];
           }
         }
         tmem_st_wait();
@@ -545,10 +644,10 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
         // All loads, then the arithmetic, then all stores: the compiler may not move a load
         // of a maximum or a sum above a store of a weight.
         auto weights = [&](auto width) {
-          constexpr int W = decltype(width)::value;
-          float mu[W], lv[W], sc[W];
+          constexpr int N = decltype(width)::value;
+          float mu[N], lv[N], sc[N];
 #pragma unroll
-          for (int c = 0; c < W; ++c) {
+          for (int c = 0; c < N; ++c) {
             mu[c] = mc[q0 + c];
             sc[c] = Q8 ? fc[q0 + c] : p.scale_log2;
             if (NQ > 16) lv[c] = l_s[(q0 + c) * 128 + tid];
@@ -556,9 +655,9 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
           if constexpr (!Q8) {
             uint8_t* pbox = p_s + (j % C::kPBufs) * C::kPBytes + (tid >> 6) * (2 * NQ * 128) + (tid & 7) * 2;
             const int chunk = (tid & 63) >> 3;
-            T high[W], low[W];
+            T high[N], low[N];
 #pragma unroll
-            for (int c = 0; c < W; ++c) {
+            for (int c = 0; c < N; ++c) {
               const float pr = ex2_approx(fmaf(__uint_as_float(sr[c]), sc[c], -mu[c]));
               if (NQ > 16) lv[c] += pr;
               else l_lane[c] += pr;
@@ -567,7 +666,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
               low[c] = Elem<T>::from_f((up - Elem<T>::to_f(high[c])) * kRestUp<T>);
             }
 #pragma unroll
-            for (int c = 0; c < W; ++c) {
+            for (int c = 0; c < N; ++c) {
               uint8_t* dst = pbox + (q0 + c) * 128 + ((chunk ^ (c & 7)) << 4);
               *reinterpret_cast<T*>(dst) = high[c];
               *reinterpret_cast<T*>(dst + NQ * 128) = low[c];
@@ -575,9 +674,9 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
           } else {
             uint8_t* pbox = p_s + (j % C::kPBufs) * C::kPBytes + (tid & 15);
             const int chunk = tid >> 4;
-            uint32_t piece[WP][W / 2];  // two columns each
+            uint32_t piece[WP][N / 2];  // two columns each
 #pragma unroll
-            for (int c = 0; c < W; c += 2) {
+            for (int c = 0; c < N; c += 2) {
               const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c]), sc[c], -mu[c]));
               const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + 1]), sc[c + 1], -mu[c + 1]));
               if (NQ > 16) lv[c] += p0, lv[c + 1] += p1;
@@ -596,17 +695,17 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
               }
             }
 #pragma unroll
-            for (int c = 0; c < W; ++c)
+            for (int c = 0; c < N; ++c)
 #pragma unroll
               for (int k = 0; k < WP; ++k)
                 pbox[k * (NQ * 128) + (q0 + c) * 128 + ((chunk ^ (c & 7)) << 4)] =
                     (uint8_t)(piece[k][c / 2] >> ((c & 1) * 8));
           }
 #pragma unroll
-          for (int c = 0; c < W; ++c)
+          for (int c = 0; c < N; ++c)
             if (NQ > 16) l_s[(q0 + c) * 128 + tid] = lv[c];
         };
-        by_width(p.rows - q0, weights);
+        widths(p.rows - q0, weights);
         if (NQ == 16) break;
       }
       if (base < lo || base + kKeys > hi) {
@@ -638,18 +737,18 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       for (int q0 = 0; q0 < p.rows; q0 += 16) {
         float mine_sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
+        for (int c = 0; c < W; ++c)
           if (q0 + c < p.rows) {
             const float s = warp_sum(NQ == 16 ? l_lane[c] : l_s[(q0 + c) * 128 + tid]);
             if (lane == c) mine_sum = s;
           }
         if (lane < 16 && q0 + lane < p.rows) red[(q0 + lane) * 4 + warp] = mine_sum;
         if (warp * 32 < D) {
-          uint32_t low[16];
-          tmem_ld_cols(o_tmem + q0, sr);
-          tmem_ld_cols(o_tmem + NQ + q0, low);
+          uint32_t low[W];
+          tmem_ld_w<W>(o_tmem + q0, sr);
+          tmem_ld_w<W>(o_tmem + NQ + q0, low);
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
+          for (int c = 0; c < W; ++c)
             if (q0 + c < p.rows)
               op[(q0 + c) * D + tid] = fmaf(__uint_as_float(low[c]), low_down, __uint_as_float(sr[c])) * o_up;
         }
@@ -731,12 +830,17 @@ int64_t most_blocks(const PagedAttnArgs& a) {
   return (keys + kKeys - 1) / kKeys;
 }
 
-// Shares per (row, KV head): the rule of attention_decode.cu.
+// Shares per (row, KV head): as many as bring the grid to the CTAs the chip holds at once, and
+// on to three times as many while a share keeps 16 blocks: the rows' lengths are not known
+// here, and with shares of the longest row first the chip's last places fill up (64 rows x 8
+// heads x 64..4095 keys: 127 us in whole rows, 117 in halves by index; what the order adds
+// stands at kSortedRows). Clusters have to find their CTAs' places in one GPC, hence the limits
+// of attention_decode.cu.
 int cluster_of(int64_t pairs, int64_t blocks, int per_sm) {
   const int64_t room = (int64_t)sms() * per_sm;
   int csize = 1;
   while (csize < 16 && csize * 2 <= blocks &&
-         (pairs * csize * 2 <= room || (pairs * csize < 4 * room && blocks >= 32 * csize * 2))) {
+         (pairs * csize * 2 <= room || (pairs * csize <= room && blocks >= 32 * csize * 2))) {
     if (csize == 8 && pairs > 6 * per_sm) break;
     if (csize == 4 && per_sm == 1 && pairs > 12) break;
     csize *= 2;
@@ -744,7 +848,7 @@ int cluster_of(int64_t pairs, int64_t blocks, int per_sm) {
   return csize;
 }
 
-template <typename T, bool Q8, int D, int NQ>
+template <typename T, bool Q8, int D, int NQ, int W>
 int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   using C = PagedDecCfg<T, Q8, D, NQ>;
   CUtensorMap tk, tv;
@@ -755,9 +859,9 @@ int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) 
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_seen[dev & 63]) {
-    if (cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, NQ, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)C::kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed,
+        cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, NQ, W>, cudaFuncAttributeNonPortableClusterSizeAllowed,
                              1) != cudaSuccess)
       return -1;
     attr_seen[dev & 63] = true;
@@ -768,7 +872,8 @@ int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) 
   p.scale_log2 = a.scale * kLog2eF;
   const int64_t pairs = a.batch * a.c.kv_heads;
   const int csize = cluster_of(pairs, most_blocks(a), C::kPerSm);
-  if (launch_pdl(attention_paged_decode_kernel<T, Q8, D, NQ>, dim3((unsigned)(pairs * csize)), dim3(kThreadsDec), C::kSmem,
+  p.longest_first = a.batch > 1 && a.batch <= kSortedRows && pairs * csize > (int64_t)sms() * C::kPerSm;
+  if (launch_pdl(attention_paged_decode_kernel<T, Q8, D, NQ, W>, dim3((unsigned)(pairs * csize)), dim3(kThreadsDec), C::kSmem,
                  s, (unsigned)csize, a.batch * a.t, tk, tv, p) != cudaSuccess)
     return -1;
   snprintf(cfg, cfg_len, "{rows:%d,bkv:%d,d:%d,box:%d,cluster:%d%s}", NQ, kKeys, a.c.d, p.box, csize, Q8 ? ",e4m3" : "");
@@ -778,9 +883,11 @@ int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) 
 template <typename T, bool Q8, int D>
 int run_width(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   const int64_t rows = a.t * (a.heads / a.c.kv_heads);
-  if (rows <= 16) return run_rows<T, Q8, D, 16>(a, s, cfg, cfg_len);
-  if (rows <= 32) return run_rows<T, Q8, D, 32>(a, s, cfg, cfg_len);
-  return run_rows<T, Q8, D, 64>(a, s, cfg, cfg_len);
+  if (rows <= 4) return run_rows<T, Q8, D, 16, 4>(a, s, cfg, cfg_len);
+  if (rows <= 8) return run_rows<T, Q8, D, 16, 8>(a, s, cfg, cfg_len);
+  if (rows <= 16) return run_rows<T, Q8, D, 16, 16>(a, s, cfg, cfg_len);
+  if (rows <= 32) return run_rows<T, Q8, D, 32, 16>(a, s, cfg, cfg_len);
+  return run_rows<T, Q8, D, 64, 16>(a, s, cfg, cfg_len);
 }
 
 template <typename T>
