@@ -971,52 +971,63 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
   }
 }
 
-// The parts of the items that more than one CTA had: block (CTA, eight columns), a thread a row.
+// The parts of the items that more than one CTA had: block (CTA, kMergeCols columns), a thread a
+// row. Bound by the trips to memory one after another (the split item, its parts, the store):
+// hence two parts' 34 loads at a time and a grid that fits the chip at once.
+constexpr int kMergeCols = 16;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attention_paged_merge_kernel(const __grid_constant__ PagedTcParams p) {
   pdl_trigger();
   pdl_wait();
   const PagedAttnArgs& a = p.a;
-  const int* h = p.heads_of_split + (int64_t)blockIdx.x * kSplitInts;
-  if (h[0] == 0) return;
-  const int b = h[1], hk = h[2], t0 = h[3], n_live = h[4], last = h[5];
-  const int row = threadIdx.x, d0 = blockIdx.y * 8;
+  const int4* h = reinterpret_cast<const int4*>(p.heads_of_split + (int64_t)blockIdx.x * kSplitInts);
+  const int4 h0 = h[0], h1 = h[1];
+  if (h0.x == 0) return;
+  const int b = h0.y, hk = h0.z, t0 = h0.w, n_live = h1.x, last = h1.y;
+  const int row = threadIdx.x, d0 = blockIdx.y * kMergeCols;
   const int in_tile = row & 127;
   const int t_row = t0 + (row >> 7) * p.tile_tokens + in_tile / p.group;
   const int head = hk * p.group + in_tile % p.group;
   if (in_tile >= p.tile_tokens * p.group || t_row >= a.t) return;
-  float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f, acc[kMergeCols];
+#pragma unroll
+  for (int e = 0; e < kMergeCols; ++e) acc[e] = 0.f;
   if (t_row < n_live) {
     // the first part lies in its CTA's second slot, the others in their CTAs' first
     auto part_of = [&](int k) { return p.parts + ((int64_t)k * 2 + (k == (int)blockIdx.x ? 1 : 0)) * kPartFloats<D>; };
-    // four parts' loads at a time: one after the other, each waits its microsecond
-    for (int k0 = blockIdx.x; k0 <= last; k0 += 4) {
-      float mr[4], lr[4], x[4][8];
+    for (int k0 = blockIdx.x; k0 <= last; k0 += 2) {
+      float mr[2], lr[2], x[2][kMergeCols];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         const bool there = k0 + u <= last;
         const float* part = part_of(there ? k0 + u : last);
         mr[u] = part[D * 256 + row];
         lr[u] = there ? part[D * 256 + 256 + row] : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][e] = part[(d0 + e) * 256 + row];
+        for (int e = 0; e < kMergeCols; ++e) x[u][e] = part[(d0 + e) * 256 + row];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         if (lr[u] == 0.f) continue;  // no key of this row there (NaN scores leave the maximum at -inf, the sum says so)
         const float m_new = fmaxf(m, mr[u]);
         const float f0 = m == -INFINITY ? 1.f : ex2_approx(m - m_new), f1 = mr[u] == -INFINITY ? 1.f : ex2_approx(mr[u] - m_new);
         l = fmaf(l, f0, f1 * lr[u]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], f0, f1 * x[u][e]);
+        for (int e = 0; e < kMergeCols; ++e) acc[e] = fmaf(acc[e], f0, f1 * x[u][e]);
         m = m_new;
       }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  stg128((T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh + d0,
-         make_uint4(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[2] * inv, acc[3] * inv),
-                    Elem<T>::pack(acc[4] * inv, acc[5] * inv), Elem<T>::pack(acc[6] * inv, acc[7] * inv)));
+  T* o = (T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh + d0;
+#pragma unroll
+  for (int v = 0; v < kMergeCols / 8; ++v) {
+    if (d0 + v * 8 >= a.c.d) break;  // padded head dim
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack(acc[v * 8 + 2 * e] * inv, acc[v * 8 + 2 * e + 1] * inv);
+    stg128(o + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
   if (a.lse != nullptr && d0 == 0)
     a.lse[((int64_t)b * a.heads + head) * a.t + t_row] = l == 0.f ? -INFINITY : kLn2F * (m + log2f(l));
 }
@@ -1071,8 +1082,8 @@ int run(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   if (launch_pdl(attention_paged_tc_kernel<T, Q8, D>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1,
                  a.batch * a.t, tq, tk, tv, p) != cudaSuccess)
     return -1;
-  if (launch_pdl(attention_paged_merge_kernel<T, D>, dim3((unsigned)grid, (unsigned)(a.c.d / 8)), dim3(256), 0, s, 1,
-                 a.batch * a.t, p) != cudaSuccess)
+  if (launch_pdl(attention_paged_merge_kernel<T, D>, dim3((unsigned)grid, (unsigned)((a.c.d + kMergeCols - 1) / kMergeCols)),
+                 dim3(256), 0, s, 1, 0, p) != cudaSuccess)
     return -1;
   snprintf(cfg, cfg_len, "{bq:%d,bkv:%d,d:%d,box:%d,grid:%d%s}", 2 * kBQ, kBKV, a.c.d, p.box, grid, Q8 ? ",e4m3" : "");
   return 0;

@@ -3,9 +3,11 @@
 // size (`attention_paged_exact`; the tensor-core kernels are in their own files).
 //
 // Write and read move every byte once and are bound by HBM, or by the chain
-// start -> table -> page of dependent loads where there is little to move. A lane owns 16
-// elements of a head row: two 16-byte accesses on the 16-bit side, one on the 8-bit side;
-// a row's D / 16 lanes find its largest value among themselves.
+// start -> table -> page of dependent loads where there is little to move. A lane owns 8
+// elements of a head row, 16 bytes on the 16-bit side and 8 on the 8-bit side, so that a
+// warp's accesses are whole lines (with 16 elements a lane every other 16 bytes: 113 us
+// against 103 for reading six rows of 3000 to 16384 e4m3 tokens, 117 against 100 in bf16,
+// which is 6.4 TB/s); a row's lanes find its largest value among themselves.
 #include <math.h>
 
 #include <initializer_list>
@@ -36,77 +38,106 @@ __device__ __forceinline__ int64_t page_of(const PagedCache& c, int64_t b, int64
 }
 
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, uint4 (&u)[2]) {
-  u[0] = ldg128(p);
-  u[1] = ldg128(p + 8);
-}
-template <typename T>
-__device__ __forceinline__ void widen16(const uint4 (&u)[2], float (&f)[16]) {
+__device__ __forceinline__ void widen8(uint4 u, float* f) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t w = i < 4 ? (i == 0 ? u[0].x : i == 1 ? u[0].y : i == 2 ? u[0].z : u[0].w)
-                             : (i == 4 ? u[1].x : i == 5 ? u[1].y : i == 6 ? u[1].z : u[1].w);
-    const float2 v = Elem<T>::unpack(w);
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = Elem<T>::unpack(w[i]);
     f[2 * i] = v.x, f[2 * i + 1] = v.y;
   }
 }
 
-// One token's head row a group of LPR lanes; blockIdx.y: keys or values.
+// n / d for 0 <= n < 2^31 without a division: (floor(n m / 2^32) + n) >> shift with
+// m = floor(2^32 (2^shift - d) / d) + 1, 2^shift >= d (Granlund and Montgomery's method).
+struct Divider {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> shift; }
+};
+Divider divider(uint32_t d) {
+  Divider v{d, 0, 0};
+  while ((1ull << v.shift) < d) ++v.shift;
+  v.m = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+  return v;
+}
+
+// Head rows a thread has a part of at once, their look-ups and loads on their way together. A
+// row on its way into 8 bits holds 16 values in registers: there more threads an SM do more
+// (10240 tokens x 8 heads x 128: 20.9 us with four, 17.5 with two, 18.9 with one).
+template <bool Q8Write>
+constexpr int kRowsAtOnce = Q8Write ? 2 : 4;
+
+// Values of a head row that a lane has: whole lines go out and in with 8 of them (16 bytes on
+// the 16-bit side); into 8 bits 16, whose e4m3 values are one 16-byte store and whose row
+// needs a shuffle less (10240 tokens x 8 heads x 128: 21 us against 25).
+template <bool Q8>
+constexpr int kPerLane = Q8 ? 16 : 8;
+
+// A token's head row a group of LPR lanes; block (run of a row's head rows, keys or values,
+// row). One head row a thread, with its row and head from 64-bit divisions, took 26 us for
+// 10240 tokens x 8 heads x 128 into e4m3.
 template <typename T, bool Q8, int LPR>
-__global__ void __launch_bounds__(kThreadsPaged) cache_write_kernel(const CacheWriteArgs a) {
+__global__ void __launch_bounds__(kThreadsPaged) cache_write_kernel(const CacheWriteArgs a, const Divider heads, const Divider page_size) {
+  constexpr int E = kPerLane<Q8>, N = kRowsAtOnce<Q8>;
   pdl_trigger();
   pdl_wait();
   const bool is_v = blockIdx.y != 0;
-  const int64_t g = (int64_t)blockIdx.x * kThreadsPaged + threadIdx.x;
-  const int64_t rows = a.batch * a.t * a.c.kv_heads;
-  const int64_t row = g / LPR;
-  const int sub = (int)(g % LPR);
-  const bool live = row < rows;
-  const int64_t token = live ? row / a.c.kv_heads : 0;
-  const int h = live ? (int)(row % a.c.kv_heads) : 0;
-  const int64_t b = token / a.t, i = token % a.t;
+  const int b = blockIdx.z, sub = threadIdx.x % LPR;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  const bool real = live && i < r.n;
-  uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  int64_t page = -1;
-  int slot = 0;
-  if (real) {
-    load16<T>(is_v ? (const T*)a.v + b * a.v_sb + i * a.v_st + h * a.v_sh + sub * 16
-                   : (const T*)a.k + b * a.k_sb + i * a.k_st + h * a.k_sh + sub * 16, u);
-    const int64_t pos = r.start + i;
-    const int64_t at = pos / a.c.page_size;
-    slot = (int)(pos - at * a.c.page_size);
-    page = page_of(a.c, b, at, a.status);
-  }
-  if (r.bad && live && i == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
-  const int64_t to = is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh;
-  if constexpr (!Q8) {
-    if (page < 0) return;
-    T* dst = (T*)(is_v ? a.c.v : a.c.k) + to + sub * 16;
-    stg128(dst, u[0]);
-    stg128(dst + 8, u[1]);
-  } else {
-    float f[16];
-    widen16<T>(u, f);
-    // the largest as an integer: a NaN's bits are above every number's, and stay so
-    uint32_t top = 0;
+  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  const uint32_t rows = (uint32_t)r.n * a.c.kv_heads;  // of this sequence's chunk
+  const uint32_t row0 = blockIdx.x * (kThreadsPaged / LPR * N) + threadIdx.x / LPR;
+  if (blockIdx.x * (kThreadsPaged / LPR * N) >= rows) return;  // the whole block: shuffles stay whole
+  const T* src = is_v ? (const T*)a.v + b * a.v_sb : (const T*)a.k + b * a.k_sb;
+  const int64_t src_t = is_v ? a.v_st : a.k_st, src_h = is_v ? a.v_sh : a.k_sh;
+  const int64_t sp = is_v ? a.c.v_sp : a.c.k_sp, ss = is_v ? a.c.v_ss : a.c.k_ss, sh = is_v ? a.c.v_sh : a.c.k_sh;
+  uint4 u[N][E / 8];
+  int64_t page[N];
+  uint32_t slot[N], head[N];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+  for (int k = 0; k < N; ++k) {
+    const uint32_t row = row0 + k * (kThreadsPaged / LPR);
+    page[k] = -1;
+    const uint32_t i = heads.div(row);
+    head[k] = row - i * heads.d;
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (page < 0) return;
-    const uint32_t code = scale_code(__uint_as_float(top));
-    const float inv = code == 255u ? 0.f : scale_inverse(code);
-    uint32_t w[4];
+    for (int e = 0; e < E / 8; ++e) u[k][e] = make_uint4(0, 0, 0, 0);
+    if (row < rows) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t lo = to_e4m3x2(f[4 * e] * inv, f[4 * e + 1] * inv), hi = to_e4m3x2(f[4 * e + 2] * inv, f[4 * e + 3] * inv);
-      w[e] = code == 255u ? 0u : lo | (hi << 16);
+      for (int e = 0; e < E / 8; ++e) u[k][e] = ldg128(src + i * src_t + head[k] * src_h + sub * E + e * 8);
+      const uint32_t pos = (uint32_t)r.start + i, at = page_size.div(pos);
+      slot[k] = pos - at * page_size.d;
+      page[k] = page_of(a.c, b, at, a.status);
     }
-    stg128((uint8_t*)(is_v ? a.c.v : a.c.k) + to + sub * 16, make_uint4(w[0], w[1], w[2], w[3]));
-    if (sub == 0) {
-      if (is_v) a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] = (uint8_t)code;
-      else a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot] = (uint8_t)code;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int64_t to = page[k] * sp + slot[k] * ss + head[k] * sh + sub * E;
+    if constexpr (!Q8) {
+      if (page[k] >= 0) stg128((T*)(is_v ? a.c.v : a.c.k) + to, u[k][0]);
+    } else {
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E / 8; ++e) widen8<T>(u[k][e], f + 8 * e);
+      // the largest as an integer: a NaN's bits are above every number's, and stay so
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (page[k] < 0) continue;
+      const uint32_t code = scale_code(__uint_as_float(top));
+      const float inv = code == 255u ? 0.f : scale_inverse(code);
+      uint32_t w[E / 4];
+#pragma unroll
+      for (int e = 0; e < E / 4; ++e) {
+        const uint32_t lo = to_e4m3x2(f[4 * e] * inv, f[4 * e + 1] * inv), hi = to_e4m3x2(f[4 * e + 2] * inv, f[4 * e + 3] * inv);
+        w[e] = code == 255u ? 0u : lo | (hi << 16);
+      }
+      stg128((uint8_t*)(is_v ? a.c.v : a.c.k) + to, make_uint4(w[0], w[1], w[2], w[3]));
+      if (sub == 0) {
+        if (is_v) a.c.v_scale[page[k] * a.c.vs_sp + head[k] * a.c.vs_sh + slot[k]] = (uint8_t)code;
+        else a.c.k_scale[page[k] * a.c.ks_sp + head[k] * a.c.ks_sh + slot[k]] = (uint8_t)code;
+      }
     }
   }
 }
@@ -151,54 +182,66 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_any_kernel(const Ca
   }
 }
 
-// Sixteen e4m3 values times their scale, rounded to the stream type.
+// Eight e4m3 values times their scale, rounded to the stream type.
 template <typename T>
-__device__ __forceinline__ void widen_e4m3(uint4 u, float scale, uint32_t (&w)[8]) {
-  const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 lo = from_e4m3x2(in[e] & 0xffffu), hi = from_e4m3x2(in[e] >> 16);
-    w[2 * e] = Elem<T>::pack(lo.x * scale, lo.y * scale);
-    w[2 * e + 1] = Elem<T>::pack(hi.x * scale, hi.y * scale);
-  }
+__device__ __forceinline__ uint4 widen_e4m3(uint2 u, float scale) {
+  const float2 a = from_e4m3x2(u.x & 0xffffu), b = from_e4m3x2(u.x >> 16), c = from_e4m3x2(u.y & 0xffffu), d = from_e4m3x2(u.y >> 16);
+  return make_uint4(Elem<T>::pack(a.x * scale, a.y * scale), Elem<T>::pack(b.x * scale, b.y * scale),
+                    Elem<T>::pack(c.x * scale, c.y * scale), Elem<T>::pack(d.x * scale, d.y * scale));
 }
 
+__device__ __forceinline__ uint2 ldg64(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// As cache_write_kernel is laid out; rows behind a sequence's end are zeros.
 template <typename T, bool Q8, int LPR>
-__global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheReadArgs a) {
+__global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheReadArgs a, const Divider heads, const Divider page_size) {
+  constexpr int N = kRowsAtOnce<false>;
   pdl_trigger();
   pdl_wait();
   const bool is_v = blockIdx.y != 0;
-  const int64_t g = (int64_t)blockIdx.x * kThreadsPaged + threadIdx.x;
-  const int64_t row = g / LPR;
-  const int sub = (int)(g % LPR);
-  if (row >= a.batch * a.len * a.c.kv_heads) return;
-  const int64_t token = row / a.c.kv_heads;
-  const int h = (int)(row % a.c.kv_heads);
-  const int64_t b = token / a.len, pos = token % a.len;
+  const int b = blockIdx.z, sub = threadIdx.x % LPR;
   const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
-  if (r.bad && pos == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
-  uint32_t w[8] = {};
-  if (pos < r.n) {
-    const int64_t at = pos / a.c.page_size;
-    const int slot = (int)(pos - at * a.c.page_size);
-    const int64_t page = page_of(a.c, b, at, a.status);
-    if (page >= 0) {
-      const int64_t from = (is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh) + sub * 16;
-      if constexpr (Q8) {
-        const uint4 u = ldg128((const uint8_t*)(is_v ? a.c.v : a.c.k) + from);
-        const uint32_t code = is_v ? a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] : a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot];
-        widen_e4m3<T>(u, scale_value(code), w);
-      } else {
-        uint4 u[2];
-        load16<T>((const T*)(is_v ? a.c.v : a.c.k) + from, u);
-        w[0] = u[0].x, w[1] = u[0].y, w[2] = u[0].z, w[3] = u[0].w;
-        w[4] = u[1].x, w[5] = u[1].y, w[6] = u[1].z, w[7] = u[1].w;
+  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  const uint32_t rows = (uint32_t)a.len * a.c.kv_heads;
+  const uint32_t row0 = blockIdx.x * (kThreadsPaged / LPR * N) + threadIdx.x / LPR;
+  const int64_t sp = is_v ? a.c.v_sp : a.c.k_sp, ss = is_v ? a.c.v_ss : a.c.k_ss, sh = is_v ? a.c.v_sh : a.c.k_sh;
+  T* out = is_v ? (T*)a.v + b * a.v_sb : (T*)a.k + b * a.k_sb;
+  const int64_t out_t = is_v ? a.v_st : a.k_st, out_h = is_v ? a.v_sh : a.k_sh;
+  std::conditional_t<Q8, uint2, uint4> u[N];
+  uint32_t code[N], head[N], token[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const uint32_t row = row0 + k * (kThreadsPaged / LPR);
+    token[k] = heads.div(row);
+    head[k] = row - token[k] * heads.d;
+    code[k] = 0u;
+    u[k] = {};
+    if (row < rows && token[k] < (uint32_t)r.n) {
+      const uint32_t at = page_size.div(token[k]), slot = token[k] - at * page_size.d;
+      const int64_t page = page_of(a.c, b, at, a.status);
+      if (page >= 0) {
+        const int64_t from = page * sp + slot * ss + head[k] * sh + sub * 8;
+        if constexpr (Q8) {
+          u[k] = ldg64((const uint8_t*)(is_v ? a.c.v : a.c.k) + from);
+          code[k] = is_v ? a.c.v_scale[page * a.c.vs_sp + head[k] * a.c.vs_sh + slot]
+                         : a.c.k_scale[page * a.c.ks_sp + head[k] * a.c.ks_sh + slot];
+        } else {
+          u[k] = ldg128((const T*)(is_v ? a.c.v : a.c.k) + from);
+        }
       }
     }
   }
-  T* dst = is_v ? (T*)a.v + b * a.v_sb + pos * a.v_st + h * a.v_sh + sub * 16 : (T*)a.k + b * a.k_sb + pos * a.k_st + h * a.k_sh + sub * 16;
-  stg128(dst, make_uint4(w[0], w[1], w[2], w[3]));
-  stg128(dst + 8, make_uint4(w[4], w[5], w[6], w[7]));
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (row0 + k * (kThreadsPaged / LPR) >= rows) continue;
+    T* dst = out + token[k] * out_t + head[k] * out_h + sub * 8;
+    if constexpr (Q8) stg128(dst, widen_e4m3<T>(u[k], scale_value(code[k])));
+    else stg128(dst, u[k]);
+  }
 }
 
 template <typename T, bool Q8>
@@ -325,9 +368,10 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
   if (a.lse != nullptr && threadIdx.x == 0) a.lse[(b * a.heads + h) * a.t + i] = total == 0.f ? -INFINITY : top + logf(total);
 }
 
-int lanes_a_row(int d) {
-  if (d % 16 != 0 || d > 512) return 0;
-  const int l = d / 16;
+// Lanes a row of d values takes at `per` a lane: a power of two, a warp's at most; 0 = no such.
+int lanes_a_row(int d, int per) {
+  if (d % per != 0 || d > 32 * per) return 0;
+  const int l = d / per;
   return (l & (l - 1)) == 0 ? l : 0;
 }
 bool on_grid(const void* p, std::initializer_list<int64_t> strides, int64_t size) {
@@ -343,21 +387,27 @@ bool pages_on_grid(const PagedCache& c) {
 
 unsigned blocks_of(int64_t n, int64_t per) { return (unsigned)((n + per - 1) / per); }
 
+// Whether a vector kernel's block and row numbers hold the call: 31 bits of head rows a sequence.
+bool within(const PagedCache& c, int64_t batch, int64_t tokens) {
+  return batch <= 65535 && tokens * c.kv_heads < (int64_t)1 << 31;
+}
+
 template <typename T, bool Q8>
 int run_write(const CacheWriteArgs& a, cudaStream_t s) {
   const int64_t rows = a.batch * a.t * a.c.kv_heads;
-  const int lpr = lanes_a_row(a.c.d);
+  const int lpr = lanes_a_row(a.c.d, kPerLane<Q8>);
   if constexpr (!std::is_same<T, float>::value) {
-    if (lpr != 0 && pages_on_grid(a.c) && on_grid(a.k, {a.k_sb, a.k_st, a.k_sh}, 2) && on_grid(a.v, {a.v_sb, a.v_st, a.v_sh}, 2)) {
-      const dim3 grid(blocks_of(rows * lpr, kThreadsPaged), 2), block(kThreadsPaged);
+    if (lpr != 0 && within(a.c, a.batch, a.t) && pages_on_grid(a.c) && on_grid(a.k, {a.k_sb, a.k_st, a.k_sh}, 2) && on_grid(a.v, {a.v_sb, a.v_st, a.v_sh}, 2)) {
+      const dim3 grid(blocks_of(a.t * a.c.kv_heads * lpr, kThreadsPaged * kRowsAtOnce<Q8>), 2, (unsigned)a.batch), block(kThreadsPaged);
+      const Divider heads = divider((uint32_t)a.c.kv_heads), page = divider((uint32_t)a.c.page_size);
       const int64_t pdl = a.batch * a.t;
       switch (lpr) {
-        case 1: launch_pdl(cache_write_kernel<T, Q8, 1>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 2: launch_pdl(cache_write_kernel<T, Q8, 2>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 4: launch_pdl(cache_write_kernel<T, Q8, 4>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 8: launch_pdl(cache_write_kernel<T, Q8, 8>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 16: launch_pdl(cache_write_kernel<T, Q8, 16>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 32: launch_pdl(cache_write_kernel<T, Q8, 32>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 1: launch_pdl(cache_write_kernel<T, Q8, 1>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 2: launch_pdl(cache_write_kernel<T, Q8, 2>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 4: launch_pdl(cache_write_kernel<T, Q8, 4>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 8: launch_pdl(cache_write_kernel<T, Q8, 8>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 16: launch_pdl(cache_write_kernel<T, Q8, 16>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 32: launch_pdl(cache_write_kernel<T, Q8, 32>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
       }
     }
   }
@@ -368,18 +418,19 @@ int run_write(const CacheWriteArgs& a, cudaStream_t s) {
 template <typename T, bool Q8>
 int run_read(const CacheReadArgs& a, cudaStream_t s) {
   const int64_t rows = a.batch * a.len * a.c.kv_heads;
-  const int lpr = lanes_a_row(a.c.d);
+  const int lpr = lanes_a_row(a.c.d, 8);
   if constexpr (!std::is_same<T, float>::value) {
-    if (lpr != 0 && pages_on_grid(a.c) && on_grid(a.k, {a.k_sb, a.k_st, a.k_sh}, 2) && on_grid(a.v, {a.v_sb, a.v_st, a.v_sh}, 2)) {
-      const dim3 grid(blocks_of(rows * lpr, kThreadsPaged), 2), block(kThreadsPaged);
+    if (lpr != 0 && within(a.c, a.batch, a.len) && pages_on_grid(a.c) && on_grid(a.k, {a.k_sb, a.k_st, a.k_sh}, 2) && on_grid(a.v, {a.v_sb, a.v_st, a.v_sh}, 2)) {
+      const dim3 grid(blocks_of(a.len * a.c.kv_heads * lpr, kThreadsPaged * kRowsAtOnce<false>), 2, (unsigned)a.batch), block(kThreadsPaged);
+      const Divider heads = divider((uint32_t)a.c.kv_heads), page = divider((uint32_t)a.c.page_size);
       const int64_t pdl = a.batch * a.len;
       switch (lpr) {
-        case 1: launch_pdl(cache_read_kernel<T, Q8, 1>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 2: launch_pdl(cache_read_kernel<T, Q8, 2>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 4: launch_pdl(cache_read_kernel<T, Q8, 4>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 8: launch_pdl(cache_read_kernel<T, Q8, 8>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 16: launch_pdl(cache_read_kernel<T, Q8, 16>, grid, block, 0, s, 1, pdl, a); return 1;
-        case 32: launch_pdl(cache_read_kernel<T, Q8, 32>, grid, block, 0, s, 1, pdl, a); return 1;
+        case 1: launch_pdl(cache_read_kernel<T, Q8, 1>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 2: launch_pdl(cache_read_kernel<T, Q8, 2>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 4: launch_pdl(cache_read_kernel<T, Q8, 4>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 8: launch_pdl(cache_read_kernel<T, Q8, 8>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 16: launch_pdl(cache_read_kernel<T, Q8, 16>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
+        case 32: launch_pdl(cache_read_kernel<T, Q8, 32>, grid, block, 0, s, 1, pdl, a, heads, page); return 1;
       }
     }
   }
