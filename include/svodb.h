@@ -254,7 +254,8 @@ int svodb_combine_splits(const svodb_tensor* o_part, const svodb_tensor* m_part,
  * Position p of sequence b lies in slot p % page_size of page table[b, p / page_size];
  * entries of `table` behind a sequence's last page are never looked at, and two sequences
  * may share pages (a common prefix) as long as nobody writes them. Pages hold the stream
- * type, or e4m3 beside one power of two a token and head. A user's view of one layer of a
+ * type, or e4m3 beside one power of two a token and head (a row that is not finite is told by
+ * its scale: the codes 0x7f and 0xff, e4m3's own NaN, are no values of a page). A user's view of one layer of a
  * larger buffer is a cache: any strides do, innermost 1. */
 typedef struct svodb_paged_cache {
   const svodb_tensor* k;       /* [pages, page_size, kv_heads, D], the stream type or e4m3 */
@@ -285,7 +286,9 @@ int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, s
  * Query i of row b stands at position start[b] + i and sees keys 0 .. start[b] + lens[b] - 1
  * (lens = T without `lens`), under `causal` those up to its own position, under a window
  * those from window_left before to window_right behind it. Rows from lens[b] on and rows
- * without a key are zeros (lse -inf). Of `opts`: causal, has_window, has_scale, lse,
+ * without a key are zeros (lse -inf). Slots that hold no token of the sequence may hold anything; a
+ * NaN or an infinity in a token's own keys or values reaches every query that sees it and may
+ * reach earlier queries of the same chunk (0 * NaN). Of `opts`: causal, has_window, has_scale, lse,
  * workspace; any other option is refused. `workspace`: svodb_attention_paged_workspace_bytes
  * bytes, 16-byte aligned, for this call alone (two calls that may overlap on the GPU, or two
  * graphs that may be replayed at once, have one each). */

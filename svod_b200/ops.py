@@ -535,12 +535,17 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, sta
     and sees the `start[b] + lens[b]` keys of its sequence (T without `lens`), under
     `opts.causal` (the default without `opts`) those up to its own position, under
     `opts.window` those near it. One token a row is a decoding step, `start` zeros a prompt.
-    Rows from `lens[b]` on and rows that see no key are zeros. Other options are refused."""
+    Rows from `lens[b]` on and rows that see no key are zeros. Other options are refused.
+
+    Slots that hold no token of the sequence, and pages that a window has left behind, may hold
+    anything. A NaN or an infinity in a token's own keys or values reaches every query that sees
+    it, and may reach earlier queries of the same chunk (a product with their zero weights)."""
     global launches
     opts = opts or Attn(causal=True)
     r = (_call or _fast()).attention_paged(q, cache, table, start, lens, opts)
     if r is not None:
-        launches += 1
+        # over 64 query rows a KV head a second kernel merges the parts of the work
+        launches += 2 if q.shape[1] * q.shape[2] > 64 * cache.k.shape[2] else 1
         return r
     dev = _one_device(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, start, lens)
     if q.dim() != 4:
@@ -560,7 +565,7 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, sta
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             keep.append(ws)
             o.workspace, o.workspace_bytes = ws.data_ptr(), need
-        _check(lib.svodb_attention_paged(_p(qd), C.byref(c), _p(sd), _p(ld), C.byref(o), _p(od), _stream()))
+        _check(lib.svodb_attention_paged(_p(qd), C.byref(c), _p(sd), _p(ld), C.byref(o), _p(od), _stream()), 2 if need else 1)
     return (out, lse) if opts.want_lse else out
 
 

@@ -442,3 +442,111 @@ def test_refused_inside_packed_rows():
         with pytest.raises(ops.OpsError) as e:
             ops.attention_paged(q, cache, i32([[0], [1]]), i32([0, 0]))
         assert e.value.code == ops.ERR_UNSUPPORTED
+
+
+# --------------------------------------------------------------- what a caller may also hand over
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("heads,kv,d,page,tokens", [(2, 1, 128, 8, 1), (2, 1, 128, 8, 70), (96, 1, 64, 16, 1), (128, 1, 128, 32, 3),
+                                                    (130, 1, 64, 16, 2), (40, 1, 128, 16, 1), (7, 7, 64, 16, 65), (5, 1, 128, 64, 40)])
+def test_wide_groups_and_small_pages(dtype, quantized, heads, kv, d, page, tokens):
+    held = [150, 0, 33]
+    c = Case(heads + page, 3, tokens, held, [tokens, tokens, max(0, tokens - 1)], heads, kv, d, page, dtype, quantized)
+    c.put([0] * 3, [h + n for h, n in zip(held, c.new)])
+    check(attend(c), c)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("batch,tokens", [(75, 1), (75, 40), (1500, 1)])
+def test_wide_batches(dtype, quantized, batch, tokens):
+    held = [(37 * b) % 260 for b in range(batch)]
+    new = [0 if b % 11 == 3 else 1 + b % tokens for b in range(batch)]
+    c = Case(batch, batch, tokens, held, new, 2, 1, 64, 16, dtype, quantized)
+    c.put([0] * batch, [h + n for h, n in zip(held, new)])
+    check(attend(c), c)
+
+
+@pytest.mark.parametrize("tokens", [3, 90])
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+def test_what_stands_in_padding_does_not_matter(dtype, quantized, tokens):
+    """NaN queries behind the real ones, counts beyond the chunk and below zero, counts and
+    tables of 64-bit integers."""
+    held = [70, 5, 0]
+    c = Case(31, 3, tokens, held, [tokens - 1, tokens, 0], 4, 2, 64, 16, dtype, quantized)
+    c.put([0] * 3, [h + n for h, n in zip(held, c.new)])
+    q = c.q.cuda()
+    q[0, tokens - 1:] = math.nan
+    q[2] = math.nan
+    lens = torch.tensor([tokens - 1, tokens + 7, -3], device="cuda")
+    got = ops.attention_paged(q, cache_of(c), c.table.cuda().long(), torch.tensor(held, device="cuda"), lens)
+    c.new = [tokens - 1, tokens, 0]
+    c.q[0, tokens - 1:] = 0
+    c.q[2] = 0
+    check(got, c)
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+@pytest.mark.parametrize("tokens", [1, 80])
+def test_a_row_of_nan_stays_in_its_sequence(dtype, quantized, tokens):
+    """A key row that holds a NaN makes NaN of every query that sees it, and of nothing in
+    the rows beside it."""
+    held = [90, 90]
+    c = Case(17, 2, tokens, held, [tokens] * 2, 4, 2, 64, 16, dtype, quantized)
+    c.keys[0][20, 1, 3] = math.nan
+    c.values[0][20, 1, 3] = math.inf
+    c.put([0] * 2, [h + tokens for h in held])
+    got = attend(c)
+    ops.device_status()
+    assert torch.isnan(got[0, :, 2:].float()).all() and torch.isfinite(got[0, :, :2].float()).all()
+    want, _, bound = c.attention()
+    assert ((got[1].double().cpu() - want[1]).abs() <= bound[1]).all()
+
+
+def test_reads_past_the_table_are_reported():
+    c = Case(3, 2, 1, [20, 9], [0, 0], 1, 1, 64, 16, BF16, False).put([0, 0], [20, 9])
+    table = c.table[:, :2].contiguous().cuda()
+    k, _ = ops.cache_read(cache_of(c), table, i32([33, 9]), 40)
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    assert (k[0] == 0).all() and torch.equal(k[1, :9].cpu(), c.keys[1])
+    k, _ = ops.cache_read(cache_of(c), table, i32([20, -4]), 40)
+    ops.device_status()
+    assert torch.equal(k[0, :20].cpu(), c.keys[0]) and (k[1] == 0).all()
+
+
+def test_which_kernel_ran():
+    q = torch.randn(2, 40, 4, 64, device="cuda").to(BF16)
+    cache, start = ops.PagedCache.empty(12, 16, 2, 64), i32([0, 0])
+    table = i32([[0, 1, 2], [3, 4, 5]])
+    ops.attention_paged(q, cache, table, start)
+    assert ops.chosen().startswith("attention_paged: kernel paged_flash_attention")
+    ops.attention_paged(q[:, :5], cache, table, start)
+    assert ops.chosen().startswith("attention_paged: kernel paged_decode")
+    odd = ops.PagedCache.empty(12, 15, 2, 64)
+    ops.attention_paged(q, odd, table, start)
+    assert ops.chosen() == "attention_paged: graph shape"
+    ops.cache_write(q[:, :, :2], q[:, :, 2:], cache, table, start)
+    assert ops.chosen().startswith("cache_write: kernel")
+    ops.cache_read(cache, table, start)
+    assert ops.chosen().startswith("cache_read: kernel")
+    ops.device_status()
+
+
+def test_a_workspace_too_small_is_refused():
+    import ctypes as C
+    lib = L.load()
+    q, cache, table, start = (torch.zeros(1, 70, 2, 64, dtype=BF16, device="cuda"), ops.PagedCache.empty(8, 16, 1, 64),
+                              i32([list(range(8))]), i32([0]))
+    keep, out = [], torch.empty_like(q)
+    c = ops._paged(cache, table, keep)
+    qd, sd, od = ops._desc(q), ops._desc(start), ops._desc(out)
+    need = lib.svodb_attention_paged_workspace_bytes(C.byref(qd), C.byref(c))
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    o = L.AttnOpts()
+    call = lambda: lib.svodb_attention_paged(C.byref(qd), C.byref(c), C.byref(sd), None, C.byref(o), C.byref(od), torch.cuda.current_stream().cuda_stream)
+    assert call() == L.ERR_WORKSPACE
+    o.workspace, o.workspace_bytes = ws.data_ptr(), need - 1
+    assert call() == L.ERR_WORKSPACE
+    o.workspace_bytes = need
+    assert call() == L.OK
+    ops.device_status()
