@@ -1083,9 +1083,9 @@ size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_
   PagedAttnArgs a{};
   if (paged_cache("attention_paged", cache, q->shape[0], q->dtype, a.c) != SVODB_OK) return 0;
   if (numel(q) == 0 || q->shape[3] != a.c.d || q->shape[2] % a.c.kv_heads != 0 || !is_half(q->dtype) || a.c.d > 128) return 0;
-  a.batch = q->shape[0], a.t = q->shape[1], a.heads = (int)q->shape[2];
+  a.batch = q->shape[0], a.t = q->shape[1], a.heads = (int)q->shape[2], a.dtype = q->dtype;
   // the few-row kernel merges on the chip
-  return a.t <= 64 && a.t * (a.heads / a.c.kv_heads) <= 64 ? 0 : attention_paged_tc_workspace(a);
+  return attention_paged_few_rows(a) ? 0 : attention_paged_tc_workspace(a);
 }
 
 int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache, const svodb_tensor* start,

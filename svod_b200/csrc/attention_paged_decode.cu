@@ -3,7 +3,7 @@
 //
 // What bounds it: the cache's bytes. The layout is attention_decode.cu's: keys are the M of
 // both contractions, so a block of 128 keys costs two small MMAs whatever the number of rows,
-//     S^T [128 keys x NQ]  = K [128 x D] . Q^T            O^T [D x NQ] += V^T [D x 128] . P^T
+//     S^T [128 keys x 16]  = K [128 x D] . Q^T            O^T [D x 16] += V^T [D x 128] . P^T
 // a softmax thread owns one key, a cluster of C CTAs takes one (row, KV head) and merges its
 // C partial states through distributed shared memory: one launch, no workspace.
 //
@@ -56,27 +56,27 @@ constexpr float kRemainderUp = 131072.f;  // 2^17: the remainder of a weight of 
 template <bool Q8>
 constexpr float kAdoptAbove = Q8 ? 2.f : kRescaleAbove;
 
-template <typename T, bool Q8, int D, int NQ>
+constexpr int kRows = 16;  // query rows of a KV head: the N of both MMAs
+
+template <typename T, bool Q8, int D>
 struct PagedDecCfg {
   static_assert(!Q8 || D == 128, "8-bit rows are a 128-byte tile, zero-filled behind the head");
   static constexpr int kBoxes = Q8 ? 1 : D / 64;  // 128-byte boxes of a row
   static constexpr int kSlotBytes = kKeys * 128 * kBoxes;
-  static constexpr int kSlots = Q8 ? (NQ == 16 ? 3 : NQ == 32 ? 8 : 6)
-                                   : D == 128 ? (NQ == 16 ? 3 : NQ == 32 ? 5 : 4) : (NQ == 16 ? 3 : NQ == 32 ? 10 : 8);
-  static constexpr int kPerSm = NQ > 16 ? 1 : !Q8 && D == 128 ? 2 : 3;
+  static constexpr int kSlots = 3;
+  static constexpr int kPerSm = !Q8 && D == 128 ? 2 : 3;
   static constexpr int kRing = kSlots * kSlotBytes;
-  static constexpr int kQBytes = Q8 ? kQueryPieces<T> * NQ * 128 : NQ * D * 2;
-  static constexpr int kPBytes = Q8 ? kWeightPieces<T> * NQ * 128 : 2 * 2 * NQ * 128;
-  static constexpr int kPBufs = NQ == 64 || (NQ == 16 && D == 128 && (!Q8 || kWeightPieces<T> > 4)) ? 1 : 2;
-  static constexpr int kLBytes = NQ > 16 ? NQ * 128 * 4 : 0;
-  static constexpr int kRedBytes = NQ * 4 * 4;
-  static constexpr int kTail = kQBytes + kPBufs * kPBytes + kLBytes + kRedBytes + 7 * NQ * 4 + 32 + 256;
+  static constexpr int kQBytes = Q8 ? kQueryPieces<T> * kRows * 128 : kRows * D * 2;
+  static constexpr int kPBytes = Q8 ? kWeightPieces<T> * kRows * 128 : 2 * 2 * kRows * 128;
+  // A second buffer of weights lets a block's exponentials run under the previous block's P.V.
+  static constexpr int kPBufs = D == 128 && (!Q8 || kWeightPieces<T> > 4) ? 1 : 2;
+  static constexpr int kRedBytes = kRows * 4 * 4;
+  static constexpr int kTail = kQBytes + kPBufs * kPBytes + kRedBytes + 7 * kRows * 4 + 32 + 256;
   static constexpr size_t kSmem = 1024 + (size_t)kRing + (kTail > kBox ? kTail : kBox);
-  static constexpr int kTmemCols = 4 * NQ;
-  static_assert(kSmem <= 232448, "beyond the 227 KiB a CTA may hold");
+  static constexpr int kTmemCols = 4 * kRows;
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "the CTAs of an SM fit its shared memory");
   static_assert(kPBufs * kPBytes >= 4 * 1024, "the lengths of kSortedRows rows lie over the weights");
-  static_assert(NQ * D * 4 <= kRing, "the partial outputs are laid over the ring");
+  static_assert(kRows * D * 4 <= kRing, "the partial outputs are laid over the ring");
 };
 
 // Rows of a batch that a CTA puts in order: their lengths fit the smallest weights' buffer.
@@ -86,6 +86,7 @@ struct PagedDecParams {
   PagedAttnArgs a;
   int group, rows;  // rows = t * group query rows per KV head
   int box;          // keys of a box
+  Divider page_size;
   int longest_first;  // rows in the order of their visible keys, where the grid does not fit the chip at once
   float scale_log2;
 };
@@ -167,14 +168,14 @@ __device__ __forceinline__ void tmem_st_w(uint32_t at, const uint32_t (&r)[W]) {
   }
 }
 
-// NQ: rows of the MMAs; W: the columns of a chunk that softmax threads keep in registers, as
-// few as hold the query rows where these are 16 at most (a register each for scores and sums:
-// three CTAs an SM leave 96).
-template <typename T, bool Q8, int D, int NQ, int W>
-__global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerSm))
+// W: the columns (query rows) that softmax threads keep in registers, the least of 4, 8 and 16
+// that holds them (a register each for scores and sums, and three CTAs an SM leave 96; 16 rows
+// x 8000..32767 e4m3 keys, two query rows a KV head: 145 us with 16 columns, 118 with 4).
+template <typename T, bool Q8, int D, int W>
+__global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
     attention_paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                                   const __grid_constant__ PagedDecParams p) {
-  using C = PagedDecCfg<T, Q8, D, NQ>;
+  using C = PagedDecCfg<T, Q8, D>;
   constexpr int S = C::kSlots;
   constexpr int QP = kQueryPieces<T>, WP = kWeightPieces<T>;
   const PagedAttnArgs& a = p.a;
@@ -182,13 +183,12 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = ring + C::kRing;
   uint8_t* p_s = q_s + C::kQBytes;
-  float* l_s = reinterpret_cast<float*>(p_s + C::kPBufs * C::kPBytes);  // [NQ][128] (NQ > 16)
-  float* red = l_s + C::kLBytes / 4;                              // [NQ][4 warps]
-  float* mc = red + NQ * 4;                                       // [2][NQ]: the maximum in use, the rescale factor
-  float* ml = mc + 2 * NQ;                                        // [2][NQ]: this CTA's m (as it runs) and l
-  float* fc = ml + 2 * NQ;                                        // [NQ]: log2 units a raw score
-  int* lim = reinterpret_cast<int*>(fc + NQ);                     // [2][NQ]: a column's keys [lo, hi)
-  int* vred = lim + 2 * NQ;                                       // [4] (8 words kept): per-warp largest V scale code
+  float* red = reinterpret_cast<float*>(p_s + C::kPBufs * C::kPBytes);  // [kRows][4 warps]
+  float* mc = red + kRows * 4;                                       // [2][kRows]: the maximum in use, the rescale factor
+  float* ml = mc + 2 * kRows;                                        // [2][kRows]: this CTA's m (as it runs) and l
+  float* fc = ml + 2 * kRows;                                        // [kRows]: log2 units a raw score
+  int* lim = reinterpret_cast<int*>(fc + kRows);                     // [2][kRows]: a column's keys [lo, hi)
+  int* vred = lim + 2 * kRows;                                       // [4] (8 words kept): per-warp largest V scale code
   uint64_t* bars = reinterpret_cast<uint64_t*>(vred + 8);
   uint64_t* full = bars;
   uint64_t* empty = full + S;
@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
     const int j = g * kKeys + my_box * p.box;
     slot_in_page = 0;
     if (!mine || j + p.box <= lo || j >= hi) return (int)a.c.pages;
-    const int page = j / a.c.page_size;
-    slot_in_page = j - page * a.c.page_size;
+    const uint32_t page = p.page_size.div((uint32_t)j);
+    slot_in_page = j - (int)(page * p.page_size.d);
     const int id = table[page];
     if (id < 0 || id >= a.c.pages) {
       atomicExch(a.status, (uint32_t)kStatusBadIndex);
@@ -337,12 +337,12 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       return u;
     };
     if constexpr (!Q8) {
-      for (int i = tid; i < NQ * (D / 8); i += 128) {
+      for (int i = tid; i < kRows * (D / 8); i += 128) {
         const int row = i / (D / 8), c = i % (D / 8);
-        *reinterpret_cast<uint4*>(q_s + (c >> 3) * (NQ * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = query(row, c * 8);
+        *reinterpret_cast<uint4*>(q_s + (c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = query(row, c * 8);
       }
     } else {
-      for (int i = tid; i < NQ * 16; i += 128) {  // 16 lanes a row, 8 values each
+      for (int i = tid; i < kRows * 16; i += 128) {  // 16 lanes a row, 8 values each
         const int row = i >> 4, c = i & 15;
         const uint4 u = query(row, c * 8);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -370,17 +370,17 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
             const float2 x = from_e4m3x2(piece[e]);
             f[2 * e] -= x.x, f[2 * e + 1] -= x.y;
           }
-          *reinterpret_cast<uint2*>(q_s + k * (NQ * 128) + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8) =
+          *reinterpret_cast<uint2*>(q_s + k * (kRows * 128) + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8) =
               make_uint2(piece[0] | (piece[1] << 16), piece[2] | (piece[3] << 16));
         }
       }
     }
     for (int i = tid; i < C::kPBufs * C::kPBytes / 16; i += 128) reinterpret_cast<uint4*>(p_s)[i] = make_uint4(0, 0, 0, 0);
-    if (tid < NQ) {
+    if (tid < kRows) {
       const int t = tid / p.group;
       const bool live = tid < p.rows && t < r.n;
       lim[tid] = live ? first_of(t) : 0;
-      lim[NQ + tid] = live ? last_of(t) : 0;
+      lim[kRows + tid] = live ? last_of(t) : 0;
     }
     fence_proxy_async_smem();
   }
@@ -411,23 +411,23 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
         return;
       }
       tc_fence_after();
-      const uint32_t d_tmem = tmem_base + (uint32_t)((j & 1) * NQ);
+      const uint32_t d_tmem = tmem_base + (uint32_t)((j & 1) * kRows);
       if constexpr (!Q8) {
-        constexpr uint32_t idesc = umma_idesc(Elem<T>::kUmmaFormat, 128, NQ, 0, 0);
+        constexpr uint32_t idesc = umma_idesc(Elem<T>::kUmmaFormat, 128, kRows, 0, 0);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           if (leader)
             umma_ss(d_tmem, k_desc + (uint64_t)((s * C::kSlotBytes + (ks >> 2) * kBox) >> 4) + (uint64_t)((ks & 3) * 2),
-                    q_desc + (uint64_t)(((ks >> 2) * (NQ * 128)) >> 4) + (uint64_t)((ks & 3) * 2), idesc, ks != 0 ? 1u : 0u);
+                    q_desc + (uint64_t)(((ks >> 2) * (kRows * 128)) >> 4) + (uint64_t)((ks & 3) * 2), idesc, ks != 0 ? 1u : 0u);
       } else {
-        constexpr uint32_t idesc = umma_idesc_f8(0, 0, 128, NQ, 0);
+        constexpr uint32_t idesc = umma_idesc_f8(0, 0, 128, kRows, 0);
 #pragma unroll
         for (int k = 0; k < QP; ++k)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)  // 32 columns = 32 bytes a step
             if (leader)
               umma_ss_f8(d_tmem, k_desc + (uint64_t)((s * C::kSlotBytes) >> 4) + (uint64_t)(ks * 2),
-                         q_desc + (uint64_t)((k * NQ * 128) >> 4) + (uint64_t)(ks * 2), idesc, (k | ks) != 0 ? 1u : 0u);
+                         q_desc + (uint64_t)((k * kRows * 128) >> 4) + (uint64_t)(ks * 2), idesc, (k | ks) != 0 ? 1u : 0u);
       }
       if (leader) {
         tc_commit(&empty[s]);
@@ -445,22 +445,22 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       const uint64_t vb = v_desc + (uint64_t)((s * C::kSlotBytes) >> 4);
       const uint64_t pb = p_desc + (uint64_t)(((j % C::kPBufs) * C::kPBytes) >> 4);
       if constexpr (!Q8) {
-        constexpr uint32_t idesc = umma_idesc(Elem<T>::kUmmaFormat, 128, 2 * NQ, 1, 0);
+        constexpr uint32_t idesc = umma_idesc(Elem<T>::kUmmaFormat, 128, 2 * kRows, 1, 0);
 #pragma unroll
         for (int ks = 0; ks < kKeys / 16; ++ks)
           if (leader)
-            umma_ss(tmem_base + 2 * NQ, vb + (uint64_t)(ks * (2048 >> 4)),
-                    pb + (uint64_t)(((ks >> 2) * (2 * NQ * 128)) >> 4) + (uint64_t)((ks & 3) * 2), idesc,
+            umma_ss(tmem_base + 2 * kRows, vb + (uint64_t)(ks * (2048 >> 4)),
+                    pb + (uint64_t)(((ks >> 2) * (2 * kRows * 128)) >> 4) + (uint64_t)((ks & 3) * 2), idesc,
                     (j | ks) != 0 ? 1u : 0u);
       } else {
 #pragma unroll
         for (int k = 0; k < WP; ++k) {
-          const uint32_t idesc = k == 0 ? umma_idesc_f8(0, 0, 128, NQ, 1) : umma_idesc_f8(0, 1, 128, NQ, 1);
+          const uint32_t idesc = k == 0 ? umma_idesc_f8(0, 0, 128, kRows, 1) : umma_idesc_f8(0, 1, 128, kRows, 1);
 #pragma unroll
           for (int ks = 0; ks < kKeys / 32; ++ks)  // 32 keys = 4 KiB of V, 32 bytes of a weight row
             if (leader)
-              umma_ss_f8(tmem_base + (uint32_t)((k == 0 ? 2 : 3) * NQ), vb + (uint64_t)(ks * (4096 >> 4)),
-                         pb + (uint64_t)((k * NQ * 128) >> 4) + (uint64_t)(ks * 2), idesc,
+              umma_ss_f8(tmem_base + (uint32_t)((k == 0 ? 2 : 3) * kRows), vb + (uint64_t)(ks * (4096 >> 4)),
+                         pb + (uint64_t)((k * kRows * 128) >> 4) + (uint64_t)(ks * 2), idesc,
                          (j | ks) != 0 || k > 1 ? 1u : 0u);
         }
       }
@@ -473,105 +473,83 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
   } else {
     // ---------------- softmax: thread = key ----------------
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    const uint32_t o_tmem = tmem_base + 2 * NQ + lane_addr;
-    // `f` on the columns there are: W where the registers hold all of them
-    auto widths = [&](int live, auto&& f) {
-      if constexpr (NQ == 16) f(std::integral_constant<int, W>{});
-      else by_width(live, f);
-    };
+    const uint32_t o_tmem = tmem_base + 2 * kRows + lane_addr;
     float m_run = -INFINITY;  // of column `tid`: thread c keeps the running maximum of column c
     float l_lane[W];
 #pragma unroll
     for (int c = 0; c < W; ++c) l_lane[c] = 0.f;
-    if (tid < 2 * NQ) mc[tid] = 0.f;
+    if (tid < 2 * kRows) mc[tid] = 0.f;
     // the maxima as they are compared with: nothing is above those of columns that are not there
-    if (tid < NQ) ml[tid] = tid < p.rows ? -INFINITY : INFINITY;
-    if (NQ > 16)
-      for (int c = 0; c < NQ; ++c) l_s[c * 128 + tid] = 0.f;
-    const float my_fc = Q8 ? (tid < NQ ? fc[tid] : 0.f) : p.scale_log2;
+    if (tid < kRows) ml[tid] = tid < p.rows ? -INFINITY : INFINITY;
+    const float my_fc = Q8 ? (tid < kRows ? fc[tid] : 0.f) : p.scale_log2;
     bool live = true;  // false once a bounded wait ran out: barriers are still walked, nothing is waited for
     uint32_t sr[W];
     // 8-bit pages: my key's scale codes, its page looked up a block ahead
     uint32_t k_code = 127, v_code = 127;
     int v_top = -1;  // the largest V scale code so far: weights are taken relative to it
-    auto key_page = [&](int j) -> int {
+    int page_next = -1, slot_next = 0;
+    auto key_page = [&](int j, int& slot) -> int {
       const int key = (g_lo + j) * kKeys + tid;
-      return j < n && key >= lo && key < hi ? table[key / a.c.page_size] : -1;
+      slot = 0;
+      if (j >= n || key < lo || key >= hi) return -1;
+      const uint32_t page = p.page_size.div((uint32_t)key);
+      slot = key - (int)(page * p.page_size.d);
+      return table[page];
     };
-    auto key_codes = [&](int j, int page, uint32_t& kc, uint32_t& vc) {
-      const int key = (g_lo + j) * kKeys + tid;
+    auto key_codes = [&](int page, int slot, uint32_t& kc, uint32_t& vc) {
       kc = vc = 127u;
       if (page >= 0 && page < a.c.pages) {
-        const int64_t slot = key % a.c.page_size;
         kc = a.c.k_scale[page * a.c.ks_sp + hk * a.c.ks_sh + slot];
         vc = a.c.v_scale[page * a.c.vs_sp + hk * a.c.vs_sh + slot];
       }
     };
-    int page_next = -1;
     if constexpr (Q8) {
-      key_codes(0, key_page(0), k_code, v_code);
-      page_next = key_page(1);
+      const int page = key_page(0, slot_next);
+      key_codes(page, slot_next, k_code, v_code);
+      page_next = key_page(1, slot_next);
     }
     for (int j = 0; j < n; ++j) {
       uint32_t k_code_next = 127, v_code_next = 127;
       if constexpr (Q8) {
-        key_codes(j + 1, page_next, k_code_next, v_code_next);
-        page_next = key_page(j + 2);
+        key_codes(page_next, slot_next, k_code_next, v_code_next);
+        page_next = key_page(j + 2, slot_next);
       }
       if (live && !mbar_wait(&s_full[j & 1], (j >> 1) & 1, a.status)) live = false;
       tc_fence_after();
-      const uint32_t s_tmem = tmem_base + (uint32_t)((j & 1) * NQ) + lane_addr;
+      const uint32_t s_tmem = tmem_base + (uint32_t)((j & 1) * kRows) + lane_addr;
       const int base = (g_lo + j) * kKeys;
       const int key = base + tid;
       const bool real = key >= lo && key < hi;
       // whether some query token of the row does not see some key of the block
       const bool edge = base < all_lo || base + kKeys > all_hi;
       const float ks = Q8 ? scale_value(k_code) : 1.f;
-      auto load_scores = [&](int q0) {
-        tmem_ld_w<W>(s_tmem + q0, sr);
-        if (Q8) {
+      tmem_ld_w<W>(s_tmem, sr);
+      if (Q8) {
 #pragma unroll
-          for (int c = 0; c < W; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * ks);
-        }
-        if (edge) {
+        for (int c = 0; c < W; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * ks);
+      }
+      if (edge) {
 #pragma unroll
-          for (int c = 0; c < W; ++c)
-            if (key < lim[q0 + c] || key >= lim[NQ + q0 + c]) sr[c] = 0xff800000u;
-        }
-      };
+        for (int c = 0; c < W; ++c)
+          if (key < lim[c] || key >= lim[kRows + c]) sr[c] = 0xff800000u;
+      }
       // Most blocks bring no score (and no V scale) above what the running maxima allow: one
       // barrier says so, and the maxima and the reference stay. The first block sets them.
       bool over = j == 0;
-#pragma unroll 1
-      for (int q0 = 0; q0 < p.rows; q0 += 16) {
-        load_scores(q0);
-        auto compare = [&](auto width) {
 #pragma unroll
-          for (int c = 0; c < decltype(width)::value; ++c)
-            over = over || __uint_as_float(sr[c]) * (Q8 ? fc[q0 + c] : p.scale_log2) > ml[q0 + c] + kAdoptAbove<Q8>;
-        };
-        widths(p.rows - q0, compare);
-        if (NQ == 16) break;
-      }
+      for (int c = 0; c < W; ++c)
+        over = over || __uint_as_float(sr[c]) * (Q8 ? fc[c] : p.scale_log2) > ml[c] + kAdoptAbove<Q8>;
       if constexpr (Q8) over = over || (real && v_code != 255u && (int)v_code > v_top);
       bool moved = false;
       float v_corr = 1.f;  // 2^(old - new) of the V scales' reference
       if (barrier_or(2, over)) {
-#pragma unroll 1
-        for (int q0 = 0; q0 < p.rows; q0 += 16) {
-          if (NQ > 16) load_scores(q0);
-          float mine_max = 0.f;
-          auto maxima = [&](auto width) {
+        float mine_max = 0.f;
 #pragma unroll
-            for (int c = 0; c < decltype(width)::value; ++c) {
-              const float wm = redux_max(__uint_as_float(sr[c]));
-              if (lane == c) mine_max = wm;
-            }
-          };
-          widths(p.rows - q0, maxima);
-          if (lane < 16 && q0 + lane < p.rows) red[(q0 + lane) * 4 + warp] = mine_max;
-          if (NQ == 16) break;
+        for (int c = 0; c < W; ++c) {
+          const float wm = redux_max(__uint_as_float(sr[c]));
+          if (lane == c) mine_max = wm;
         }
+        if (lane < p.rows) red[lane * 4 + warp] = mine_max;
         if constexpr (Q8) {
           const int wv = __reduce_max_sync(0xffffffffu, real && v_code != 255u ? (int)v_code : -1);
           if (lane == 0) vred[warp] = wv;
@@ -598,7 +576,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
             m_run = m_new;
           }
           mc[tid] = m_run == -INFINITY ? 0.f : m_run;
-          mc[NQ + tid] = corr;
+          mc[kRows + tid] = corr;
           ml[tid] = m_run;
         }
         moved = barrier_or(2, moved);
@@ -607,28 +585,19 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
         // O holds the blocks before this one: rescale it once the last P.V is complete
         if (live && !mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, a.status)) live = false;
         tc_fence_after();
+        float f[W];
+#pragma unroll
+        for (int c = 0; c < W; ++c) f[c] = mc[kRows + c];
 #pragma unroll 1
-        for (int q0 = 0; q0 < p.rows; q0 += 16) {
-          float f[W];
+        for (int half = 0; half < 2; ++half) {
+          uint32_t orr[W];
+          tmem_ld_w<W>(o_tmem + half * kRows, orr);
 #pragma unroll
-          for (int c = 0; c < W; ++c) f[c] = mc[NQ + q0 + c];
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            uint32_t orr[W];
-            tmem_ld_w<W>(o_tmem + half * NQ + q0, orr);
-#pragma unroll
-            for (int c = 0; c < W; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * (f[c] * v_corr));
-            tmem_st_w<W>(o_tmem + half * NQ + q0, orr);
-          }
-          if (NQ == 16) {
-#pragma unroll
-            for (int c = 0; c < W; ++c) l_lane[c] *= f[c];
-            break;
-          } else {
-#pragma unroll
-            for (int c = 0; c < W; ++c) l_s[(q0 + c) * 128 + tid] *= f[c];
-          }
+          for (int c = 0; c < W; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * (f[c] * v_corr));
+          tmem_st_w<W>(o_tmem + half * kRows, orr);
         }
+#pragma unroll
+        for (int c = 0; c < W; ++c) l_lane[c] *= f[c];
         tmem_st_wait();
       }
       // the block that last used this buffer of weights has been multiplied
@@ -638,75 +607,56 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       // this key's V scale over the largest; a NaN row's is NaN
       float vs = 1.f;
       if constexpr (Q8) vs = !real ? 0.f : v_code == 255u ? __uint_as_float(0x7fffffffu) : power_below((int)v_code - v_top);
-#pragma unroll 1
-      for (int q0 = 0; q0 < p.rows; q0 += 16) {
-        if (NQ > 16) load_scores(q0);
-        // All loads, then the arithmetic, then all stores: the compiler may not move a load
-        // of a maximum or a sum above a store of a weight.
-        auto weights = [&](auto width) {
-          constexpr int N = decltype(width)::value;
-          float mu[N], lv[N], sc[N];
+      // All loads, then the arithmetic, then all stores: the compiler may not move a load of a
+      // maximum above a store of a weight.
+      float mu[W], sc[W];
 #pragma unroll
-          for (int c = 0; c < N; ++c) {
-            mu[c] = mc[q0 + c];
-            sc[c] = Q8 ? fc[q0 + c] : p.scale_log2;
-            if (NQ > 16) lv[c] = l_s[(q0 + c) * 128 + tid];
+      for (int c = 0; c < W; ++c) mu[c] = mc[c], sc[c] = Q8 ? fc[c] : p.scale_log2;
+      if constexpr (!Q8) {
+        uint8_t* pbox = p_s + (j % C::kPBufs) * C::kPBytes + (tid >> 6) * (2 * kRows * 128) + (tid & 7) * 2;
+        const int chunk = (tid & 63) >> 3;
+        T high[W], low[W];
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          const float pr = ex2_approx(fmaf(__uint_as_float(sr[c]), sc[c], -mu[c]));
+          l_lane[c] += pr;
+          const float up = pr * kValueUp<T>;
+          high[c] = Elem<T>::from_f(up);
+          low[c] = Elem<T>::from_f((up - Elem<T>::to_f(high[c])) * kRestUp<T>);
+        }
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          uint8_t* dst = pbox + c * 128 + ((chunk ^ (c & 7)) << 4);
+          *reinterpret_cast<T*>(dst) = high[c];
+          *reinterpret_cast<T*>(dst + kRows * 128) = low[c];
+        }
+      } else {
+        uint8_t* pbox = p_s + (j % C::kPBufs) * C::kPBytes + (tid & 15);
+        const int chunk = tid >> 4;
+        uint32_t piece[WP][W / 2];  // two columns each
+#pragma unroll
+        for (int c = 0; c < W; c += 2) {
+          const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c]), sc[c], -mu[c]));
+          const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + 1]), sc[c + 1], -mu[c + 1]));
+          l_lane[c] += p0, l_lane[c + 1] += p1;
+          float w0 = real ? p0 * vs : 0.f, w1 = real ? p1 * vs : 0.f;
+          piece[0][c / 2] = to_e4m3x2(w0, w1);
+          const float2 x = from_e4m3x2(piece[0][c / 2]);
+          w0 = (w0 - x.x) * kRemainderUp, w1 = (w1 - x.y) * kRemainderUp;
+#pragma unroll
+          for (int k = 1; k < WP; ++k) {
+            piece[k][c / 2] = to_e5m2x2(w0, w1);
+            if (k + 1 < WP) {
+              const float2 y = from_e5m2x2(piece[k][c / 2]);
+              w0 -= y.x, w1 -= y.y;
+            }
           }
-          if constexpr (!Q8) {
-            uint8_t* pbox = p_s + (j % C::kPBufs) * C::kPBytes + (tid >> 6) * (2 * NQ * 128) + (tid & 7) * 2;
-            const int chunk = (tid & 63) >> 3;
-            T high[N], low[N];
+        }
 #pragma unroll
-            for (int c = 0; c < N; ++c) {
-              const float pr = ex2_approx(fmaf(__uint_as_float(sr[c]), sc[c], -mu[c]));
-              if (NQ > 16) lv[c] += pr;
-              else l_lane[c] += pr;
-              const float up = pr * kValueUp<T>;
-              high[c] = Elem<T>::from_f(up);
-              low[c] = Elem<T>::from_f((up - Elem<T>::to_f(high[c])) * kRestUp<T>);
-            }
+        for (int c = 0; c < W; ++c)
 #pragma unroll
-            for (int c = 0; c < N; ++c) {
-              uint8_t* dst = pbox + (q0 + c) * 128 + ((chunk ^ (c & 7)) << 4);
-              *reinterpret_cast<T*>(dst) = high[c];
-              *reinterpret_cast<T*>(dst + NQ * 128) = low[c];
-            }
-          } else {
-            uint8_t* pbox = p_s + (j % C::kPBufs) * C::kPBytes + (tid & 15);
-            const int chunk = tid >> 4;
-            uint32_t piece[WP][N / 2];  // two columns each
-#pragma unroll
-            for (int c = 0; c < N; c += 2) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c]), sc[c], -mu[c]));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + 1]), sc[c + 1], -mu[c + 1]));
-              if (NQ > 16) lv[c] += p0, lv[c + 1] += p1;
-              else l_lane[c] += p0, l_lane[c + 1] += p1;
-              float w0 = real ? p0 * vs : 0.f, w1 = real ? p1 * vs : 0.f;
-              piece[0][c / 2] = to_e4m3x2(w0, w1);
-              const float2 x = from_e4m3x2(piece[0][c / 2]);
-              w0 = (w0 - x.x) * kRemainderUp, w1 = (w1 - x.y) * kRemainderUp;
-#pragma unroll
-              for (int k = 1; k < WP; ++k) {
-                piece[k][c / 2] = to_e5m2x2(w0, w1);
-                if (k + 1 < WP) {
-                  const float2 y = from_e5m2x2(piece[k][c / 2]);
-                  w0 -= y.x, w1 -= y.y;
-                }
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < N; ++c)
-#pragma unroll
-              for (int k = 0; k < WP; ++k)
-                pbox[k * (NQ * 128) + (q0 + c) * 128 + ((chunk ^ (c & 7)) << 4)] =
-                    (uint8_t)(piece[k][c / 2] >> ((c & 1) * 8));
-          }
-#pragma unroll
-          for (int c = 0; c < N; ++c)
-            if (NQ > 16) l_s[(q0 + c) * 128 + tid] = lv[c];
-        };
-        widths(p.rows - q0, weights);
-        if (NQ == 16) break;
+          for (int k = 0; k < WP; ++k)
+            pbox[k * (kRows * 128) + c * 128 + ((chunk ^ (c & 7)) << 4)] = (uint8_t)(piece[k][c / 2] >> ((c & 1) * 8));
       }
       if (base < lo || base + kKeys > hi) {
         // The block's rows outside the visible keys hold whatever the pages hold there:
@@ -733,26 +683,20 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       float* op = reinterpret_cast<float*>(ring);
       const float low_down = Q8 ? 1.f / kRemainderUp : 1.f / kRestUp<T>;
       const float o_up = Q8 ? scale_value(v_top < 0 ? 127u : (uint32_t)v_top) : 1.f / kValueUp<T>;
-#pragma unroll 1
-      for (int q0 = 0; q0 < p.rows; q0 += 16) {
-        float mine_sum = 0.f;
+      float mine_sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        const float x = warp_sum(l_lane[c]);
+        if (lane == c) mine_sum = x;
+      }
+      if (lane < p.rows) red[lane * 4 + warp] = mine_sum;
+      if (warp * 32 < D) {
+        uint32_t low[W];
+        tmem_ld_w<W>(o_tmem, sr);
+        tmem_ld_w<W>(o_tmem + kRows, low);
 #pragma unroll
         for (int c = 0; c < W; ++c)
-          if (q0 + c < p.rows) {
-            const float s = warp_sum(NQ == 16 ? l_lane[c] : l_s[(q0 + c) * 128 + tid]);
-            if (lane == c) mine_sum = s;
-          }
-        if (lane < 16 && q0 + lane < p.rows) red[(q0 + lane) * 4 + warp] = mine_sum;
-        if (warp * 32 < D) {
-          uint32_t low[W];
-          tmem_ld_w<W>(o_tmem + q0, sr);
-          tmem_ld_w<W>(o_tmem + NQ + q0, low);
-#pragma unroll
-          for (int c = 0; c < W; ++c)
-            if (q0 + c < p.rows)
-              op[(q0 + c) * D + tid] = fmaf(__uint_as_float(low[c]), low_down, __uint_as_float(sr[c])) * o_up;
-        }
-        if (NQ == 16) break;
+          if (c < p.rows) op[c * D + tid] = fmaf(__uint_as_float(low[c]), low_down, __uint_as_float(sr[c])) * o_up;
       }
       named_barrier(1, 128);
     }
@@ -763,7 +707,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
         l = (w4.x + w4.y) + (w4.z + w4.w);
       }
       ml[tid] = n > 0 ? m_run : -INFINITY;
-      ml[NQ + tid] = l;
+      ml[kRows + tid] = l;
     }
     tc_fence_before();
   }
@@ -784,18 +728,31 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D, NQ>::kPerS
       const int h = hk * p.group + c % p.group;
       float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (tq < r.n) {
-        for (uint32_t k = 0; k < csize; ++k) m = fmaxf(m, ld_cluster_f32(cluster_at(ml_addr + c * 4, k)));
-        for (uint32_t k = 0; k < csize; ++k) {
-          const float mr = ld_cluster_f32(cluster_at(ml_addr + c * 4, k));
-          const float lr = ld_cluster_f32(cluster_at(ml_addr + (NQ + c) * 4, k));
-          if (lr == 0.f) continue;  // the share saw no key (its sum says so: NaN scores leave the maximum at -inf too)
-          const float w = mr == -INFINITY ? 1.f : ex2_approx(mr - m);
-          l = fmaf(w, lr, l);
-          const uint32_t src = cluster_at(op_addr + (c * D + d0) * 4, k);
-          const float4 x = ld_cluster_f32x4(src), y = ld_cluster_f32x4(src + 16);
-          acc[0] = fmaf(w, x.x, acc[0]), acc[1] = fmaf(w, x.y, acc[1]), acc[2] = fmaf(w, x.z, acc[2]);
-          acc[3] = fmaf(w, x.w, acc[3]), acc[4] = fmaf(w, y.x, acc[4]), acc[5] = fmaf(w, y.y, acc[5]);
-          acc[6] = fmaf(w, y.z, acc[6]), acc[7] = fmaf(w, y.w, acc[7]);
+        // four CTAs' states at a time: one after the other, each is a trip across the cluster
+        for (uint32_t k0 = 0; k0 < csize; k0 += 4) {
+          float mr[4], lr[4];
+          float4 x[4], y[4];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t k = k0 + u < csize ? k0 + u : k0;
+            mr[u] = ld_cluster_f32(cluster_at(ml_addr + c * 4, k));
+            lr[u] = ld_cluster_f32(cluster_at(ml_addr + (kRows + c) * 4, k));
+            const uint32_t src = cluster_at(op_addr + (c * D + d0) * 4, k);
+            x[u] = ld_cluster_f32x4(src), y[u] = ld_cluster_f32x4(src + 16);
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) {
+            // a share that saw no key (its sum says so: NaN scores leave the maximum at -inf too), or none at all
+            if (k0 + u >= csize || lr[u] == 0.f) continue;
+            const float m_new = fmaxf(m, mr[u]);
+            const float f0 = m == -INFINITY ? 1.f : ex2_approx(m - m_new), f1 = mr[u] == -INFINITY ? 1.f : ex2_approx(mr[u] - m_new);
+            m = m_new;
+            l = fmaf(l, f0, f1 * lr[u]);
+            acc[0] = fmaf(acc[0], f0, f1 * x[u].x), acc[1] = fmaf(acc[1], f0, f1 * x[u].y);
+            acc[2] = fmaf(acc[2], f0, f1 * x[u].z), acc[3] = fmaf(acc[3], f0, f1 * x[u].w);
+            acc[4] = fmaf(acc[4], f0, f1 * y[u].x), acc[5] = fmaf(acc[5], f0, f1 * y[u].y);
+            acc[6] = fmaf(acc[6], f0, f1 * y[u].z), acc[7] = fmaf(acc[7], f0, f1 * y[u].w);
+          }
         }
       }
       const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -842,26 +799,26 @@ int cluster_of(int64_t pairs, int64_t blocks, int per_sm) {
   while (csize < 16 && csize * 2 <= blocks &&
          (pairs * csize * 2 <= room || (pairs * csize <= room && blocks >= 32 * csize * 2))) {
     if (csize == 8 && pairs > 6 * per_sm) break;
-    if (csize == 4 && per_sm == 1 && pairs > 12) break;
     csize *= 2;
   }
   return csize;
 }
 
-template <typename T, bool Q8, int D, int NQ, int W>
+template <typename T, bool Q8, int D, int W>
 int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
-  using C = PagedDecCfg<T, Q8, D, NQ>;
+  using C = PagedDecCfg<T, Q8, D>;
   CUtensorMap tk, tv;
   PagedDecParams p{};
   p.box = page_box(a.c.page_size, kKeys);
+  p.page_size = divider((uint32_t)a.c.page_size);
   if (!page_map(&tk, a.c, false, Q8 ? 128 : 64, p.box) || !page_map(&tv, a.c, true, Q8 ? 128 : 64, p.box)) return -1;
   static bool attr_seen[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_seen[dev & 63]) {
-    if (cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, NQ, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)C::kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, NQ, W>, cudaFuncAttributeNonPortableClusterSizeAllowed,
+        cudaFuncSetAttribute(attention_paged_decode_kernel<T, Q8, D, W>, cudaFuncAttributeNonPortableClusterSizeAllowed,
                              1) != cudaSuccess)
       return -1;
     attr_seen[dev & 63] = true;
@@ -873,21 +830,19 @@ int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) 
   const int64_t pairs = a.batch * a.c.kv_heads;
   const int csize = cluster_of(pairs, most_blocks(a), C::kPerSm);
   p.longest_first = a.batch > 1 && a.batch <= kSortedRows && pairs * csize > (int64_t)sms() * C::kPerSm;
-  if (launch_pdl(attention_paged_decode_kernel<T, Q8, D, NQ, W>, dim3((unsigned)(pairs * csize)), dim3(kThreadsDec), C::kSmem,
+  if (launch_pdl(attention_paged_decode_kernel<T, Q8, D, W>, dim3((unsigned)(pairs * csize)), dim3(kThreadsDec), C::kSmem,
                  s, (unsigned)csize, a.batch * a.t, tk, tv, p) != cudaSuccess)
     return -1;
-  snprintf(cfg, cfg_len, "{rows:%d,bkv:%d,d:%d,box:%d,cluster:%d%s}", NQ, kKeys, a.c.d, p.box, csize, Q8 ? ",e4m3" : "");
+  snprintf(cfg, cfg_len, "{rows:%d,bkv:%d,d:%d,box:%d,cluster:%d%s}", W, kKeys, a.c.d, p.box, csize, Q8 ? ",e4m3" : "");
   return 0;
 }
 
 template <typename T, bool Q8, int D>
 int run_width(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   const int64_t rows = a.t * (a.heads / a.c.kv_heads);
-  if (rows <= 4) return run_rows<T, Q8, D, 16, 4>(a, s, cfg, cfg_len);
-  if (rows <= 8) return run_rows<T, Q8, D, 16, 8>(a, s, cfg, cfg_len);
-  if (rows <= 16) return run_rows<T, Q8, D, 16, 16>(a, s, cfg, cfg_len);
-  if (rows <= 32) return run_rows<T, Q8, D, 32, 16>(a, s, cfg, cfg_len);
-  return run_rows<T, Q8, D, 64, 16>(a, s, cfg, cfg_len);
+  if (rows <= 4) return run_rows<T, Q8, D, 4>(a, s, cfg, cfg_len);
+  if (rows <= 8) return run_rows<T, Q8, D, 8>(a, s, cfg, cfg_len);
+  return run_rows<T, Q8, D, 16>(a, s, cfg, cfg_len);
 }
 
 template <typename T>
@@ -941,11 +896,17 @@ bool attention_paged_tiles(const PagedAttnArgs& a) {
   return true;
 }
 
-bool attention_paged_decode_covers(const PagedAttnArgs& a) {
-  if (!attention_paged_tiles(a)) return false;
-  const int64_t rows = a.t * (a.heads / a.c.kv_heads);
-  return a.t <= 64 && rows <= 64 && a.batch * a.c.kv_heads <= (1 << 26);
+// Up to 16 query rows a KV head, whatever the keys. With more of them this form loses to the
+// 128-row tiles, which share the keys out evenly and take 64 rows for what they take for one
+// (measured here with 32 and 64 columns against there: 24 rows x 100..2500 keys x 27 query rows
+// 66 us | 27; 64 x 64..4095 x 24 196 | 173; 16 x 8000..32767 in e4m3 x 24 516 | 386; 1 x 30000 x
+// 60 148 | 62; 1 x 776 x 24 20 | 19). Where it takes the call, the other way round: 24 rows x 15
+// query rows 20 | 27, 64 x 12 110 | 174, 16 in e4m3 x 12 215 | 386, 1 x 776 x 12 12 | 19.
+bool attention_paged_few_rows(const PagedAttnArgs& a) {
+  return a.t * (a.heads / a.c.kv_heads) <= kRows && a.batch * a.c.kv_heads <= (1 << 26);
 }
+
+bool attention_paged_decode_covers(const PagedAttnArgs& a) { return attention_paged_tiles(a) && attention_paged_few_rows(a); }
 
 int launch_attention_paged_decode(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   return a.dtype == SVODB_BF16 ? run_type<__nv_bfloat16>(a, s, cfg, cfg_len) : run_type<__half>(a, s, cfg, cfg_len);

@@ -282,7 +282,8 @@ struct PagedAttnArgs {
 int launch_attention_paged_exact(const PagedAttnArgs& a, cudaStream_t s);
 // What the tensor-core kernels over pages take in common.
 bool attention_paged_tiles(const PagedAttnArgs& a);
-// Up to 64 query rows a KV head: keys as the M of both MMAs.
+// Whether the few-row kernel (keys as the M of both MMAs) is the better one, by the shapes alone.
+bool attention_paged_few_rows(const PagedAttnArgs& a);
 bool attention_paged_decode_covers(const PagedAttnArgs& a);
 int launch_attention_paged_decode(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len);
 // Any number of query rows: 128-row tiles of tokens x the heads of a KV head.

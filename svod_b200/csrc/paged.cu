@@ -47,19 +47,6 @@ __device__ __forceinline__ void widen8(uint4 u, float* f) {
   }
 }
 
-// n / d for 0 <= n < 2^31 without a division: (floor(n m / 2^32) + n) >> shift with
-// m = floor(2^32 (2^shift - d) / d) + 1, 2^shift >= d (Granlund and Montgomery's method).
-struct Divider {
-  uint32_t d, m, shift;
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> shift; }
-};
-Divider divider(uint32_t d) {
-  Divider v{d, 0, 0};
-  while ((1ull << v.shift) < d) ++v.shift;
-  v.m = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
-  return v;
-}
-
 // Head rows a thread has a part of at once, their look-ups and loads on their way together. A
 // row on its way into 8 bits holds 16 values in registers: there more threads an SM do more
 // (10240 tokens x 8 heads x 128: 20.9 us with four, 17.5 with two, 18.9 with one).

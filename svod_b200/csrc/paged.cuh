@@ -60,5 +60,18 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t u) {
   return __half22float2(__half2(h));
 }
 
+// n / d for 0 <= n < 2^31 without a division: (floor(n m / 2^32) + n) >> shift with
+// m = floor(2^32 (2^shift - d) / d) + 1, 2^shift >= d (Granlund and Montgomery's method).
+struct Divider {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> shift; }
+};
+inline Divider divider(uint32_t d) {
+  Divider v{d, 0, 0};
+  while ((1ull << v.shift) < d) ++v.shift;
+  v.m = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+  return v;
+}
+
 }  // namespace paged
 }  // namespace svodb
