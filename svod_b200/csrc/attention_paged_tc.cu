@@ -25,7 +25,7 @@
 //
 // 8-bit pages: a fourth warpgroup widens each block from a ring of raw e4m3 blocks into the
 // 16-bit rings, value * 2^e, exact in bf16 (a value is 4 bits) and rounded once in f16's
-// subnormals. A thread moves half a key's row: the e4m3 fields are shifted to where the 16-bit
+// subnormals. A thread moves a key's row: the e4m3 fields are shifted to where the 16-bit
 // type has them and one packed multiply puts exponent bias and scale right, 5 instructions a
 // pair of values (a conversion through f32 is 6, on slower pipes).
 //
@@ -69,7 +69,7 @@ struct PagedTcParams {
   PagedAttnArgs a;
   int group, tile_tokens;  // tokens of a 128-row tile: 128 / group
   int box;
-  int n_qt;                // items of two tiles a (row, KV head)
+  Divider page_size;
   float scale_log2;
   int* heads_of_split;     // [grid][kSplitInts]: the split item whose first part a CTA has
   float* parts;            // [grid][2][part floats]
@@ -203,21 +203,21 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       mbar_init(&tail_done[i], 1);
       mbar_init(&o_empty[i], 4);                // the tile's four softmax warps
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], Q8 ? 15 : 11);  // query loader, two issuers, eight softmax warps, four widening ones
+      mbar_init(&item_empty[i], Q8 ? 15 : 11);  // value loader, two issuers, eight softmax warps, four widening ones
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);  // one arrival per softmax warp
     }
     for (int i = 0; i < S; ++i) {
-      mbar_init(&k_full[i], Q8 ? 4 : 1);  // widening warps, or the loader's copies
+      mbar_init(&k_full[i], Q8 ? 2 : 1);  // widening warps, or the loader's copies
       mbar_init(&k_empty[i], 2);          // released by both tiles' issuers
-      mbar_init(&v_full[i], Q8 ? 4 : 1);
+      mbar_init(&v_full[i], Q8 ? 2 : 1);
       mbar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < R; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 4);
+      mbar_init(&raw_empty[i], 2);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmap_q);
@@ -238,8 +238,61 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int nb = kBKV / p.box;
+    constexpr int kCols = Q8 ? 1 : D / 64;
+    const int my_box = lane % nb, my_col = lane / nb;
+    const bool mine = my_col < kCols;
+    // Lane 0's bounded wait, for the warp.
+    auto wait_by_lane0 = [&](uint64_t* bar, uint32_t parity) {
+      bool done = true;
+      if (lane == 0) done = mbar_wait(bar, parity, a.status);
+      return __shfl_sync(0xffffffffu, (int)done, 0) != 0;
+    };
+    // A part's blocks of keys (or values), the lanes issuing a block's boxes side by side; `pos`
+    // counts the blocks of all parts. A copy per lane is a trip through the warp's uniform
+    // registers each: keys and values go by a warp of their own (pages of 16 tokens: 16 copies a
+    // block, 1.5 us by one warp where the block's arithmetic takes 1.2).
+    auto load_blocks = [&](const PagedWork& w, int kv, uint32_t& pos) {
+      const int32_t* table = a.c.table + (int64_t)w.b * a.c.table_sb;
+      auto look_up = [&](int blk, int& at) -> int {
+        const int j = blk * kBKV + my_box * p.box;
+        at = 0;
+        if (!mine || blk >= w.u_hi || j + p.box <= w.key_lo || j >= w.key_hi) return (int)a.c.pages;
+        const uint32_t page = p.page_size.div((uint32_t)j);
+        at = j - (int)(page * p.page_size.d);
+        const int id = table[page];
+        if (id < 0 || id >= a.c.pages) {
+          atomicExch(a.status, (uint32_t)kStatusBadIndex);
+          return (int)a.c.pages;
+        }
+        return id;
+      };
+      const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
+      int next_at;
+      int next_id = look_up(w.u_lo, next_at);
+      for (int j = w.u_lo; j < w.u_hi; ++j, ++pos) {
+        const int id = next_id, at = next_at;
+        next_id = look_up(j + 1, next_at);
+        uint64_t *full, *empty;
+        uint8_t* to;
+        uint32_t round;
+        if constexpr (Q8) {  // the raw ring's stages: K V K V
+          static_assert(R == 4);
+          const int st = (int)((pos & 1) << 1) | kv;
+          full = raw_full + st, empty = raw_empty + st, to = raw_s + st * C::kRawBytes, round = pos >> 1;
+        } else {
+          const int st = (int)(pos % S);
+          full = (kv ? v_full : k_full) + st, empty = (kv ? v_empty : k_empty) + st, to = (kv ? v_s : k_s) + st * KB, round = pos / S;
+        }
+        if (!wait_by_lane0(empty, (round & 1) ^ 1)) return false;
+        if (lane == 0) mbar_expect_tx(full, Q8 ? C::kRawBytes : KB);
+        __syncwarp();
+        if (mine) tma_load_4d(to + my_col * KBOX + my_box * p.box * 128, map, full, my_col * 64, w.hk, at, id);
+      }
+      return true;
+    };
     if (warp == 0) {
-      // ---------------- the CTA's run of the work, and the TMA loads ----------------
+      // ---------------- the CTA's run of the work, and its keys ----------------
       // What a row's items weigh, for one KV head.
       auto weigh = [&](const Row& r) -> int64_t {
         int64_t w = 0;
@@ -304,19 +357,8 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         for (int64_t w = item_blocks(p, row, 0) + kItemCost; x + w <= c0; w = item_blocks(p, row, q) + kItemCost) x += w, ++q;
       }
       SplitItem split{0, 0, 0, 0, 0, 0};
-      const int nb = kBKV / p.box;
-      constexpr int kCols = Q8 ? 1 : D / 64;
-      const int my_box = lane % nb, my_col = lane / nb;
-      const bool mine = my_col < kCols;
-      int s = 0;  // ring slot of the next block (16-bit pages) or copy (8-bit)
-      uint32_t ph = 0;
+      uint32_t pos = 0;
       bool ok = true;
-      auto wait_by_lane0 = [&](uint64_t* bar, uint32_t parity) {
-        bool done = true;
-        if (lane == 0) done = mbar_wait(bar, parity, a.status);
-        ok = __shfl_sync(0xffffffffu, (int)done, 0) != 0;
-        return ok;
-      };
       uint32_t n_it = 0;
       // (a CTA whose run would begin behind the last item has none)
       while (c0 < c1 && x < c1 && ok) {
@@ -354,52 +396,15 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
             w.u_lo = w.r1.lo, w.u_hi = w.r1.hi;
           }
           const int slot = (int)(n_it & 1);
-          if (!wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1)) break;
+          ok = wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1);
+          if (!ok) break;
           if (lane == 0) {
             item_ring[slot] = w;
             __threadfence_block();
             mbar_arrive(&item_full[slot]);
           }
           ++n_it;
-          const int32_t* table = a.c.table + (int64_t)b * a.c.table_sb;
-          auto look_up = [&](int blk, int& at) -> int {
-            const int j = blk * kBKV + my_box * p.box;
-            at = 0;
-            if (!mine || blk >= w.u_hi || j + p.box <= w.key_lo || j >= w.key_hi) return (int)a.c.pages;
-            const int page = j / a.c.page_size;
-            at = j - page * a.c.page_size;
-            const int id = table[page];
-            if (id < 0 || id >= a.c.pages) {
-              atomicExch(a.status, (uint32_t)kStatusBadIndex);
-              return (int)a.c.pages;
-            }
-            return id;
-          };
-          int next_at;
-          int next_id = look_up(w.u_lo, next_at);
-          for (int j = w.u_lo; j < w.u_hi && ok; ++j) {
-            const int id = next_id, at = next_at;
-            next_id = look_up(j + 1, next_at);
-            for (int kv = 0; kv < 2; ++kv) {
-              const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
-              if constexpr (Q8) {
-                if (!wait_by_lane0(&raw_empty[s], ph ^ 1)) break;
-                if (lane == 0) mbar_expect_tx(&raw_full[s], C::kRawBytes);
-                __syncwarp();
-                if (mine) tma_load_4d(raw_s + s * C::kRawBytes + my_box * p.box * 128, map, &raw_full[s], 0, hk, at, id);
-                if (++s == R) s = 0, ph ^= 1;
-              } else {
-                uint64_t* full = kv ? v_full : k_full;
-                if (!wait_by_lane0(kv ? &v_empty[s] : &k_empty[s], ph ^ 1)) break;
-                if (lane == 0) mbar_expect_tx(&full[s], KB);
-                __syncwarp();
-                if (mine)
-                  tma_load_4d((kv ? v_s : k_s) + s * KB + my_col * KBOX + my_box * p.box * 128, map, &full[s], my_col * 64, hk,
-                              at, id);
-              }
-            }
-            if (!Q8 && ok && ++s == S) s = 0, ph ^= 1;
-          }
+          ok = load_blocks(w, 0, pos);
         }
         // the next item
         x += weight;
@@ -426,35 +431,33 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       if (!ok)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA's memory goes
     } else if (warp == 2) {
-      // ---------------- query tiles: a warp of its own, so that an item's first keys do not wait ----------------
-      // ---------------- until the last one's last scores have read the tile ----------------
-      if (lane == 0) {
-        uint32_t q_items[2] = {0, 0};  // live items so far, per tile
-        bool ok = true;
-        for (uint32_t n_it = 0; ok; ++n_it) {
-          const int slot = (int)(n_it & 1);
-          if (!mbar_wait(&item_full[slot], (n_it >> 1) & 1, a.status)) break;
-          const PagedWork w = item_ring[slot];
-          mbar_arrive(&item_empty[slot]);
-          if (!w.valid) break;
-          for (int i = 0; i < 2; ++i) {
-            if (i == 0 ? w.r0.hi <= w.r0.lo : w.r1.hi <= w.r1.lo) continue;
-            // the issuer's last QK of the tile's previous live item has read this Q tile
-            if (!mbar_wait(&q_empty[i], (q_items[i] & 1) ^ 1, a.status)) {
-              ok = false;
-              break;
-            }
-            ++q_items[i];
+      // ---------------- query tiles and values ----------------
+      uint32_t q_items[2] = {0, 0};  // live items so far, per tile
+      uint32_t pos = 0;
+      bool ok = true;
+      for (uint32_t n_it = 0; ok; ++n_it) {
+        const int slot = (int)(n_it & 1);
+        if (!wait_by_lane0(&item_full[slot], (n_it >> 1) & 1)) break;
+        const PagedWork w = item_ring[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[slot]);
+        if (!w.valid) break;
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (i == 0 ? w.r0.hi <= w.r0.lo : w.r1.hi <= w.r1.lo) continue;
+          // the issuer's last QK of the tile's previous live item has read this Q tile
+          ok = wait_by_lane0(&q_empty[i], (q_items[i] & 1) ^ 1);
+          ++q_items[i];
+          if (ok && lane == 0) {
             mbar_expect_tx(&q_full[i], (uint32_t)(p.tile_tokens * p.group * 128 * (D / 64)));
             for (int c = 0; c < D / 64; ++c)
               tma_load_4d(q_s + i * QB + c * (128 * 128), &tmap_q, &q_full[i], c * 64, w.hk * p.group,
                           w.t0 + i * p.tile_tokens, w.b);
           }
         }
-        if (!ok)
-          for (int i = 0; i < 64; ++i) __nanosleep(1000);
+        if (ok) ok = load_blocks(w, 1, pos);
       }
-      __syncwarp();
+      if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
     } else {
       // ---------------- MMA issuers: warp 1 drives tile 0, warp 3 tile 1 (attention_tc_p.cu) ----------------
       const int i = warp == 1 ? 0 : 1;
@@ -572,17 +575,17 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ---------------- widening: raw e4m3 blocks into the 16-bit rings ----------------
     if constexpr (Q8) {
-      const int tid = threadIdx.x - 384;
-      const int r = tid & 63, half = tid >> 6;  // a key of the block, half of its row
-      constexpr int kPieces = D / 32;           // 16-byte pieces of half a row
+      // two warps the keys, two the values: a thread a key's row
+      const int tid = threadIdx.x - 384, r = tid & 63, kv = tid >> 6;
+      constexpr int kPieces = D / 16;  // 16-byte pieces of a raw row
       const int page_size = a.c.page_size;
       const int pages_on = kBKV / page_size, slots_on = kBKV % page_size;  // from a block to the next
-      // where the pieces of my half row lie: 16-byte piece c of a 128-byte row r at (c ^ r) mod 8
-      const uint32_t src_at = (uint32_t)(r * 128 + (((half * kPieces) ^ (r & 7)) << 4));
-      const uint32_t dst_at = (uint32_t)(r * 128 + ((((half * kPieces * 2) & 7) ^ (r & 7)) << 4) + ((half * kPieces * 2) >> 3) * KBOX);
+      uint64_t* const full = kv ? v_full : k_full;
+      uint64_t* const empty = kv ? v_empty : k_empty;
+      // 16-byte piece c of a 128-byte row r lies at (c ^ r) mod 8
+      const uint32_t src0 = smem_u32(raw_s) + kv * C::kRawBytes + r * 128 + ((r & 7) << 4);
+      const uint32_t dst0 = smem_u32(kv ? v_s : k_s) + r * 128 + ((r & 7) << 4);
       uint32_t pos = 0;  // K/V blocks so far (ring position)
-      int rs = 0;
-      uint32_t rph = 0;
       bool ok = true;
       for (uint32_t n_it = 0; ok; ++n_it) {
         const int islot = (int)(n_it & 1);
@@ -592,89 +595,74 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         if (lane == 0) mbar_arrive(&item_empty[islot]);
         if (!w.valid) break;
         const int32_t* table = a.c.table + (int64_t)w.b * a.c.table_sb;
-        const uint8_t* ks_base = a.c.k_scale + (int64_t)w.hk * a.c.ks_sh;
-        const uint8_t* vs_base = a.c.v_scale + (int64_t)w.hk * a.c.vs_sh;
+        const uint8_t* scales = kv ? a.c.v_scale + (int64_t)w.hk * a.c.vs_sh : a.c.k_scale + (int64_t)w.hk * a.c.ks_sh;
+        const int64_t scales_sp = kv ? a.c.vs_sp : a.c.ks_sp;
         // my key's page and slot walk a block at a time; its page id is looked up two blocks
-        // ahead, its scale codes one
-        int page = (w.u_lo * kBKV + r) / page_size, slot = (w.u_lo * kBKV + r) - page * page_size;
-        auto id_of = [&](int key, int pg) -> int { return key >= w.key_lo && key < w.key_hi ? table[pg] : -1; };
-        auto codes_of = [&](int id, int sl, uint32_t& kc, uint32_t& vc) {
-          kc = vc = 0u;
-          if (id >= 0 && id < a.c.pages) {
-            kc = ks_base[id * a.c.ks_sp + sl];
-            vc = vs_base[id * a.c.vs_sp + sl];
-          }
-        };
+        // ahead, its scale code one
+        int key = w.u_lo * kBKV + r;
+        int page = key / page_size, slot = key - page * page_size;
+        auto id_of = [&](int k) -> int { return k >= w.key_lo && k < w.key_hi && k < w.u_hi * kBKV ? table[page] : -1; };
+        auto code_of = [&](int id) -> uint32_t { return id >= 0 && id < a.c.pages ? scales[id * scales_sp + slot] : 0u; };
         auto step = [&]() {
           page += pages_on, slot += slots_on;
           if (slot >= page_size) slot -= page_size, ++page;
         };
-        int key = w.u_lo * kBKV + r;
-        uint32_t kc, vc;
-        codes_of(id_of(key, page), slot, kc, vc);
+        uint32_t code = code_of(id_of(key));
         step();
-        int id_next = w.u_lo + 1 < w.u_hi ? id_of(key + kBKV, page) : -1;
-        // One copy of the code for K and V, the rare path rolled up: with both unrolled the
-        // roles' code no longer stays in the instruction cache and these warps, which run
-        // theirs once a block, wait for every line of it (1100 cycles for 180 instructions).
-        for (int j = w.u_lo; j < w.u_hi && ok; ++j, ++pos, key += kBKV) {
-          uint32_t kc_next, vc_next;
-          codes_of(id_next, slot, kc_next, vc_next);
+        int id_next = id_of(key + kBKV);
+        // The rare path rolled up: the roles' code has to stay in the instruction cache. (With
+        // both paths unrolled, for keys and for values, these warps waited for every line of
+        // theirs: 1100 cycles for 180 instructions.)
+        for (int j = w.u_lo; j < w.u_hi; ++j, ++pos, key += kBKV) {
+          const uint32_t code_next = code_of(id_next);
           step();
-          id_next = j + 2 < w.u_hi ? id_of(key + 2 * kBKV, page) : -1;
-          const int s = (int)(pos % S);
-          const uint32_t ph = (pos / S) & 1;
+          id_next = id_of(key + 2 * kBKV);
+          const int s = (int)(pos % S), st = (int)((pos & 1) << 1);
           const bool real = key >= w.key_lo && key < w.key_hi;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            if (!mbar_wait(&raw_full[rs], rph, a.status) || !mbar_wait((kv ? v_empty : k_empty) + s, ph ^ 1, a.status)) {
-              ok = false;
-              break;
-            }
-            const uint32_t src = smem_u32(raw_s) + rs * C::kRawBytes + src_at;
-            const uint32_t dst = smem_u32(kv ? v_s : k_s) + s * KB + dst_at;
-            const uint32_t code = kv ? vc : kc;
-            // a slot beside the item's keys becomes zeros, whatever it holds: every pattern is finite here
-            const uint32_t factor = widen_factor<T>(code), up = real ? factor : 0u;
-            if (!real || factor != 0u) {
-              uint4 in[kPieces];
-#pragma unroll
-              for (int i = 0; i < kPieces; ++i) in[i] = lds128(src ^ (uint32_t)(i << 4));
-#pragma unroll
-              for (int i = 0; i < kPieces; ++i) {
-                // piece i of 16 values: 32 bytes, the 16-byte pieces 2 i and 2 i + 1 behind dst's
-                const uint32_t to = (dst ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
-                sts128(to, widen_pair<T>(in[i].x, 0, up), widen_pair<T>(in[i].x, 1, up), widen_pair<T>(in[i].y, 0, up),
-                       widen_pair<T>(in[i].y, 1, up));
-                sts128(to ^ 16u, widen_pair<T>(in[i].z, 0, up), widen_pair<T>(in[i].z, 1, up), widen_pair<T>(in[i].w, 0, up),
-                       widen_pair<T>(in[i].w, 1, up));
-              }
-            } else {
-              // a scale beyond the type's normal numbers, or NaN: through f32
-              const float scale = scale_value(code);
-#pragma unroll 1
-              for (int i = 0; i < kPieces; ++i) {
-                const uint4 in = lds128(src ^ (uint32_t)(i << 4));
-                const uint32_t to = (dst ^ (uint32_t)(((2 * i) & 7) << 4)) + (uint32_t)(((2 * i) >> 3) * KBOX);
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                  const uint32_t wa = h ? in.z : in.x, wb = h ? in.w : in.y;
-                  const float2 x = from_e4m3x2(wa & 0xffffu), y = from_e4m3x2(wa >> 16);
-                  const float2 z = from_e4m3x2(wb & 0xffffu), u = from_e4m3x2(wb >> 16);
-                  sts128(to ^ (uint32_t)(h << 4), Elem<T>::pack(x.x * scale, x.y * scale), Elem<T>::pack(y.x * scale, y.y * scale),
-                         Elem<T>::pack(z.x * scale, z.y * scale), Elem<T>::pack(u.x * scale, u.y * scale));
-                }
-              }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive((kv ? v_full : k_full) + s);
-              mbar_arrive(&raw_empty[rs]);
-            }
-            if (++rs == R) rs = 0, rph ^= 1;
+          if (!mbar_wait(&raw_full[st | kv], (pos >> 1) & 1, a.status) || !mbar_wait(&empty[s], ((pos / S) & 1) ^ 1, a.status)) {
+            ok = false;
+            break;
           }
-          kc = kc_next, vc = vc_next;
+          const uint32_t src = src0 + st * C::kRawBytes, dst = dst0 + s * KB;
+          // a slot beside the item's keys becomes zeros, whatever it holds: every pattern is finite here
+          const uint32_t factor = widen_factor<T>(code), up = real ? factor : 0u;
+          if (!real || factor != 0u) {
+#pragma unroll 1
+            for (int h = 0; h < kPieces / 4; ++h) {
+              // four pieces of 16 values: a 64-column box of the 16-bit row
+              uint4 in[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) in[i] = lds128(src ^ (uint32_t)((4 * h + i) << 4));
+              const uint32_t to = dst + h * KBOX;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                sts128(to ^ (uint32_t)((2 * i) << 4), widen_pair<T>(in[i].x, 0, up), widen_pair<T>(in[i].x, 1, up),
+                       widen_pair<T>(in[i].y, 0, up), widen_pair<T>(in[i].y, 1, up));
+                sts128(to ^ (uint32_t)((2 * i + 1) << 4), widen_pair<T>(in[i].z, 0, up), widen_pair<T>(in[i].z, 1, up),
+                       widen_pair<T>(in[i].w, 0, up), widen_pair<T>(in[i].w, 1, up));
+              }
+            }
+          } else {
+            // a scale beyond the type's normal numbers, or NaN: through f32
+            const float scale = scale_value(code);
+#pragma unroll 1
+            for (int i = 0; i < 2 * kPieces; ++i) {
+              const uint4 in = lds128(src ^ (uint32_t)((i >> 1) << 4));
+              const uint32_t wa = i & 1 ? in.z : in.x, wb = i & 1 ? in.w : in.y;
+              const float2 x = from_e4m3x2(wa & 0xffffu), y = from_e4m3x2(wa >> 16);
+              const float2 z = from_e4m3x2(wb & 0xffffu), u = from_e4m3x2(wb >> 16);
+              sts128((dst + (i >> 3) * KBOX) ^ (uint32_t)((i & 7) << 4), Elem<T>::pack(x.x * scale, x.y * scale),
+                     Elem<T>::pack(y.x * scale, y.y * scale), Elem<T>::pack(z.x * scale, z.y * scale),
+                     Elem<T>::pack(u.x * scale, u.y * scale));
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&full[s]);
+            mbar_arrive(&raw_empty[st | kv]);
+          }
+          code = code_next;
         }
       }
     }
@@ -1056,7 +1044,7 @@ int run(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) {
   p.tile_tokens = 128 / p.group;
   p.box = page_box(a.c.page_size, kBKV);
   p.scale_log2 = a.scale * kLog2eF;
-  p.n_qt = (int)((a.t + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens));
+  p.page_size = divider((uint32_t)a.c.page_size);
   const int grid = grid_of(a);
   p.parts = (float*)a.workspace;
   p.heads_of_split = (int*)(p.parts + (int64_t)grid * 2 * kPartFloats<D>);
