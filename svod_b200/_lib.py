@@ -274,9 +274,9 @@ def fastops():
             if mod.torch != torch.__version__:
                 raise ImportError(f"{path} was built for torch {mod.torch}, this is {torch.__version__}")
             lib = load()
-            mod.init(*[C.cast(getattr(lib, f"svodb_{n}"), C.c_void_p).value for n in (
-                "linear", "attention", "attention_packed", "layer_norm", "rms_norm", "add_layer_norm", "add_rms_norm",
-                "cache_write", "cache_read", "attention_paged", "attention_paged_workspace_bytes")])
+            at = lambda *names: [C.cast(getattr(lib, f"svodb_{n}"), C.c_void_p).value for n in names]
+            mod.init(*at("linear", "attention", "attention_packed", "layer_norm", "rms_norm", "add_layer_norm", "add_rms_norm"))
+            mod.init_paged(*at("cache_write", "cache_read", "attention_paged", "attention_paged_workspace_bytes"))
             _fast = mod
         except ImportError as e:
             warnings.warn(f"ops take 15-30 us a call longer than need be: {e}; build with `python -m svod_b200.build`")

@@ -455,18 +455,22 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// init(address of svodb_linear, svodb_attention, svodb_attention_packed, svodb_layer_norm,
-// svodb_rms_norm, svodb_add_layer_norm, svodb_add_rms_norm, svodb_cache_write, svodb_cache_read,
-// svodb_attention_paged, svodb_attention_paged_workspace_bytes)
-PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr int kEntries = 11;
-  if (n != kEntries) {
-    PyErr_SetString(PyExc_TypeError, "eleven entry point addresses");
-    return nullptr;
+// The addresses in `args`, `n` of them; false with a TypeError otherwise.
+template <int N>
+bool addresses(PyObject* const* args, Py_ssize_t n, void* (&p)[N]) {
+  if (n != N) {
+    PyErr_Format(PyExc_TypeError, "%d entry point addresses", N);
+    return false;
   }
-  void* p[kEntries];
-  for (int i = 0; i < kEntries; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
-  if (PyErr_Occurred()) return nullptr;
+  for (int i = 0; i < N; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  return !PyErr_Occurred();
+}
+
+// init(address of svodb_linear, svodb_attention, svodb_attention_packed, svodb_layer_norm,
+// svodb_rms_norm, svodb_add_layer_norm, svodb_add_rms_norm)
+PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  void* p[7];
+  if (!addresses(args, n, p)) return nullptr;
   p_linear = (decltype(p_linear))p[0];
   p_attention = (decltype(p_attention))p[1];
   p_attention_packed = (decltype(p_attention_packed))p[2];
@@ -474,17 +478,25 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   p_rms_norm = (decltype(p_rms_norm))p[4];
   p_add_layer_norm = (decltype(p_add_layer_norm))p[5];
   p_add_rms_norm = (decltype(p_add_rms_norm))p[6];
-  p_cache_write = (decltype(p_cache_write))p[7];
-  p_cache_read = (decltype(p_cache_read))p[8];
-  p_attention_paged = (decltype(p_attention_paged))p[9];
-  p_attention_paged_workspace_bytes = (decltype(p_attention_paged_workspace_bytes))p[10];
 #define INTERN(n) s_##n = PyUnicode_InternFromString(#n);
   NAMES(INTERN)
   Py_RETURN_NONE;
 }
 
+// init_paged(address of svodb_cache_write, svodb_cache_read, svodb_attention_paged,
+// svodb_attention_paged_workspace_bytes); after `init`, which names the attributes
+PyObject* init_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  void* p[4];
+  if (!addresses(args, n, p)) return nullptr;
+  p_cache_write = (decltype(p_cache_write))p[0];
+  p_cache_read = (decltype(p_cache_read))p[1];
+  p_attention_paged = (decltype(p_attention_paged))p[2];
+  p_attention_paged_workspace_bytes = (decltype(p_attention_paged_workspace_bytes))p[3];
+  Py_RETURN_NONE;
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {FAST(init), FAST(linear), FAST(attention), FAST(attention_packed), FAST(norm), FAST(cache_write),
+PyMethodDef kMethods[] = {FAST(init), FAST(init_paged), FAST(linear), FAST(attention), FAST(attention_packed), FAST(norm), FAST(cache_write),
                           FAST(cache_read), FAST(attention_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastops", "compiled call path of svod_b200.ops", -1, kMethods};
 

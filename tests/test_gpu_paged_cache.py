@@ -550,3 +550,41 @@ def test_a_workspace_too_small_is_refused():
     o.workspace_bytes = need
     assert call() == L.OK
     ops.device_status()
+
+
+def test_other_python_threads_run_while_a_call_waits(tmp_path):
+    """The compiled call path lets the interpreter go around the paged cache's entry points
+    (each replaced by one that sleeps), and what torch cannot give is an exception."""
+    import ctypes as C
+    import subprocess
+    import threading
+    import time
+    (tmp_path / "nap.c").write_text("#include <unistd.h>\nint nap(void) { usleep(400000); return 0; }\nlong none(void) { return 0; }\n")
+    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "nap.c"), "-o", str(tmp_path / "nap2.so")], check=True)
+    lib = C.CDLL(str(tmp_path / "nap2.so"))
+    nap, none = (C.cast(f, C.c_void_p).value for f in (lib.nap, lib.none))
+    q, kv = torch.zeros(1, 2, 4, 64, dtype=BF16, device="cuda"), torch.zeros(1, 2, 2, 64, dtype=BF16, device="cuda")
+    cache, table, start = ops.PagedCache.empty(4, 16, 2, 64), i32([[0, 1]]), i32([0])
+    fast = L.fastops()
+    ticks, stop = [0], threading.Event()
+
+    def tick():
+        while not stop.wait(0.005):
+            ticks[0] += 1
+
+    other = threading.Thread(target=tick)
+    other.start()
+    try:
+        fast.init_paged(nap, nap, nap, none)
+        for call in (lambda: fast.cache_write(kv, kv, cache, table, start, None), lambda: fast.cache_read(cache, table, start, 5, BF16),
+                     lambda: fast.attention_paged(q, cache, table, start, None, ops.Attn(causal=True))):
+            before, t = ticks[0], time.monotonic()
+            assert call() is not None and time.monotonic() - t > 0.3
+            assert ticks[0] - before > 10
+    finally:
+        stop.set()
+        other.join()
+        L._fast = None
+        ops._call = None
+        L.fastops()  # bound to the library again
+    assert ops.attention_paged(q, cache, table, start).shape == q.shape and ops.chosen().startswith("attention_paged")
