@@ -68,7 +68,7 @@ def test_queries_behind_a_shared_instruction(quantized):
     said = rng.integers(0, V, 32)
     queries = [rng.integers(0, V, n) for n in (5, 40, 23)]
     first = m.extend(i32(said[None]), caches, i32([[7, 3]]), i32([0]))
-    assert np.abs(first[0].double().cpu() - embed64(p, said, quantized)).max() < TOL
+    assert (first[0].double().cpu() - embed64(p, said, quantized)).abs().max() < TOL
     table = i32([[7, 3, 0, 1, 2], [7, 3, 4, 5, 6], [7, 3, 8, 9, 10]])
     ids = np.zeros((3, 40), dtype=np.int64)
     for r, q in enumerate(queries):
@@ -76,13 +76,13 @@ def test_queries_behind_a_shared_instruction(quantized):
     got = m.extend(i32(ids), caches, table, i32([32] * 3), i32([len(q) for q in queries]))
     ops.device_status()
     for r, q in enumerate(queries):
-        assert np.abs(got[r].double().cpu() - embed64(p, np.concatenate([said, q]), quantized)).max() < TOL
+        assert (got[r].double().cpu() - embed64(p, np.concatenate([said, q]), quantized)).abs().max() < TOL
     tail = queries[0]
     for _ in range(3):
         new = rng.integers(0, V, 1)
         got = m.extend(i32(new[None]), caches, table[:1], i32([32 + len(tail)]))
         tail = np.concatenate([tail, new])
-        assert np.abs(got[0].double().cpu() - embed64(p, np.concatenate([said, tail]), quantized)).max() < TOL
+        assert (got[0].double().cpu() - embed64(p, np.concatenate([said, tail]), quantized)).abs().max() < TOL
     ops.device_status()
 
 
@@ -102,8 +102,8 @@ def test_a_document_by_chunks_is_the_document():
     ops.device_status()
     for r in (0, 1):
         want = embed64(p, ids[r, :lengths[r]], False)
-        assert np.abs(rows[r].double().cpu() - want).max() < TOL
-        assert np.abs(whole[r].double().cpu() - want).max() < TOL
+        assert (rows[r].double().cpu() - want).abs().max() < TOL
+        assert (whole[r].double().cpu() - want).abs().max() < TOL
 
 
 def test_a_captured_step_moves_on():
