@@ -49,8 +49,11 @@ namespace {
 using namespace fa_parts;
 using namespace paged;
 
-constexpr int kItemCost = 2;   // what an item costs beside its blocks, in blocks
-constexpr int kLeastShare = 4; // blocks (and items' costs) a CTA takes at least, where there are few
+constexpr int kItemCost = 2;  // what an item costs beside its blocks, in blocks
+// Blocks (and items' costs) a CTA takes at least, where there are few. 16 heads on 8 KV heads
+// with 2, 4 and 8: 150 tokens from the start on 15, 18 and 20 us; 2 x 64 tokens behind up to
+// 1000 held ones, where a share of 2 is a part of one block, 22, 20 and 21.
+constexpr int kLeastShare = 4;
 
 template <bool Q8, int D>
 struct PagedTcCfg {
