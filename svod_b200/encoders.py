@@ -253,7 +253,9 @@ class Qwen3Embedder:
         if len(caches) != c.num_hidden_layers:
             raise ValueError(f"extend: {len(caches)} caches for {c.num_hidden_layers} layers")
         B, T = ids.shape
-        at = (start[:, None] + torch.arange(T, dtype=torch.int32, device=start.device)).to(torch.int32)
+        start = start.to(torch.int32).contiguous()
+        last = torch.full_like(start, T) if lens is None else lens.to(torch.int32).contiguous()
+        at = start[:, None] + torch.arange(T, dtype=torch.int32, device=start.device)
         cos, sin = ops.rope_table(c.rope_theta, at, hd, c.dtype, ids.device)
         rope = (cos.view(B, T, 1, hd // 2), sin.view(B, T, 1, hd // 2))
         x = ops.embed(ids, p["embed"])
@@ -262,13 +264,12 @@ class Qwen3Embedder:
             qkv = ops.linear(xn, lp["qkv_w"], Linear(qkv=Qkv(H, Hkv, hd, lp["qn_w"], lp["kn_w"], c.rms_norm_eps, rope), w_static=True))
             # q, k and v are read in place from the packed projection
             heads = qkv.view(B, T, H + 2 * Hkv, hd)
-            ops.cache_write(heads[:, :, H:H + Hkv], heads[:, :, H + Hkv:], cache, table, start, lens)
-            a = ops.attention_paged(heads[:, :, :H], cache, table, start, lens, Attn(causal=True)).view(B, T, H * hd)
+            ops.cache_write(heads[:, :, H:H + Hkv], heads[:, :, H + Hkv:], cache, table, start, last)
+            a = ops.attention_paged(heads[:, :, :H], cache, table, start, last, Attn(causal=True)).view(B, T, H * hd)
             h = ops.linear(a, lp["o_w"], Linear(residual=x, w_static=True))
             hn = ops.rms_norm(h, lp["post_w"], c.rms_norm_eps)
             g = ops.linear(hn, lp["gu_w"], Linear(act=Act.SILU, gated=True, w_static=True))
             x = ops.linear(g, lp["down_w"], Linear(residual=h, w_static=True))
-        last = lens if lens is not None else torch.full((B,), T, dtype=torch.int32, device=ids.device)
         return ops.norm_pool(x, p["norm_w"], None, c.rms_norm_eps, layer=False, aux=last, mode=ops.POOL_LAST, out=out)
 
     def forward(self, ids, lengths, out=None, gather=None):

@@ -134,3 +134,18 @@ def test_a_captured_step_moves_on():
         assert torch.equal(out, want[t])
     ops.device_status()
     del g
+
+
+def test_counts_of_any_integer_type_and_stride():
+    """`start` and `lens` as columns of a wider table of 64-bit integers."""
+    p, rng = weights(), np.random.default_rng(11)
+    m = model(p)
+    ids = i32(rng.integers(0, V, (3, 20)))
+    table = i32([[0, 1], [2, 3], [4, 5]])
+    meta = torch.tensor([[0, 20], [0, 7], [0, 13]], device="cuda")
+    want = m.extend(ids, m.paged_caches(6, 16), table, i32([0, 0, 0]), i32([20, 7, 13]))
+    got = m.extend(ids, m.paged_caches(6, 16), table, meta[:, 0], meta[:, 1])
+    meta32 = meta.to(torch.int32)
+    narrow = m.extend(ids, m.paged_caches(6, 16), table, meta32[:, 0], meta32[:, 1])
+    ops.device_status()
+    assert torch.equal(got, want) and torch.equal(narrow, want)
