@@ -1084,8 +1084,11 @@ size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_
   if (paged_cache("attention_paged", cache, q->shape[0], q->dtype, a.c) != SVODB_OK) return 0;
   if (numel(q) == 0 || q->shape[3] != a.c.d || q->shape[2] % a.c.kv_heads != 0 || !is_half(q->dtype) || a.c.d > 128) return 0;
   a.batch = q->shape[0], a.t = q->shape[1], a.heads = (int)q->shape[2], a.dtype = q->dtype;
-  // the few-row kernel merges on the chip
-  return attention_paged_few_rows(a) ? 0 : attention_paged_tc_workspace(a);
+  a.q = a.o = q->data;
+  a.q_sb = a.o_sb = q->stride[0], a.q_st = a.o_st = q->stride[1], a.q_sh = a.o_sh = q->stride[2];
+  a.scale = 1.f;
+  // the few-row kernel merges on the chip, the exact one has nothing to merge
+  return attention_paged_few_rows(a) || !attention_paged_tc_covers(a) ? 0 : attention_paged_tc_workspace(a);
 }
 
 int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache, const svodb_tensor* start,

@@ -425,7 +425,7 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// attention_paged(q, cache, table, start, lens | None, opts): opts is an `Attn`
+// attention_paged(q, cache, table, start, lens | None, opts): opts is an `Attn`; (result, launches)
 PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 6 || p_attention_paged == nullptr) return none();
@@ -451,7 +451,8 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   void* st = stream();
   const svodb_tensor* lens = args[4] != Py_None ? &keep.lens : nullptr;
   if (unlocked([&] { return p_attention_paged(&q, &c, &keep.start, lens, &o, &y, st); }) != SVODB_OK) return none();
-  return with_lse(std::move(out), std::move(lse), want);
+  // the tiles' parts are merged by a kernel of their own
+  return Py_BuildValue("(Ni)", with_lse(std::move(out), std::move(lse), want), need > 0 ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }
 

@@ -544,9 +544,8 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, sta
     opts = opts or Attn(causal=True)
     r = (_call or _fast()).attention_paged(q, cache, table, start, lens, opts)
     if r is not None:
-        # over 64 query rows a KV head a second kernel merges the parts of the work
-        launches += 2 if q.shape[1] * q.shape[2] > 64 * cache.k.shape[2] else 1
-        return r
+        launches += r[1]
+        return r[0]
     dev = _one_device(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, start, lens)
     if q.dim() != 4:
         raise OpsError(L.ERR_SHAPE, f"attention_paged: q has shape {list(q.shape)}, expected [B, T, H, D]")

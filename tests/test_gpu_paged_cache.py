@@ -531,6 +531,45 @@ def test_which_kernel_ran():
     ops.device_status()
 
 
+def test_launches_are_counted():
+    """Two for the 128-row tiles and their merge, one for few rows, one for pages no tile takes."""
+    q = torch.randn(2, 40, 4, 64, device="cuda").to(BF16)
+    start, table = i32([0, 0]), i32([[0, 1, 2], [3, 4, 5]])
+    for page, tokens, want in ((16, 40, 2), (16, 9, 2), (16, 8, 1), (15, 40, 1)):
+        cache = ops.PagedCache.empty(12, page, 2, 64)
+        for lens in (None, torch.tensor([tokens, 3], device="cuda")):  # the compiled call path and the general one
+            before = ops.launches
+            ops.attention_paged(q[:, :tokens], cache, table, start, lens)
+            assert ops.launches - before == want
+    ops.device_status()
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+def test_two_calls_at_once(dtype, quantized):
+    """The tiles, few rows and a read over one cache on three streams side by side, in turns."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    mk = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dtype)
+    cache = ops.PagedCache.empty(200, 16, 2, 128, dtype, quantized)
+    table = torch.randperm(200, device="cuda", generator=g).to(torch.int32).view(2, 100)
+    ops.cache_write(mk(2, 1600, 2, 128), mk(2, 1600, 2, 128), cache, table, i32([0, 0]))
+    chunk, step = mk(2, 300, 8, 128), mk(2, 1, 8, 128)
+    calls = [lambda: ops.attention_paged(chunk, cache, table, i32([1300, 700])),
+             lambda: ops.attention_paged(step, cache, table, i32([1599, 800])),
+             lambda: ops.cache_read(cache, table, i32([1600, 900]), 1600, dtype)[1]]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], [], []]
+    for _ in range(20):
+        for f, s, out in zip(calls, streams, got):
+            with torch.cuda.stream(s):
+                out.append(f())
+    torch.cuda.synchronize()
+    for w, out in zip(want, got):
+        assert all(torch.equal(w, x) for x in out)
+    ops.device_status()
+
+
 def test_a_workspace_too_small_is_refused():
     import ctypes as C
     lib = L.load()
