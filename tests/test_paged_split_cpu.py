@@ -5,7 +5,7 @@ import random
 
 import pytest
 
-COST, LEAST, BLOCK = 2, 8, 64
+COST, LEAST, BLOCK = 2, 4, 64  # kItemCost, kLeastShare and the keys of a block
 
 
 def first_key(pos, window):
