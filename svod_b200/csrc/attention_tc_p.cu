@@ -519,12 +519,17 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
     const int other_turn = 1 + (1 - i) * 4 + quarter;
     uint32_t my_blocks = 0;   // blocks of this tile in all earlier items
     uint32_t tail_count = 0;  // tail commits of this tile in all earlier items
-    // A warp whose bounded wait ran out stops computing but keeps walking the
-    // queue and, for every later item, arrives on its partner's barrier at each
-    // turn the partner may take (`ok` stays false): the partner, which sees the
-    // same items, is never left waiting, and the warp that gave up never waits
-    // on a named barrier (they have no limit) again. Both leave when the queue
-    // ends or stops being fed.
+    // Turns on the MUFU unit (see the one-item kernel): tile 0 takes its n-th block that both
+    // tiles have, then tile 1 its own, and so on from item to item. A named barrier counts
+    // arrivals and does not know their turn: were a warp to arrive twice before its partner has
+    // waited once (tile 0 at its next item while tile 1 has yet to begin this one's last turn),
+    // the two arrivals would complete the barrier between them and the partner, whose wait has
+    // no limit, would stay. So each side waits for the other's last turn before every one of
+    // its own, the CTA's first excepted. A warp whose bounded wait ran out stops computing but
+    // walks all turns of this item and the later ones (`ok` stays false): its partner sees the
+    // same items, and no wait of either is left unanswered. Both leave when the queue ends or
+    // stops being fed.
+    uint32_t turns = 0;  // of all earlier items and this one
     bool ok = true;
     for (uint32_t n_it = 0;; ++n_it) {
       const int slot = (int)(n_it & 1);
@@ -543,12 +548,23 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       if (!w.valid) break;
+      const int n_paired = paired_blocks(w.r0, w.r1);
+      int turns_done = 0;  // of this item
+      auto take_turn = [&]() {
+        if (i == 1 || turns > 0) named_barrier(my_turn, 64);
+      };
+      auto pass_turn = [&]() {
+        named_barrier_arrive(other_turn, 64);
+        ++turns, ++turns_done;
+      };
+      auto walk_turns = [&]() {
+        while (turns_done < n_paired) {
+          take_turn();
+          pass_turn();
+        }
+      };
       if (!ok) {
-        const int pairs = paired_blocks(w.r0, w.r1);
-        // arrivals only: a partner still computing is released at each of its
-        // turns, and this warp never waits on a barrier without a limit again
-        for (int m = 0; m < pairs; ++m)
-          if (i == 0 || m + 1 < pairs) named_barrier_arrive(other_turn, 64);
+        walk_turns();
         continue;
       }
       const Range r = i == 0 ? w.r0 : w.r1;
@@ -587,18 +603,12 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
       float m_run = -INFINITY;
       float l_run = 0.f;
       const int nblk = r.hi - r.lo;
-      // The hand-over of the MUFU unit between the two tiles (see the one-item
-      // kernel): a named barrier per (tile, quarter); a warp that gave up still
-      // walks the rest of the item's sequence.
-      const int n_paired = paired_blocks(w.r0, w.r1);
-      int turns_done = 0;
       uint32_t sr[2][32];
       bool requested = false;
       for (int j = r.lo; j < r.hi && ok; ++j) {
         const int n = j - r.lo;
         const uint32_t N = my_blocks + (uint32_t)n;
         const int buf = (int)(N & 1);
-        turns_done = n;
         const uint32_t s_tmem = tmem_base + (uint32_t)((i * 2 + buf) * kBKV) + lane_addr;
         if (!requested) {
           if (!mbar_wait(&s_full[i * 2 + buf], (N >> 1) & 1, p.status)) {
@@ -707,8 +717,8 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
         }
         m_run = m_new;
         float m_use = m_run == -INFINITY ? 0.f : m_run;
-        if (n < n_paired && (i == 1 || n > 0)) {
-          named_barrier(my_turn, 64);
+        if (n < n_paired) {
+          take_turn();
           asm volatile("" : "+f"(m_use));
         }
         const float2 sl2_2 = make_float2(sl2, sl2), nm_2 = make_float2(-m_use, -m_use);
@@ -735,8 +745,7 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
           }
         }
         tmem_st32(s_tmem, pk);
-        if (n < n_paired && (i == 0 || n + 1 < n_paired)) named_barrier_arrive(other_turn, 64);
-        turns_done = n + 1;
+        if (n < n_paired) pass_turn();
         l_run += (la.x + la.y) + (lb.x + lb.y);
         requested = false;
         if (n + 1 < nblk) {
@@ -761,8 +770,7 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
         if (lane == 0) mbar_arrive(&p_full[i * 2 + buf]);
       }
       if (!ok) {
-        for (int m = turns_done; m < n_paired; ++m)
-          if (i == 0 || m + 1 < n_paired) named_barrier_arrive(other_turn, 64);
+        walk_turns();
         continue;
       }
       // ---- epilogue: O / l, or this split's unnormalised state ----

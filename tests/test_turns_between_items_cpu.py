@@ -1,0 +1,59 @@
+"""The turns that two query tiles take on the exponential unit, from item to item: the rules are
+read out of the persistent attention kernels' sources and walked on the host in every order that
+chance brings. A named barrier of 64 threads is complete with any two warps' arrivals, so a warp
+that arrives twice before its partner has waited leaves the partner, whose wait has no limit,
+without an arrival."""
+import random
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parent.parent / "svod_b200" / "csrc"
+KERNELS = ["attention_tc_p.cu", "attention_paged_tc.cu"]
+
+
+def rules(name, call):
+    """The conditions under which the kernel makes `call`, as Python; those of its loops that
+    only run when no more items come are left out."""
+    lines = (CSRC / name).read_text().splitlines()
+    found = []
+    for k, line in enumerate(lines):
+        if call not in line or "for (" in line or line.strip().startswith("//"):
+            continue
+        here = line if "if (" in line else lines[k - 1] if lines[k - 1].rstrip().endswith("{") and "if (" in lines[k - 1] else None
+        cond = re.search(r"if \((.*)\)", here[:here.rindex(")") + 1].split("named_barrier")[0]).group(1) if here else "True"
+        found.append(cond.replace("||", " or ").replace("&&", " and "))
+    return found
+
+
+@pytest.mark.parametrize("name", KERNELS)
+@pytest.mark.parametrize("seed", range(60))
+def test_no_warp_arrives_twice_before_its_partner_waits(name, seed):
+    g = random.Random(seed)
+    items = [g.choice([0, 1, 1, 2, 3, 7]) for _ in range(g.randint(2, 25))]
+    waits, passes = rules(name, "named_barrier(my_turn"), rules(name, "named_barrier_arrive(other_turn")
+    assert len(waits) == 1 and passes
+
+    def walk(i):
+        turns = 0
+        for n_paired in items:
+            for n in range(n_paired):
+                env = dict(i=i, n=n, m=n, n_paired=n_paired, pairs=n_paired, turns=turns)
+                if eval(waits[0], {}, env):
+                    yield "wait"
+                if all(eval(p, {}, env) for p in passes):
+                    yield "pass"
+                turns += 1
+
+    steps, at, arrived = [list(walk(0)), list(walk(1))], [0, 0], [0, 0]
+    while at[0] < len(steps[0]) or at[1] < len(steps[1]):
+        able = [i for i in (0, 1) if at[i] < len(steps[i]) and (steps[i][at[i]] == "pass" or arrived[i] > 0)]
+        assert able, "both wait"
+        i = g.choice(able)
+        if steps[i][at[i]] == "wait":
+            arrived[i] -= 1
+        else:
+            arrived[1 - i] += 1
+            assert arrived[1 - i] <= 1, "two arrivals before the partner has waited"
+        at[i] += 1
