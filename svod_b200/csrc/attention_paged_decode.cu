@@ -75,22 +75,30 @@ struct PagedDecCfg {
   static constexpr size_t kSmem = 1024 + (size_t)kRing + (kTail > kBox ? kTail : kBox);
   static constexpr int kTmemCols = 4 * kRows;
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "the CTAs of an SM fit its shared memory");
-  static_assert(kPBufs * kPBytes >= 4 * 1024, "the lengths of kSortedRows rows lie over the weights");
+  static_assert(kPBufs * kPBytes >= 2 * 1024, "the order of the rows is found over the weights");
   static_assert(kRows * D * 4 <= kRing, "the partial outputs are laid over the ring");
 };
 
-// Rows of a batch that a CTA puts in order, longest first, so that short rows fill the places
-// that long ones leave: their lengths fit the smallest weights' buffer. In the batch's order
-// and in this one, 8 KV heads: 64 rows x 64..4095 keys in bf16 120 and 88 us, 16 rows x
-// 8000..32767 in e4m3 137 and 116; 64 rows of 4095 163 and 165.
+// Rows of a batch that are taken in order, longest first, so that short rows fill the places
+// that long ones leave: a class of length a byte for each has to fit the smallest weights'
+// buffer beside the classes' counts. The order pays where the CTAs are a few times what the chip
+// holds at once; beyond that its places fill themselves, and every wave of CTAs pays the 1 to
+// 2.5 us of the order. In order | as they lie, 8 KV heads, us: 64..4095 keys in bf16, 64 rows
+// (1.7 times) 90 | 126, 112 rows (3.0) 156 | 174, 160 rows (4.3) 220 | 230; in e4m3 64 rows (1.2)
+// 57 | 68, 128 rows (2.3) 104 | 111, 192 rows (3.5) 155 | 155, 256 rows (4.6) 204 | 192;
+// 64..16000 keys, 80 rows in bf16 (2.2) 384 | 505, 120 in e4m3 (2.2) 300 | 378; 100..1000 keys in
+// bf16, 64 rows 37.5 | 41.1, 96 rows (2.6) 54.7 | 55.6, 128 rows (3.5) 71 | 67, 512 rows (14) 264 |
+// 220, 1024 rows (28) 543 | 428; in e4m3 128 rows 48 | 46; 64 rows of 4095 each 167 | 164.
+constexpr int kOrderedWaves = 3;
 constexpr int kSortedRows = 1024;
+constexpr int kClasses = 256;
 
 struct PagedDecParams {
   PagedAttnArgs a;
   int group, rows;  // rows = t * group query rows per KV head
   int box;          // keys of a box
   Divider page_size;
-  int longest_first;  // rows in the order of their visible keys, where the grid does not fit the chip at once
+  int longest_first;  // rows in the order of their visible keys (kOrderedWaves)
   float scale_log2;
 };
 
@@ -104,6 +112,79 @@ __device__ __forceinline__ int last_seen(const PagedAttnArgs& a, const Row& r, i
   if (a.causal && r.start + t + 1 < x) x = r.start + t + 1;
   if (a.has_window && r.start + t + a.win_right + 1 < x) x = r.start + t + a.win_right + 1;
   return (int)x;
+}
+
+// A row's class of length: its blocks of visible keys to three bits behind the first, so rows
+// of one class differ by an eighth at most. 0 for a row without keys, 200 at most.
+__device__ __forceinline__ int length_class(const PagedAttnArgs& a, const Row& r) {
+  if (r.n <= 0) return 0;
+  const int blocks = (last_seen(a, r, r.n - 1) + kKeys - 1) / kKeys - first_seen(a, r, 0) / kKeys;
+  return blocks <= 0 ? 0 : (int)(__float_as_uint((float)blocks) >> 20) - (127 << 3) + 1;
+}
+
+// The row that comes `at`-th when the batch is put in order, longest classes first and rows of
+// one class as they lie: the chip takes the long rows first, the short ones fill its last places.
+// Work in proportion to the batch: every row's class is counted, every warp finds from the counts
+// which class holds the place and from the classes which of its rows that is. `mem` (2 KB) is
+// free again when the call returns.
+__device__ __forceinline__ int longest_first_row(const PagedAttnArgs& a, int at, int64_t capacity, uint8_t* mem) {
+  const int tid = threadIdx.x, lane = tid & 31, batch = (int)a.batch;
+  int* counts = reinterpret_cast<int*>(mem);  // [kClasses]
+  uint8_t* classes = mem + kClasses * 4;      // [32 lanes][per]
+  const int per = (batch + 127) / 128 * 4;    // rows that a lane looks through
+  for (int k = tid; k < kClasses; k += kThreadsDec) counts[k] = 0;
+  __syncthreads();
+  for (int k = tid; k < 32 * per; k += kThreadsDec) {
+    int c = kClasses - 1;  // no row's
+    if (k < batch) {
+      c = length_class(a, row_of(a.start, a.lens, k, a.t, capacity));
+      atomicAdd(&counts[c], 1);
+    }
+    classes[k] = (uint8_t)c;
+  }
+  __syncthreads();
+  // lane l has the classes 255 - 8 l down to 248 - 8 l
+  int mine[8], sum = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) mine[e] = counts[kClasses - 1 - 8 * lane - e], sum += mine[e];
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  int left = at - (upto - sum), cls = 0;  // rows of my classes before the place
+  bool here = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (here) continue;
+    if (left >= 0 && left < mine[e]) here = true, cls = kClasses - 1 - 8 * lane - e;
+    else left -= mine[e];
+  }
+  const int who = __ffs((int)__ballot_sync(0xffffffffu, here)) - 1;
+  cls = __shfl_sync(0xffffffffu, cls, who), left = __shfl_sync(0xffffffffu, left, who);
+  // the row that has `left` of its class before it
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(classes + lane * per);
+  const uint32_t want = (uint32_t)cls * 0x01010101u;
+  int found = 0;
+  for (int w = 0; w < per / 4; ++w) found += __popc(__vcmpeq4(words[w], want)) >> 3;
+  upto = found;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  left -= upto - found;
+  here = left >= 0 && left < found;
+  int row = 0;
+  if (here) {
+    for (row = lane * per;; ++row)
+      if (classes[row] == cls && left-- == 0) break;
+  }
+  const int owner = __ffs((int)__ballot_sync(0xffffffffu, here)) - 1;
+  row = __shfl_sync(0xffffffffu, row, owner);
+  __syncthreads();  // before anything is written over the counts
+  return row;
 }
 
 __device__ __forceinline__ uint32_t to_e5m2x2(float lo, float hi) {
@@ -213,34 +294,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
 
   pdl_wait();
   const int64_t capacity = a.c.width * a.c.page_size;
-  if (p.longest_first) {
-    // This CTA's row is the b-th by visible keys: the chip takes the long ones first and the
-    // short ones fill its last places. (The weights' buffer holds the lengths meanwhile.)
-    int* keys = reinterpret_cast<int*>(p_s);
-    const int batch = (int)a.batch, padded = (batch + 3) & ~3;
-    for (int k = tid; k < padded; k += kThreadsDec) {
-      int n = -1;
-      if (k < batch) {
-        const Row r = row_of(a.start, a.lens, k, a.t, capacity);
-        n = r.n > 0 ? last_seen(a, r, r.n - 1) - first_seen(a, r, 0) : 0;
-      }
-      keys[k] = n;
-    }
-    __syncthreads();
-    for (int k = tid; k < batch; k += kThreadsDec) {
-      const int mine = keys[k];
-      int rank_of = 0;
-      for (int o = 0; o < padded; o += 4) {
-        const int4 n = *reinterpret_cast<const int4*>(keys + o);
-        rank_of += (n.x > mine || (n.x == mine && o < k)) + (n.y > mine || (n.y == mine && o + 1 < k)) +
-                   (n.z > mine || (n.z == mine && o + 2 < k)) + (n.w > mine || (n.w == mine && o + 3 < k));
-      }
-      if (rank_of == b) lim[0] = k;
-    }
-    __syncthreads();
-    b = lim[0];
-    __syncthreads();  // before anything is written over either
-  }
+  if (p.longest_first) b = longest_first_row(a, b, capacity, p_s);
   const Row r = row_of(a.start, a.lens, b, a.t, capacity);
   if (r.bad && tid == 0 && rank == 0 && hk == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
   auto first_of = [&](int t) { return first_seen(a, r, t); };
@@ -834,11 +888,13 @@ int run_rows(const PagedAttnArgs& a, cudaStream_t s, char* cfg, size_t cfg_len) 
   p.scale_log2 = a.scale * kLog2eF;
   const int64_t pairs = a.batch * a.c.kv_heads;
   const int csize = cluster_of(pairs, most_blocks(a), C::kPerSm);
-  p.longest_first = a.batch > 1 && a.batch <= kSortedRows && pairs * csize > (int64_t)sms() * C::kPerSm;
+  const int64_t room = (int64_t)sms() * C::kPerSm;
+  p.longest_first = a.batch > 1 && a.batch <= kSortedRows && pairs * csize > room && pairs * csize <= kOrderedWaves * room;
   if (launch_pdl(attention_paged_decode_kernel<T, Q8, D, W>, dim3((unsigned)(pairs * csize)), dim3(kThreadsDec), C::kSmem,
                  s, (unsigned)csize, a.batch * a.t, tk, tv, p) != cudaSuccess)
     return -1;
-  snprintf(cfg, cfg_len, "{rows:%d,bkv:%d,d:%d,box:%d,cluster:%d%s}", W, kKeys, a.c.d, p.box, csize, Q8 ? ",e4m3" : "");
+  snprintf(cfg, cfg_len, "{rows:%d,bkv:%d,d:%d,box:%d,cluster:%d%s%s}", W, kKeys, a.c.d, p.box, csize, Q8 ? ",e4m3" : "",
+           p.longest_first ? ",longest_first" : "");
   return 0;
 }
 
