@@ -286,7 +286,8 @@ int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, s
  * Query i of row b stands at position start[b] + i and sees keys 0 .. start[b] + lens[b] - 1
  * (lens = T without `lens`), under `causal` those up to its own position, under a window
  * those from window_left before to window_right behind it. Rows from lens[b] on and rows
- * without a key are zeros (lse -inf). Slots that hold no token of the sequence may hold anything; a
+ * without a key are zeros (lse -inf). A position whose table entry is no page counts as a key and
+ * a value of zeros, as reading it back gives, and `svodb_device_status` reports it. Slots that hold no token of the sequence may hold anything; a
  * NaN or an infinity in a token's own keys or values reaches every query that sees it and may
  * reach earlier queries of the same chunk (0 * NaN). Of `opts`: causal, has_window, has_scale, lse,
  * workspace; any other option is refused. `workspace`: svodb_attention_paged_workspace_bytes

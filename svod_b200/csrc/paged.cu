@@ -301,10 +301,10 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
     const int64_t at = j / a.c.page_size;
     const int slot = (int)(j - at * a.c.page_size);
     const int64_t page = page_of(a.c, b, at, a.status);
-    if (page < 0) continue;
+    const bool there = page >= 0;  // where no page is, a key and a value of zeros, as reading gives
     const int64_t fk = page * a.c.k_sp + slot * a.c.k_ss + hk * a.c.k_sh, fv = page * a.c.v_sp + slot * a.c.v_ss + hk * a.c.v_sh;
     float ks = 1.f, vs = 1.f;
-    if constexpr (Q8) {
+    if (Q8 && there) {
       ks = scale_value(a.c.k_scale[page * a.c.ks_sp + hk * a.c.ks_sh + slot]);
       vs = scale_value(a.c.v_scale[page * a.c.vs_sp + hk * a.c.vs_sh + slot]);
     }
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
     for (int e = 0; e < kPer; ++e) {
       const int c = lane + 32 * e;
       v[e] = 0.f;
-      if (c < d) {
+      if (c < d && there) {
         if constexpr (Q8) {
           s = fmaf(q[e], from_e4m3x2(((const uint8_t*)a.c.k)[fk + c]).x * ks, s);
           v[e] = from_e4m3x2(((const uint8_t*)a.c.v)[fv + c]).x * vs;

@@ -535,7 +535,9 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, sta
     and sees the `start[b] + lens[b]` keys of its sequence (T without `lens`), under
     `opts.causal` (the default without `opts`) those up to its own position, under
     `opts.window` those near it. One token a row is a decoding step, `start` zeros a prompt.
-    Rows from `lens[b]` on and rows that see no key are zeros. Other options are refused.
+    Rows from `lens[b]` on and rows that see no key are zeros. A position whose table entry is
+    no page counts as a key and a value of zeros, and `device_status()` raises. Other options
+    are refused.
 
     Slots that hold no token of the sequence, and pages that a window has left behind, may hold
     anything. A NaN or an infinity in a token's own keys or values reaches every query that sees
