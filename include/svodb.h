@@ -277,7 +277,8 @@ int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_
                       const svodb_tensor* start, const svodb_tensor* lens, void* stream);
 
 /* Reads rows back: k, v [B, L, kv_heads, D] in the stream type (the pages', or any float type
- * for e4m3 pages: value * scale, rounded once). Positions from lens[b] on are zeros; so are
+ * for e4m3 pages: value * scale, rounded once, the type's largest number for products beyond it:
+ * e4m3 may round a row's topmost values up past them). Positions from lens[b] on are zeros; so are
  * those without a page, which `svodb_device_status` reports. */
 int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, svodb_tensor* k, svodb_tensor* v,
                      void* stream);

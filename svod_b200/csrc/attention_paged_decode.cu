@@ -813,9 +813,13 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
         }
       }
       const float inv = l == 0.f ? 0.f : 1.0f / l;
+      // (65504 in f16 is 65536 as the pages hold it)
+      auto pair = [&](float x, float y) {
+        if constexpr (Q8 && std::is_same<T, __half>::value) return Elem<T>::pack(in_range<T>(x * inv), in_range<T>(y * inv));
+        else return Elem<T>::pack(x * inv, y * inv);
+      };
       stg128((T*)a.o + (int64_t)b * a.o_sb + tq * a.o_st + (int64_t)h * a.o_sh + d0,
-             make_uint4(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[2] * inv, acc[3] * inv),
-                        Elem<T>::pack(acc[4] * inv, acc[5] * inv), Elem<T>::pack(acc[6] * inv, acc[7] * inv)));
+             make_uint4(pair(acc[0], acc[1]), pair(acc[2], acc[3]), pair(acc[4], acc[5]), pair(acc[6], acc[7])));
       if (a.lse != nullptr && d0 == 0)
         a.lse[((int64_t)b * a.heads + h) * a.t + tq] = l == 0.f ? -INFINITY : kLn2F * (m + log2f(l));
     }

@@ -25,7 +25,8 @@
 //
 // 8-bit pages: a fourth warpgroup widens each block from a ring of raw e4m3 blocks into the
 // 16-bit rings, value * 2^e, exact in bf16 (a value is 4 bits) and rounded once in f16's
-// subnormals. A thread moves a key's row: the e4m3 fields are shifted to where the 16-bit
+// subnormals and at its top (`in_range`; weights rounded to f16 could carry an average of its
+// largest values past it, so such results are kept in range too). A thread moves a key's row: the e4m3 fields are shifted to where the 16-bit
 // type has them and one packed multiply puts exponent bias and scale right, 5 instructions a
 // pair of values (a conversion through f32 is 6, on slower pipes).
 //
@@ -654,9 +655,8 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
               const uint32_t wa = i & 1 ? in.z : in.x, wb = i & 1 ? in.w : in.y;
               const float2 x = from_e4m3x2(wa & 0xffffu), y = from_e4m3x2(wa >> 16);
               const float2 z = from_e4m3x2(wb & 0xffffu), u = from_e4m3x2(wb >> 16);
-              sts128((dst + (i >> 3) * KBOX) ^ (uint32_t)((i & 7) << 4), Elem<T>::pack(x.x * scale, x.y * scale),
-                     Elem<T>::pack(y.x * scale, y.y * scale), Elem<T>::pack(z.x * scale, z.y * scale),
-                     Elem<T>::pack(u.x * scale, u.y * scale));
+              auto pair = [&](float2 v) { return Elem<T>::pack(in_range<T>(v.x * scale), in_range<T>(v.y * scale)); };
+              sts128((dst + (i >> 3) * KBOX) ^ (uint32_t)((i & 7) << 4), pair(x), pair(y), pair(z), pair(u));
             }
           }
           fence_proxy_async_smem();
@@ -929,6 +929,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
           const unsigned long long mine = row_ok ? (unsigned long long)orow : 0ull;
           T* const row_even = (T*)__shfl_sync(0xffffffffu, mine, lane & 30);
           T* const row_odd = (T*)__shfl_sync(0xffffffffu, mine, lane | 1);
+          auto result = [](float x) { return Q8 && std::is_same<T, __half>::value ? in_range<T>(x) : x; };
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t orr[16], o[8];
@@ -936,7 +937,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              o[e] = l_run == 0.f ? 0u : Elem<T>::pack(__uint_as_float(orr[2 * e]) * inv, __uint_as_float(orr[2 * e + 1]) * inv);
+              o[e] = l_run == 0.f ? 0u : Elem<T>::pack(result(__uint_as_float(orr[2 * e]) * inv), result(__uint_as_float(orr[2 * e + 1]) * inv));
             // two lanes change halves and write 32 bytes of either row side by side, whole sectors
             const bool odd = (lane & 1) != 0;
 #pragma unroll
@@ -1032,13 +1033,15 @@ __global__ void __launch_bounds__(256) attention_paged_merge_kernel(const __grid
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const bool q8 = a.c.dtype == SVODB_E4M3;
+  auto result = [&](float x) { return std::is_same<T, __half>::value && q8 ? in_range<T>(x) : x; };
   T* o = (T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh + d0;
 #pragma unroll
   for (int v = 0; v < kMergeCols / 8; ++v) {
     if (d0 + v * 8 >= a.c.d) break;  // padded head dim
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack(acc[v * 8 + 2 * e] * inv, acc[v * 8 + 2 * e + 1] * inv);
+    for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack(result(acc[v * 8 + 2 * e] * inv), result(acc[v * 8 + 2 * e + 1] * inv));
     stg128(o + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
   }
   if (a.lse != nullptr && d0 == 0)

@@ -171,10 +171,17 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_any_kernel(const Ca
 
 // Eight e4m3 values times their scale, rounded to the stream type.
 template <typename T>
-__device__ __forceinline__ uint4 widen_e4m3(uint2 u, float scale) {
-  const float2 a = from_e4m3x2(u.x & 0xffffu), b = from_e4m3x2(u.x >> 16), c = from_e4m3x2(u.y & 0xffffu), d = from_e4m3x2(u.y >> 16);
-  return make_uint4(Elem<T>::pack(a.x * scale, a.y * scale), Elem<T>::pack(b.x * scale, b.y * scale),
-                    Elem<T>::pack(c.x * scale, c.y * scale), Elem<T>::pack(d.x * scale, d.y * scale));
+__device__ __forceinline__ uint4 widen_e4m3(uint2 u, uint32_t code) {
+  const float scale = scale_value(code);
+  float2 v[4] = {from_e4m3x2(u.x & 0xffffu), from_e4m3x2(u.x >> 16), from_e4m3x2(u.y & 0xffffu), from_e4m3x2(u.y >> 16)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i].x *= scale, v[i].y *= scale;
+  if (code >= kCodeOutOfRange<T>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i].x = in_range<T>(v[i].x), v[i].y = in_range<T>(v[i].y);
+  }
+  return make_uint4(Elem<T>::pack(v[0].x, v[0].y), Elem<T>::pack(v[1].x, v[1].y), Elem<T>::pack(v[2].x, v[2].y),
+                    Elem<T>::pack(v[3].x, v[3].y));
 }
 
 __device__ __forceinline__ uint2 ldg64(const void* p) {
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheRe
   for (int k = 0; k < N; ++k) {
     if (row0 + k * (kThreadsPaged / LPR) >= rows) continue;
     T* dst = out + token[k] * out_t + head[k] * out_h + sub * 8;
-    if constexpr (Q8) stg128(dst, widen_e4m3<T>(u[k], scale_value(code[k])));
+    if constexpr (Q8) stg128(dst, widen_e4m3<T>(u[k], code[k]));
     else stg128(dst, u[k]);
   }
 }
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_any_kernel(const Cac
   const void* base = is_v ? a.c.v : a.c.k;
   for (int e = lane; e < a.c.d; e += 32) {
     if (page < 0) dst[e] = Elem<T>::from_f(0.f);
-    else if constexpr (Q8) dst[e] = Elem<T>::from_f(from_e4m3x2(((const uint8_t*)base)[from + e]).x * scale);
+    else if constexpr (Q8) dst[e] = Elem<T>::from_f(in_range<T>(from_e4m3x2(((const uint8_t*)base)[from + e]).x * scale));
     else dst[e] = ((const T*)base)[from + e];
   }
 }
@@ -315,8 +322,8 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
       v[e] = 0.f;
       if (c < d && there) {
         if constexpr (Q8) {
-          s = fmaf(q[e], from_e4m3x2(((const uint8_t*)a.c.k)[fk + c]).x * ks, s);
-          v[e] = from_e4m3x2(((const uint8_t*)a.c.v)[fv + c]).x * vs;
+          s = fmaf(q[e], in_range<T>(from_e4m3x2(((const uint8_t*)a.c.k)[fk + c]).x * ks), s);
+          v[e] = in_range<T>(from_e4m3x2(((const uint8_t*)a.c.v)[fv + c]).x * vs);
         } else {
           s = fmaf(q[e], Elem<T>::to_f(((const T*)a.c.k)[fk + c]), s);
           v[e] = Elem<T>::to_f(((const T*)a.c.v)[fv + c]);

@@ -3,11 +3,16 @@
 // Pages `k`, `v` [pages, page_size, kv_heads, D] hold the stream type, or e4m3 beside one
 // power of two a token and head (`k_scale`, `v_scale` [pages, kv_heads, page_size], e8m0:
 // code c stands for 2^(c - 127), 255 for NaN). A power of two costs e4m3 nothing but its
-// smallest values, and multiplying by it rounds nothing: what attention computes with and
-// what is read back are the same numbers in every path.
+// smallest values, and multiplying by it rounds nothing where the stream type has the product:
+// there, what attention computes with and what is read back are the same numbers in every path.
+// f16 alone has products that it rounds (its subnormals) where keys and values are widened; the
+// few-row kernel takes them as they are. Products beyond a type's largest number: `in_range`.
 #pragma once
 
 #include <cuda_fp8.h>
+#include <float.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -58,6 +63,19 @@ __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
 __device__ __forceinline__ float2 from_e4m3x2(uint32_t u) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)u, __NV_E4M3);
   return __half22float2(__half2(h));
+}
+
+// A page's value in the stream type's range. e4m3 rounds the topmost values of a type past its
+// largest number (f16: 63488 and more to 256 * 2^8 = 65536), which then stands for them: a row
+// that was finite reads back finite, half a step off at most. NaN stays.
+template <typename T>
+constexpr float kLargest = std::is_same<T, __half>::value ? 65504.f : std::is_same<T, float>::value ? FLT_MAX : 0x1.fep127f;
+// The least scale code whose values (up to 448 * 2^(code - 127)) leave that range.
+template <typename T>
+constexpr uint32_t kCodeOutOfRange = std::is_same<T, __half>::value ? 135u : 247u;
+template <typename T>
+__device__ __forceinline__ float in_range(float x) {
+  return fabsf(x) > kLargest<T> ? copysignf(kLargest<T>, x) : x;
 }
 
 // n / d for 0 <= n < 2^31 without a division: (floor(n m / 2^32) + n) >> shift with

@@ -48,3 +48,50 @@ def test_an_entry_that_is_no_page_counts_as_zeros(dtype, quantized, page, tokens
     with pytest.raises(ops.OpsError, match="out of range"):
         ops.device_status()
     assert (k[0, 2 * page:3 * page] == 0).all() and (k[1, :page] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [64, 13])
+def test_the_top_of_a_type_reads_back_finite(dtype, d):
+    """Values that e4m3 rounds past their type's largest number read back as that number, rows
+    that are not finite as NaN."""
+    top = torch.finfo(dtype).max
+    rows = torch.tensor([1.0, 0.995, 0.96875, 0.9, -1.0, 0.5], dtype=torch.float64) * top
+    x = torch.cat([rows[:, None].expand(-1, d), torch.full((1, d), math.inf, dtype=torch.float64)]).to(dtype).view(1, 7, 1, d)
+    cache = ops.PagedCache.empty(1, 16, 1, d, dtype, quantized=True)
+    ops.cache_write(x.cuda(), -x.cuda(), cache, i32([[0]]), i32([3]))
+    k, v = ops.cache_read(cache, i32([[0]]), i32([10]), dtype=dtype)
+    ops.device_status()
+    for got, want in ((k, x), (v, -x)):
+        got = got[0, 3:10, 0].double().cpu()
+        assert torch.isnan(got[6]).all()
+        assert ((got[:6] - want[0, :6, 0].double()).abs() <= 2.0 ** -4 * want[0, :6, 0].double().abs()).all()
+        assert torch.isfinite(got[:6]).all()
+
+
+@pytest.mark.parametrize("tokens,page", [(1, 16), (8, 16), (90, 16), (3, 15)])
+def test_the_top_of_f16_is_finite_in_every_kernel(tokens, page):
+    """Keys and values of 65504 in 8-bit pages (256 * 2^8 there): by single tokens, by chunks and
+    in the exact kernel."""
+    held, d = [150, 37], 64
+    c = Case(tokens, 2, tokens, held, [tokens] * 2, 4, 2, d, page, F16, True)
+    for ks, vs in zip(c.keys, c.values):
+        ks[::5, :, 7] = 65504.0
+        ks[1::7, :, 7] = -64000.0
+        vs[::3] = 65504.0
+        vs[1::9] = -63500.0
+    c.q[..., 7] = 2.0 ** -14
+    c.put([0, 0], [h + tokens for h in held])
+    got = ops.attention_paged(c.q.cuda(), cache_of(c), c.table.cuda(), i32(held))
+    ops.device_status()
+    assert torch.isfinite(got.float()).all()
+    want, _, bound = c.attention()
+    # a key's 65536 taken as 65504 moves a score by 32 * 2^-14 / 8, a weight and their sum by as much
+    off = 2 * 32 * 2.0 ** -14 / 8 * 65536
+    assert ((got.double().cpu() - want).abs() <= bound + off).all()
+    one = torch.full_like(c.q[:, -1:], 0)
+    for vs in c.values:
+        vs[:] = 65504.0
+    c.put([0, 0], [h + tokens for h in held])
+    got = ops.attention_paged(torch.cat([c.q[:, :-1], one], 1).cuda(), cache_of(c), c.table.cuda(), i32(held))
+    assert (got.float() - 65504).abs().max() <= 64
