@@ -269,9 +269,9 @@ typedef struct svodb_paged_cache {
  * `lens`; the count is taken as within 0..T) become positions start[b] and on of sequence b.
  * With e4m3 pages a token's head row of values x gets the scale 2^e, e the least with
  * max|x| <= 448 * 2^e (2^-127 for zeros), and holds round(x / 2^e); a row that holds a NaN or an
- * infinity reads back as NaN. Slots that no token falls into stay as they are; two tokens
- * of one call that fall into the same slot leave either there. A row whose positions leave
- * the table and a token whose table entry is no page write nothing, and
+ * infinity reads back as NaN. Slots that no token falls into stay as they are; a slot that two
+ * tokens of one call fall into may hold parts of both, and belongs to neither. A row whose
+ * positions leave the table and a token whose table entry is no page write nothing, and
  * `svodb_device_status` says so. */
 int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_paged_cache* cache,
                       const svodb_tensor* start, const svodb_tensor* lens, void* stream);
@@ -287,13 +287,14 @@ int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, s
  * Query i of row b stands at position start[b] + i and sees keys 0 .. start[b] + lens[b] - 1
  * (lens = T without `lens`), under `causal` those up to its own position, under a window
  * those from window_left before to window_right behind it. Rows from lens[b] on and rows
- * without a key are zeros (lse -inf). A position whose table entry is no page counts as a key and
- * a value of zeros, as reading it back gives, and `svodb_device_status` reports it. Slots that hold no token of the sequence may hold anything; a
- * NaN or an infinity in a token's own keys or values reaches every query that sees it and may
- * reach earlier queries of the same chunk (0 * NaN). Of `opts`: causal, has_window, has_scale, lse,
- * workspace; any other option is refused. `workspace`: svodb_attention_paged_workspace_bytes
- * bytes, 16-byte aligned, for this call alone (two calls that may overlap on the GPU, or two
- * graphs that may be replayed at once, have one each). */
+ * without a key are zeros (lse -inf). A position whose table entry is no page counts as a key
+ * and a value of zeros, as reading it back gives, and `svodb_device_status` reports it. Slots
+ * that hold no token of the sequence may hold anything; a NaN or an infinity in a token's own
+ * keys or values reaches every query that sees it and may reach earlier queries of the same
+ * chunk (0 * NaN). Of `opts`: causal, has_window, has_scale, lse, workspace; any other option is
+ * refused. `workspace`: svodb_attention_paged_workspace_bytes bytes, 16-byte aligned, for this
+ * call alone (two calls that may overlap on the GPU, or two graphs that may be replayed at once,
+ * have one each). */
 size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_paged_cache* cache);
 int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache, const svodb_tensor* start,
                           const svodb_tensor* lens, const svodb_attn_opts* opts, svodb_tensor* o, void* stream);

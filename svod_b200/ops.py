@@ -482,9 +482,9 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, table: torc
     `lens[b]` tokens (all T without `lens`) become positions `start[b]` and on of sequence
     `b`. 8-bit pages: a token's head row gets the scale `2^e`, `e` the least with
     `max|x| <= 448 * 2^e`, and holds `round(x / 2^e)`; a row with a NaN or an infinity reads
-    back as NaN. Other slots stay as they are; two tokens of one call in the same slot leave
-    either. Rows that leave the table and entries that are no page write nothing, and
-    `device_status()` raises."""
+    back as NaN. Other slots stay as they are; a slot that two tokens of one call fall into
+    may hold parts of both (the values of one under the other's scale). Rows that leave the
+    table and entries that are no page write nothing, and `device_status()` raises."""
     global launches
     if (_call or _fast()).cache_write(k, v, cache, table, start, lens):
         launches += 1

@@ -95,3 +95,21 @@ def test_the_top_of_f16_is_finite_in_every_kernel(tokens, page):
     c.put([0, 0], [h + tokens for h in held])
     got = ops.attention_paged(torch.cat([c.q[:, :-1], one], 1).cuda(), cache_of(c), c.table.cuda(), i32(held))
     assert (got.float() - 65504).abs().max() <= 64
+
+
+@pytest.mark.parametrize("dtype,quantized", TYPES)
+def test_a_slot_written_twice_keeps_to_itself(dtype, quantized):
+    """Two rows of one call whose tables name the same page: what its slots hold is nobody's, and
+    every other slot is what the call says, to the bit."""
+    c = Case(23, 3, 20, [0, 0, 16], [20, 20, 20], 2, 2, 64, 16, dtype, quantized)
+    both = c.table[0, 0].item()
+    c.table[1, 0] = both
+    cache = cache_of(c)
+    k, v = (torch.stack([x[h:h + 20] for x, h in zip(xs, c.held)]).cuda() for xs in (c.keys, c.values))
+    ops.cache_write(k, v, cache, c.table.cuda(), i32(c.held))
+    ops.device_status()
+    c.put(c.held, [h + 20 for h in c.held])
+    rest = [p for p in range(c.pages) if p != both]
+    for got, want in ((cache.k, c.k), (cache.v, c.v), (cache.k_scale, c.ks), (cache.v_scale, c.vs)):
+        if want is not None:
+            assert torch.equal(raw(got.cpu())[rest], raw(want)[rest])
