@@ -396,7 +396,7 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// cache_read(cache, table, lens, length, like): (k, v) in the type of `like`, a tensor, or in the pages' own
+// cache_read(cache, table, lens, length, dtype): (k, v)
 PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 5 || p_cache_read == nullptr) return none();

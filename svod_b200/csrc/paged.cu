@@ -3,11 +3,12 @@
 // size (`attention_paged_exact`; the tensor-core kernels are in their own files).
 //
 // Write and read move every byte once and are bound by HBM, or by the chain
-// start -> table -> page of dependent loads where there is little to move. A lane owns 8
-// elements of a head row, 16 bytes on the 16-bit side and 8 on the 8-bit side, so that a
-// warp's accesses are whole lines (with 16 elements a lane every other 16 bytes: 113 us
-// against 103 for reading six rows of 3000 to 16384 e4m3 tokens, 117 against 100 in bf16,
-// which is 6.4 TB/s); a row's lanes find its largest value among themselves.
+// start -> table -> page of dependent loads where there is little to move. Reading, and writing
+// 16 bits, a lane owns 8 elements of a head row, 16 bytes on the 16-bit side and 8 on the 8-bit
+// side, so that a warp's accesses are whole lines (with 16 elements a lane every other 16 bytes:
+// 113 us against 103 for reading six rows of 3000 to 16384 e4m3 tokens, 117 against 100 in bf16,
+// which is 6.4 TB/s); writing 8 bits it owns 16 (kPerLane), and a row's lanes find its largest
+// value among themselves.
 #include <math.h>
 
 #include <initializer_list>

@@ -42,8 +42,8 @@ __device__ __forceinline__ Row row_of(const int32_t* start, const int32_t* lens,
 }
 
 // The e8m0 code of 2^e, the least power of two with amax <= 448 * 2^e: 448 = 1.75 * 2^8, so
-// the exponent of amax less 8, and one more where its significand is above 1.75. Zeros have
-// scale 1; a row that is not finite has the NaN code.
+// the exponent of amax less 8, and one more where its significand is above 1.75. Zeros, and
+// rows too small for the least code, have code 0 (2^-127); a row that is not finite has the NaN code.
 __device__ __forceinline__ uint32_t scale_code(float amax) {
   const uint32_t bits = __float_as_uint(amax);
   if (bits >= 0x7f800000u) return 255u;
