@@ -504,7 +504,11 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, lengt
     reaches; `dtype` is the pages' own, for 8-bit pages any float type (bf16 by default;
     value times scale, rounded once)."""
     global launches
-    if length is not None and dtype is not None:
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
+    if length is None and cache.k.dim() == 4 and table.dim() == 2:
+        length = table.shape[1] * cache.k.shape[1]
+    if length is not None:
         r = (_call or _fast()).cache_read(cache, table, lens, length, dtype)
         if r is not None:
             launches += 1
@@ -513,10 +517,6 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, lengt
     if cache.k.dim() != 4 or table.dim() != 2:
         raise OpsError(L.ERR_SHAPE, f"cache_read: cache k has shape {list(cache.k.shape)}, table {list(table.shape)}, expected "
                                     "[pages, page_size, kv_heads, D] and [B, width]")
-    if dtype is None:
-        dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
-    if length is None:
-        length = table.shape[1] * cache.k.shape[1]
     with torch.cuda.device(dev):
         keep: list = []
         lens = _i32(lens)

@@ -3,6 +3,8 @@ than the kernels keep."""
 import re
 from pathlib import Path
 
+import torch
+
 from svod_b200 import ops
 
 HEADER = (Path(__file__).resolve().parent.parent / "include" / "svodb.h").read_text()
@@ -16,3 +18,19 @@ def test_no_promise_about_a_slot_written_twice():
     """Values and scales of a slot are stores of several threads: neither token is left whole."""
     for text in (words(HEADER), words(ops.cache_write.__doc__)):
         assert "leave either" not in text and "may hold parts of both" in text
+
+
+def test_a_read_with_its_defaults_takes_the_compiled_call_path(monkeypatch):
+    asked = []
+
+    class Path:
+        def cache_read(self, cache, table, lens, length, dtype):
+            asked.append((length, dtype))
+            return "k", "v"
+
+    monkeypatch.setattr(ops, "_call", Path())
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for dtype, quantized, want in ((torch.float16, False, torch.float16), (torch.float16, True, torch.bfloat16)):
+        cache = ops.PagedCache.empty(4, 16, 2, 64, dtype, quantized, device="cpu")
+        assert ops.cache_read(cache, table, lens) == ("k", "v") and asked.pop() == (48, want)
+        assert ops.cache_read(cache, table, lens, 5, torch.float32) == ("k", "v") and asked.pop() == (5, torch.float32)
