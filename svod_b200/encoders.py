@@ -253,8 +253,8 @@ class Qwen3Embedder:
         if len(caches) != c.num_hidden_layers:
             raise ValueError(f"extend: {len(caches)} caches for {c.num_hidden_layers} layers")
         B, T = ids.shape
-        start = start.to(torch.int32).contiguous()
-        last = torch.full_like(start, T) if lens is None else lens.to(torch.int32).contiguous()
+        start = ops._i32(start)
+        last = torch.full_like(start, T) if lens is None else ops._i32(lens)
         at = start[:, None] + torch.arange(T, dtype=torch.int32, device=start.device)
         cos, sin = ops.rope_table(c.rope_theta, at, hd, c.dtype, ids.device)
         rope = (cos.view(B, T, 1, hd // 2), sin.view(B, T, 1, hd // 2))

@@ -449,14 +449,22 @@ class PagedCache:
         return PagedCache(mk(), mk(), scale(), scale())
 
 
+def _narrow(t: torch.Tensor) -> torch.Tensor:
+    """`t` as i32. What 32 bits do not hold becomes their largest or least number, which is as
+    far out of a cache's range; cut to its low bits it could name a page or a position."""
+    if t.dtype in (torch.int64, torch.uint32, torch.uint64):
+        t = t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(torch.int32)
+
+
 def _i32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else _narrow(t).contiguous()
 
 
 def _paged(cache: PagedCache, table: torch.Tensor, keep: list):
     c = L.PagedCache()
     if table.dtype != torch.int32 or (table.dim() == 2 and table.shape[1] > 1 and table.stride(1) != 1):
-        table = table.to(torch.int32).contiguous()
+        table = _narrow(table).contiguous()
     keep.append(table)
     for name, t in (("k", cache.k), ("v", cache.v), ("k_scale", cache.k_scale), ("v_scale", cache.v_scale), ("table", table)):
         if t is not None:

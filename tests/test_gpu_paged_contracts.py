@@ -113,3 +113,26 @@ def test_a_slot_written_twice_keeps_to_itself(dtype, quantized):
     for got, want in ((cache.k, c.k), (cache.v, c.v), (cache.k_scale, c.ks), (cache.v_scale, c.vs)):
         if want is not None:
             assert torch.equal(raw(got.cpu())[rest], raw(want)[rest])
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_integers_of_64_bits_that_name_nothing(tokens):
+    """A page, a position and a count beyond 32 bits: out of range, not their low halves."""
+    held = [30, 20]
+    c = Case(5, 2, tokens, held, [tokens] * 2, 4, 2, 64, 16, BF16, False)
+    c.put([0, 0], [h + tokens for h in held])
+    cache, q, table = cache_of(c), c.q.cuda(), c.table.cuda().long()
+    good = ops.attention_paged(q, cache, table, i32(held))
+    many = torch.tensor([2 ** 32 + 1, 2 ** 40], device="cuda")  # counts above the chunk's are the chunk's
+    assert torch.equal(ops.attention_paged(q, cache, table, i32(held), many), good)
+    ops.device_status()
+    start = torch.tensor([30, 2 ** 32 + 20], device="cuda")
+    got = ops.attention_paged(q, cache, table, start)
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    assert torch.equal(got[0], good[0]) and (got[1] == 0).all()
+    table[1, 0] += 2 ** 32
+    k, _ = ops.cache_read(cache, table, i32(held), 30)
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    assert (k[1, :16] == 0).all() and torch.equal(k[1, 16:20].cpu(), c.keys[1][16:20])

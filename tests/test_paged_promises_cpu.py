@@ -34,3 +34,15 @@ def test_a_read_with_its_defaults_takes_the_compiled_call_path(monkeypatch):
         cache = ops.PagedCache.empty(4, 16, 2, 64, dtype, quantized, device="cpu")
         assert ops.cache_read(cache, table, lens) == ("k", "v") and asked.pop() == (48, want)
         assert ops.cache_read(cache, table, lens, 5, torch.float32) == ("k", "v") and asked.pop() == (5, torch.float32)
+
+
+def test_integers_of_64_bits_are_not_cut():
+    """A position or a page of 2^32 + 5 is out of range; its low half would be 5."""
+    big = torch.tensor([2 ** 32 + 5, -2 ** 40, 7, 2 ** 31, -1])
+    want = [2 ** 31 - 1, -2 ** 31, 7, 2 ** 31 - 1, -1]
+    assert ops._i32(big).tolist() == want and ops._i32(big).dtype == torch.int32
+    assert ops._i32(big.repeat(2, 1).T[:, 0]).tolist() == want
+    for dtype in (torch.int8, torch.int16, torch.uint8, torch.int32):
+        assert ops._i32(torch.tensor([3, 0, 9], dtype=dtype)).tolist() == [3, 0, 9]
+    assert ops._i32(torch.tensor([2 ** 32 - 1], dtype=torch.uint32)).tolist() == [2 ** 31 - 1]
+    assert ops._i32(None) is None
