@@ -195,10 +195,10 @@ int rows_unsupported(const char* op) {
 
 }  // namespace
 
-// The status word bounded device waits report into: a module-scope device
-// variable (one instance per device that loads the library), so the op layer
-// allocates nothing.
-__device__ uint32_t g_status_word = 0;
+// The status word bounded device waits report into, and the one for indexes out of
+// range behind it: a module-scope device variable (one instance per device that
+// loads the library), so the op layer allocates nothing.
+__device__ uint32_t g_status_word[2] = {0, 0};
 
 namespace svodb {
 void set_last_error(const char* fmt, ...) {
@@ -277,19 +277,19 @@ int svodb_device_status(void* stream) {
   GUARD("device_status");
   uint32_t* w = device_status_word();
   if (w == nullptr) return fail(SVODB_ERR_LAUNCH, "device_status: no status word");
-  uint32_t host = 0;
-  cudaError_t e = cudaMemcpyAsync(&host, w, sizeof host, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+  uint32_t host[2] = {0, 0};
+  cudaError_t e = cudaMemcpyAsync(host, w, sizeof host, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
   if (e != cudaSuccess) {
     if (sticky(e)) g_poisoned = true;
     return fail(SVODB_ERR_LAUNCH, "device_status: %s", cudaGetErrorString(e));
   }
-  if (host != 0) {
+  if (host[0] != 0 || host[1] != 0) {
     cudaMemsetAsync(w, 0, sizeof host, (cudaStream_t)stream);
     cudaStreamSynchronize((cudaStream_t)stream);
-    if (host == kStatusBadIndex)
+    if (host[0] == 0)
       return fail(SVODB_ERR_SHAPE, "a device-side index was out of range (a cache row map or page table entry, or a position past the table)");
-    return fail(SVODB_ERR_TIMEOUT, "a bounded device wait ran out (code %u)", host);
+    return fail(SVODB_ERR_TIMEOUT, "a bounded device wait ran out (code %u)", host[0]);
   }
   return SVODB_OK;
 }

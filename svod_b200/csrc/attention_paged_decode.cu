@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
   const int64_t capacity = a.c.width * a.c.page_size;
   if (p.longest_first) b = longest_first_row(a, b, capacity, p_s);
   const Row r = row_of(a.start, a.lens, b, a.t, capacity);
-  if (r.bad && tid == 0 && rank == 0 && hk == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (r.bad && tid == 0 && rank == 0 && hk == 0) report_bad_index(a.status);
   auto first_of = [&](int t) { return first_seen(a, r, t); };
   auto last_of = [&](int t) { return last_seen(a, r, t); };
   const int lo = r.n > 0 ? first_of(0) : 0, hi = r.n > 0 ? last_of(r.n - 1) : 0;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
     slot_in_page = j - (int)(page * p.page_size.d);
     const int id = table[page];
     if (id < 0 || id >= a.c.pages) {
-      atomicExch(a.status, (uint32_t)kStatusBadIndex);
+      report_bad_index(a.status);
       return (int)a.c.pages;
     }
     return id;

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         at = j - (int)(page * p.page_size.d);
         const int id = table[page];
         if (id < 0 || id >= a.c.pages) {
-          atomicExch(a.status, (uint32_t)kStatusBadIndex);
+          report_bad_index(a.status);
           return (int)a.c.pages;
         }
         return id;
@@ -308,11 +308,11 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       // lane l keeps row l: a batch of up to 32 rows is read and weighed once
       const Row my_row = lane < batch ? row_at(lane) : Row{0, 0, false};
       const int64_t my_weight = weigh(my_row);
-      if (my_row.bad && blockIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+      if (my_row.bad && blockIdx.x == 0) report_bad_index(a.status);
       int64_t total = my_weight;
       for (int b = lane + 32; b < batch; b += 32) {
         const Row r = row_at(b);
-        if (r.bad && blockIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+        if (r.bad && blockIdx.x == 0) report_bad_index(a.status);
         total += weigh(r);
       }
 #pragma unroll

@@ -21,6 +21,10 @@ enum : uint32_t {
   kStatusBadIndex = 2,  // a device-side index (a cache row map or page table entry) was out of range
 };
 
+// A device-side index out of range, into the word behind the one that waits report into and look
+// at: rows beside a bad one, and calls before anybody reads the report, wait as long as ever.
+__device__ __forceinline__ void report_bad_index(uint32_t* status) { atomicExch(status + 1, (uint32_t)kStatusBadIndex); }
+
 // ---- dtype traits ----------------------------------------------------------
 template <typename T>
 struct Elem;

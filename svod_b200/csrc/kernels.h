@@ -361,7 +361,7 @@ bool gemm_tc2_preferred(const GemmArgs& a);
 // Sets the calling thread's `svodb_last_error` text (printf-style).
 void set_last_error(const char* fmt, ...);
 
-// The device status word bounded waits report into (one per device).
+// The device status word bounded waits report into (one per device); indexes out of range go into the next one.
 uint32_t* device_status_word();
 
 }  // namespace svodb

@@ -32,7 +32,7 @@ constexpr int kThreadsPaged = 256;
 __device__ __forceinline__ int64_t page_of(const PagedCache& c, int64_t b, int64_t page, uint32_t* status) {
   const int32_t id = c.table[b * c.table_sb + page];
   if (id < 0 || id >= c.pages) {
-    atomicExch(status, (uint32_t)kStatusBadIndex);
+    report_bad_index(status);
     return -1;
   }
   return id;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_kernel(const CacheW
   const bool is_v = blockIdx.y != 0;
   const int b = blockIdx.z, sub = threadIdx.x % LPR;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) report_bad_index(a.status);
   const uint32_t rows = (uint32_t)r.n * a.c.kv_heads;  // of this sequence's chunk
   const uint32_t row0 = blockIdx.x * (kThreadsPaged / LPR * N) + threadIdx.x / LPR;
   if (blockIdx.x * (kThreadsPaged / LPR * N) >= rows) return;  // the whole block: shuffles stay whole
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_any_kernel(const Ca
   const int h = (int)(row % a.c.kv_heads);
   const int64_t b = token / a.t, i = token % a.t;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (r.bad && i == 0 && lane == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (r.bad && i == 0 && lane == 0) report_bad_index(a.status);
   if (i >= r.n) return;
   const int64_t pos = r.start + i, at = pos / a.c.page_size;
   const int slot = (int)(pos - at * a.c.page_size);
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheRe
   const bool is_v = blockIdx.y != 0;
   const int b = blockIdx.z, sub = threadIdx.x % LPR;
   const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
-  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) report_bad_index(a.status);
   const uint32_t rows = (uint32_t)a.len * a.c.kv_heads;
   const uint32_t row0 = blockIdx.x * (kThreadsPaged / LPR * N) + threadIdx.x / LPR;
   const int64_t sp = is_v ? a.c.v_sp : a.c.k_sp, ss = is_v ? a.c.v_ss : a.c.k_ss, sh = is_v ? a.c.v_sh : a.c.k_sh;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_any_kernel(const Cac
   const int h = (int)(row % a.c.kv_heads);
   const int64_t b = token / a.len, pos = token % a.len;
   const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
-  if (r.bad && pos == 0 && lane == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (r.bad && pos == 0 && lane == 0) report_bad_index(a.status);
   int64_t page = -1, from = 0;
   float scale = 0.f;
   if (pos < r.n) {
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
   const int64_t i = item / a.heads % a.t, b = item / a.heads / a.t;
   const int hk = h / (a.heads / a.c.kv_heads), d = a.c.d;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (r.bad && i == 0 && h == 0 && threadIdx.x == 0) atomicExch(a.status, (uint32_t)kStatusBadIndex);
+  if (r.bad && i == 0 && h == 0 && threadIdx.x == 0) report_bad_index(a.status);
   const int64_t pos = r.start + i;
   int64_t lo = 0, hi = r.start + r.n;
   if (a.causal && pos + 1 < hi) hi = pos + 1;

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from svod_b200 import _lib as L
 from svod_b200 import ops
 from tests.paged_reference import Case
 
@@ -136,3 +137,37 @@ def test_integers_of_64_bits_that_name_nothing(tokens):
     with pytest.raises(ops.OpsError, match="out of range"):
         ops.device_status()
     assert (k[1, :16] == 0).all() and torch.equal(k[1, 16:20].cpu(), c.keys[1][16:20])
+
+
+def test_a_bad_row_does_not_shorten_the_waits_beside_it():
+    """A chunk of a million padded tokens, cleared while the row beside the bad one waits for its
+    first scores: the same result as behind a short padding."""
+    c = Case(41, 2, 200, [0, 3000], [200, 200], 16, 8, 128, 64, BF16, False)
+    c.put([0, 0], [200, 3200])
+    cache, table, start, lens = cache_of(c), c.table.cuda(), i32([-1, 3000]), i32([200, 200])
+    short = ops.attention_paged(c.q.cuda(), cache, table, start, lens)
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    c.new[0] = 0
+    want, _, bound = c.attention()
+    assert ((short.double().cpu() - want).abs() <= bound.clamp(min=2.0 ** -40)).all()
+    q = torch.empty(2, 1 << 20, 16, 128, dtype=BF16, device="cuda")
+    q[:, :200] = c.q.cuda()
+    for _ in range(2):  # the second call finds the first one's report unread
+        got = ops.attention_paged(q, cache, table, start, lens)
+        assert torch.equal(got[:, :200], short) and not got[:, 200:].any()
+        del got
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    ops.device_status()
+
+
+def test_a_timeout_is_told_before_a_bad_index():
+    cache = ops.PagedCache.empty(2, 16, 1, 64)
+    x = torch.zeros(1, 1, 1, 64, dtype=BF16, device="cuda")
+    ops.cache_write(x, x, cache, i32([[7]]), i32([0]))
+    lib = L.load()
+    assert lib.svodb_selftest_wait_timeout(2000, torch.cuda.current_stream().cuda_stream) == L.OK
+    with pytest.raises(ops.OpsError, match="wait ran out"):
+        ops.device_status()
+    ops.device_status()

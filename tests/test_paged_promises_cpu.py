@@ -46,3 +46,12 @@ def test_integers_of_64_bits_are_not_cut():
         assert ops._i32(torch.tensor([3, 0, 9], dtype=dtype)).tolist() == [3, 0, 9]
     assert ops._i32(torch.tensor([2 ** 32 - 1], dtype=torch.uint32)).tolist() == [2 ** 31 - 1]
     assert ops._i32(None) is None
+
+
+def test_an_index_out_of_range_is_no_reason_to_stop_waiting():
+    """Waits give up early when their own word is set; the reports of bad indexes go to another."""
+    csrc = Path(ops.__file__).resolve().parent / "csrc"
+    for f in sorted(csrc.glob("*.cu*")):
+        for line in f.read_text().splitlines():
+            if "kStatusBadIndex" in line and "atomicExch" in line:
+                assert "status + 1" in line, (f.name, line)
