@@ -1020,10 +1020,10 @@ int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_
     TRY(no_alias(OP, outs[i], {k, v, start, lens, cache->table}));
     for (int j = 0; j < i; ++j)
       // k and v of one buffer [.., 2, ..] interleave: their spans overlap, their slots do not
-      if (outs[j] != nullptr && outs[j]->data == outs[i]->data)
+      if (outs[j] != nullptr && outs[i]->data != nullptr && outs[j]->data == outs[i]->data)
         return fail(SVODB_ERR_ALIAS, "%s: keys, values and scales share storage", OP);
   }
-  if (B * T == 0 || a.c.pages == 0) {
+  if (B * T == 0) {
     chose_graph(OP, "shape");
     return SVODB_OK;
   }

@@ -171,3 +171,18 @@ def test_a_timeout_is_told_before_a_bad_index():
     with pytest.raises(ops.OpsError, match="wait ran out"):
         ops.device_status()
     ops.device_status()
+
+
+@pytest.mark.parametrize("dtype,quantized,d", [(*t, 64) for t in TYPES] + [(BF16, True, 13), (F32, False, 64)])
+def test_a_cache_without_pages_reports_what_it_cannot_take(dtype, quantized, d):
+    cache = ops.PagedCache.empty(0, 16, 2, d, dtype, quantized)
+    x, table = torch.ones(2, 3, 2, d, dtype=dtype, device="cuda"), i32([[0, -1], [5, 1]])
+    ops.cache_write(x, x, cache, table, i32([0, 7]), i32([0, 0]))
+    ops.device_status()
+    ops.cache_write(x, x, cache, table, i32([0, 7]))
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    k, v = ops.cache_read(cache, table, i32([3, 10]), 12, dtype)
+    with pytest.raises(ops.OpsError, match="out of range"):
+        ops.device_status()
+    assert not k.any() and not v.any()
