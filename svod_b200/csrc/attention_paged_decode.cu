@@ -415,7 +415,11 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
         for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const uint32_t code = scale_code(__uint_as_float(top));  // NaN and infinity: every score of the row is NaN
         const float inv = code == 255u ? 0.f : scale_inverse(code);
-        if (c == 0) fc[row] = p.scale_log2 * scale_value(code);
+        if (c == 0) {
+          // a factor too small for 32 bits is their least one: zero would make NaN of hidden scores
+          const float f = p.scale_log2 * scale_value(code);
+          fc[row] = f == 0.f ? __uint_as_float(1u) : f;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = code == 255u ? 0.f : f[e] * inv;
 #pragma unroll

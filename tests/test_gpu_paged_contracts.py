@@ -186,3 +186,19 @@ def test_a_cache_without_pages_reports_what_it_cannot_take(dtype, quantized, d):
     with pytest.raises(ops.OpsError, match="out of range"):
         ops.device_status()
     assert not k.any() and not v.any()
+
+
+@pytest.mark.parametrize("tokens,page", [(1, 16), (70, 16), (3, 15)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_zero_queries_under_a_scale_that_vanishes(dtype, tokens, page):
+    """8-bit pages, a query row of zeros and a tiny scale: the row's factor is below 32 bits, every
+    key it sees weighs the same and hidden keys weigh nothing."""
+    held = [130, 5]
+    c = Case(tokens + 1, 2, tokens, held, [tokens] * 2, 4, 2, 64, page, dtype, True)
+    c.q[0] = 0
+    c.q[1] = c.q[1] * 2.0 ** -14
+    c.put([0, 0], [h + tokens for h in held])
+    got = ops.attention_paged(c.q.cuda(), cache_of(c), c.table.cuda(), i32(held), None, ops.Attn(causal=True, scale=1e-30))
+    ops.device_status()
+    want, _, bound = c.attention(scale=1e-30)
+    assert ((got.double().cpu() - want).abs() <= bound).all()
