@@ -994,6 +994,26 @@ bool apart(const svodb_tensor* t) {
   return true;
 }
 
+// Whether two elements of views that are each `apart`, of one shape and one set of strides, lie
+// in one place: whether their distance (bytes) is a sum of whole steps that both shapes allow.
+// What the smaller dims reach is less than a step, so a dim has two counts of steps to try.
+bool meet(const svodb_tensor* t, int64_t distance, uint32_t dims_left) {
+  int at = -1;  // the largest stride left
+  for (int i = 0; i < t->rank; ++i)
+    if ((dims_left >> i & 1u) != 0 && t->shape[i] > 1 && (at < 0 || t->stride[i] > t->stride[at])) at = i;
+  const int64_t size = (int64_t)esize(t->dtype);
+  if (at < 0) return distance > -size && distance < size;
+  const int64_t step = t->stride[at] * size, below = distance / step - (distance % step < 0 ? 1 : 0);
+  for (int64_t c = below; c <= below + 1; ++c)
+    if (c > -t->shape[at] && c < t->shape[at] && meet(t, distance - c * step, dims_left & ~(1u << at))) return true;
+  return false;
+}
+bool same_strides(const svodb_tensor* a, const svodb_tensor* b) {
+  for (int i = 0; i < a->rank; ++i)
+    if (a->shape[i] > 1 && a->stride[i] != b->stride[i]) return false;
+  return true;
+}
+
 }  // namespace
 
 int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_paged_cache* cache,
@@ -1019,10 +1039,15 @@ int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_
     if (!apart(outs[i])) return fail(SVODB_ERR_GRAPH, "%s: a cache whose slots overlap", OP);
     TRY(no_alias(OP, outs[i], {k, v, start, lens, cache->table}));
     for (int j = 0; j < i; ++j)
-      // k and v of one buffer [.., 2, ..] interleave: their spans overlap, their slots do not
       if (outs[j] != nullptr && outs[i]->data != nullptr && outs[j]->data == outs[i]->data)
         return fail(SVODB_ERR_ALIAS, "%s: keys, values and scales share storage", OP);
   }
+  // k and v of one buffer [.., 2, ..] interleave: their spans overlap, the slots of a page do not
+  // (slots of other pages may: which pages are in use, the table says)
+  for (int i = 0; i < 4; i += 2)
+    if (outs[i] != nullptr && numel(outs[i]) > 0 && same_strides(outs[i], outs[i + 1]) &&
+        meet(outs[i], (const char*)outs[i + 1]->data - (const char*)outs[i]->data, ~1u))
+      return fail(SVODB_ERR_ALIAS, "%s: keys and values, or their scales, share slots", OP);
   if (B * T == 0) {
     chose_graph(OP, "shape");
     return SVODB_OK;

@@ -202,3 +202,45 @@ def test_zero_queries_under_a_scale_that_vanishes(dtype, tokens, page):
     ops.device_status()
     want, _, bound = c.attention(scale=1e-30)
     assert ((got.double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("layout", ["pages", "slots", "heads", "columns", "every other page"])
+def test_keys_beside_values_in_one_buffer(layout):
+    """Views whose spans overlap and whose slots do not are caches."""
+    P, S, H, D = 6, 16, 2, 64
+    kv = {"pages": lambda b: b.view(P, 2, S, H, D).unbind(1), "slots": lambda b: b.view(P, S, 2, H, D).unbind(2),
+          "heads": lambda b: b.view(P, S, H, 2, D).unbind(3), "columns": lambda b: b.view(P, S, H, 2 * D).split(D, -1),
+          "every other page": lambda b: (b.view(2 * P, S, H, D)[:-1], b.view(2 * P, S, H, D)[1:])}[layout]
+    cache = ops.PagedCache(*kv(torch.full((P * 2 * S * H * D,), math.nan, dtype=BF16, device="cuda")))
+    table = i32([[4, 0], [2, 2]])
+    x, y, q = (torch.randn(2, 20, h, D, device="cuda").to(BF16) for h in (H, H, 4))
+    ops.cache_write(x, y, cache, table, i32([0, 0]), i32([20, 9]))
+    k, v = ops.cache_read(cache, table, i32([20, 9]), 20)
+    assert torch.equal(k[0], x[0]) and torch.equal(v[0], y[0]) and torch.equal(k[1, :9], x[1, :9]) and torch.equal(v[1, :9], y[1, :9])
+    plain = ops.PagedCache(cache.k.contiguous(), cache.v.contiguous())
+    for n in (1, 20):
+        at = i32([20 - n, 0])
+        got = ops.attention_paged(q[:, :n], cache, table, at, i32([n, min(n, 9)]))
+        assert torch.isfinite(got.float()).all() and torch.equal(got, ops.attention_paged(q[:, :n], plain, table, at, i32([n, min(n, 9)])))
+    ops.device_status()
+
+
+@pytest.mark.parametrize("tokens", [1, 60])
+def test_pages_and_scales_in_records_of_one_buffer(tokens):
+    """8-bit keys, values and both scales of a page side by side, as a server's allocator lays them."""
+    held, page, h, d = [33, 70], 16, 2, 64
+    c = Case(71, 2, tokens, held, [tokens] * 2, 4, h, d, page, F16, True)
+    size = page * h * d
+    big = torch.full((c.pages, 2 * size + 2 * h * page + 64), 255, dtype=torch.uint8, device="cuda")
+    view = lambda lo, n, *s: big[:, lo:lo + n].unflatten(1, s)
+    k, v = (view(lo, size, page, h, d).view(torch.float8_e4m3fn) for lo in (0, size))
+    ks, vs = (view(2 * size + lo, h * page, h, page).view(torch.float8_e8m0fnu) for lo in (0, h * page))
+    cache = ops.PagedCache(k, v, ks, vs)
+    total = [n + tokens for n in held]
+    pad = lambda xs: torch.stack([torch.nn.functional.pad(x, (0, 0, 0, 0, 0, max(total) - x.shape[0])) for x in xs]).cuda()
+    ops.cache_write(pad(c.keys), pad(c.values), cache, c.table.cuda(), i32([0, 0]), i32(total))
+    got = ops.attention_paged(c.q.cuda(), cache, c.table.cuda(), i32(held))
+    ops.device_status()
+    want, _, bound = c.attention()
+    assert ((got.double().cpu() - want).abs() <= bound).all()
+    assert (big[:, 2 * size + 2 * h * page:] == 255).all()

@@ -3,9 +3,12 @@ than the kernels keep."""
 import re
 from pathlib import Path
 
+import pytest
 import torch
 
+from svod_b200 import _lib as L
 from svod_b200 import ops
+from tests.test_paged_cache_cpu import error, setup, write
 
 HEADER = (Path(__file__).resolve().parent.parent / "include" / "svodb.h").read_text()
 
@@ -55,3 +58,20 @@ def test_an_index_out_of_range_is_no_reason_to_stop_waiting():
         for line in f.read_text().splitlines():
             if "kStatusBadIndex" in line and "atomicExch" in line:
                 assert "status + 1" in line, (f.name, line)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("apart", [1, 8, 64, 128, 128 * 3 + 64, 128 * 15 + 127, -64, -128 * 7])
+def test_keys_and_values_that_share_slots_of_a_page_are_refused(q8, apart):
+    """Views of one buffer, some elements apart: [4, 16, 2, 64] pages whose slots are 128 elements."""
+    mk, t = setup(q8=q8)
+    kind, size = (L.E4M3, 1) if q8 else (L.BF16, 2)
+    t["v"] = mk(kind, 4, 16, 2, 64, data=t["k"].data + apart * size)
+    k, v, counts = mk(L.BF16, 2, 3, 2, 64), mk(L.BF16, 2, 3, 2, 64), mk(L.I32, 2)
+    assert write(t, k, v, counts, None) == L.ERR_ALIAS and "share" in error()
+
+
+def test_scales_that_share_slots_are_refused():
+    mk, t = setup(q8=True)
+    t["v_scale"] = mk(L.E8M0, 4, 2, 16, data=t["k_scale"].data + 5)
+    assert write(t, mk(L.BF16, 2, 3, 2, 64), mk(L.BF16, 2, 3, 2, 64), mk(L.I32, 2), None) == L.ERR_ALIAS, error()
