@@ -50,11 +50,7 @@ namespace {
 using namespace fa_parts;
 using namespace paged;
 
-constexpr int kItemCost = 2;  // what an item costs beside its blocks, in blocks
-// Blocks (and items' costs) a CTA takes at least, where there are few. 16 heads on 8 KV heads
-// with 2, 4 and 8: 150 tokens from the start on 15, 18 and 20 us; 2 x 64 tokens behind up to
-// 1000 held ones, where a share of 2 is a part of one block, 22, 20 and 21.
-constexpr int kLeastShare = 4;
+static_assert(kBlockKeys == kBKV, "the work is shared out in the blocks that the tiles take");
 
 template <bool Q8, int D>
 struct PagedTcCfg {
@@ -95,34 +91,6 @@ struct PagedWork {
   int u_lo, u_hi;
   int part;            // -1: the whole item, else the slot that the state goes to
 };
-
-// Keys [first, last) that the query token at position `pos` sees in a row of `end` keys; both
-// grow with the position.
-__device__ __forceinline__ int first_key(const PagedAttnArgs& a, int64_t pos) {
-  const int64_t x = a.has_window ? pos - a.win_left : 0;
-  return (int)(x > 0 ? x : 0);
-}
-__device__ __forceinline__ int last_key(const PagedAttnArgs& a, int64_t pos, int64_t end) {
-  int64_t x = end;
-  if (a.causal && pos + 1 < x) x = pos + 1;
-  if (a.has_window && pos + a.win_right + 1 < x) x = pos + a.win_right + 1;
-  return (int)x;
-}
-
-// The keys of item q of a row.
-__device__ __forceinline__ void item_keys(const PagedTcParams& p, const Row& r, int q, int& lo, int& hi) {
-  const int t = q * 2 * p.tile_tokens, t_last = min(t + 2 * p.tile_tokens, r.n) - 1;
-  lo = first_key(p.a, r.start + t);
-  hi = last_key(p.a, r.start + t_last, r.start + r.n);
-}
-__device__ __forceinline__ int item_blocks(const PagedTcParams& p, const Row& r, int q) {
-  int lo, hi;
-  item_keys(p, r, q, lo, hi);
-  return (hi + kBKV - 1) / kBKV - lo / kBKV;
-}
-__device__ __forceinline__ int live_items(const PagedTcParams& p, const Row& r) {
-  return (r.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-}
 
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
   uint4 v;
@@ -297,30 +265,22 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
     };
     if (warp == 0) {
       // ---------------- the CTA's run of the work, and its keys ----------------
-      // What a row's items weigh, for one KV head.
-      auto weigh = [&](const Row& r) -> int64_t {
-        int64_t w = 0;
-        for (int q = 0; q < live_items(p, r); ++q) w += item_blocks(p, r, q) + kItemCost;
-        return w;
-      };
       auto row_at = [&](int b) { return row_of(a.start, a.lens, b, a.t, capacity); };
       const int batch = (int)a.batch;
       // lane l keeps row l: a batch of up to 32 rows is read and weighed once
       const Row my_row = lane < batch ? row_at(lane) : Row{0, 0, false};
-      const int64_t my_weight = weigh(my_row);
+      const int64_t my_weight = row_weight(p, my_row);
       if (my_row.bad && blockIdx.x == 0) report_bad_index(a.status);
       int64_t total = my_weight;
       for (int b = lane + 32; b < batch; b += 32) {
         const Row r = row_at(b);
         if (r.bad && blockIdx.x == 0) report_bad_index(a.status);
-        total += weigh(r);
+        total += row_weight(p, r);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       total *= a.c.kv_heads;
-      int64_t quota = (total + gridDim.x - 1) / gridDim.x;
-      if (quota < kLeastShare) quota = kLeastShare;
-      const int64_t c0 = quota * blockIdx.x, c1 = c0 + quota < total ? c0 + quota : total;
+      const Run run = run_of(total, (int)blockIdx.x, (int)gridDim.x);
       // Row b for the whole warp.
       auto fetch_row = [&](int b) {
         if (b >= 32) return row_at(b);
@@ -330,97 +290,74 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         r.bad = false;
         return r;
       };
-      // Where the run begins: row b, KV head hk, item q, whose weight lies at [x, x + weight).
-      int b = 0, hk = 0, q = 0;
-      int64_t x = 0;
-      Row row{0, 0, false};
-      int64_t row_weight = 0;
-      if (c0 < c1) {
-        int64_t base = 0;
+      SplitItem split{0, 0, 0, 0, 0, 0};
+      uint32_t pos = 0;
+      bool ok = true;
+      uint32_t n_it = 0;
+      auto take = [&](const Row& row, const Share& sh) {
+        PagedWork w;
+        w.valid = 1, w.b = sh.b, w.hk = sh.hk, w.t0 = sh.q * 2 * p.tile_tokens, w.n_live = row.n, w.start = (int)row.start;
+        item_keys(p, row, sh.q, w.key_lo, w.key_hi);
+        const int blk_lo = w.key_lo / kBKV;
+        w.part = sh.part;
+        if (w.part == 1) split = SplitItem{1, sh.b, sh.hk, w.t0, row.n, sh.last_cta};
+        auto range = [&](int t) {
+          Range r{0, 0};
+          if (t >= row.n) return r;
+          const int t_last = min(t + p.tile_tokens, row.n) - 1;
+          const int lo = first_key(a, row.start + t) / kBKV;
+          const int hi = (last_key(a, row.start + t_last, row.start + row.n) + kBKV - 1) / kBKV;
+          const int y = max(lo, blk_lo + sh.from), z = min(hi, blk_lo + sh.to);
+          if (z > y) r.lo = y, r.hi = z;
+          return r;
+        };
+        w.r0 = range(w.t0);
+        w.r1 = range(w.t0 + p.tile_tokens);
+        const bool live0 = w.r0.hi > w.r0.lo, live1 = w.r1.hi > w.r1.lo;
+        w.u_lo = w.u_hi = 0;
+        if (live0 && live1) {
+          w.u_lo = w.r0.lo < w.r1.lo ? w.r0.lo : w.r1.lo;
+          w.u_hi = w.r0.hi > w.r1.hi ? w.r0.hi : w.r1.hi;
+        } else if (live0) {
+          w.u_lo = w.r0.lo, w.u_hi = w.r0.hi;
+        } else if (live1) {
+          w.u_lo = w.r1.lo, w.u_hi = w.r1.hi;
+        }
+        const int slot = (int)(n_it & 1);
+        ok = wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1);
+        if (!ok) return false;
+        if (lane == 0) {
+          item_ring[slot] = w;
+          __threadfence_block();
+          mbar_arrive(&item_full[slot]);
+        }
+        ++n_it;
+        ok = load_blocks(w, 0, pos);
+        return ok;
+      };
+      if (run.c0 < run.c1) {
+        // the row in which the run begins; its work begins at x
+        int b = 0;
+        int64_t x = 0, weight = 1, base = 0;
         for (int b0 = 0; b0 < batch; b0 += 32) {
-          const int64_t w = (b0 == 0 ? my_weight : b0 + lane < batch ? weigh(row_at(b0 + lane)) : 0) * a.c.kv_heads;
+          const int64_t w = (b0 == 0 ? my_weight : b0 + lane < batch ? row_weight(p, row_at(b0 + lane)) : 0) * a.c.kv_heads;
           int64_t upto = w;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += y;
           }
-          const uint32_t past = __ballot_sync(0xffffffffu, base + upto > c0);
+          const uint32_t past = __ballot_sync(0xffffffffu, base + upto > run.c0);
           if (past != 0u) {
             const int l = __ffs((int)past) - 1;
             b = b0 + l;
-            row_weight = __shfl_sync(0xffffffffu, w, l) / a.c.kv_heads;
+            weight = __shfl_sync(0xffffffffu, w, l) / a.c.kv_heads;
             x = base + __shfl_sync(0xffffffffu, upto - w, l);
             break;
           }
           base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        row = fetch_row(b);
-        hk = (int)((c0 - x) / row_weight);
-        x += hk * row_weight;
-        for (int64_t w = item_blocks(p, row, 0) + kItemCost; x + w <= c0; w = item_blocks(p, row, q) + kItemCost) x += w, ++q;
-      }
-      SplitItem split{0, 0, 0, 0, 0, 0};
-      uint32_t pos = 0;
-      bool ok = true;
-      uint32_t n_it = 0;
-      // (a CTA whose run would begin behind the last item has none)
-      while (c0 < c1 && x < c1 && ok) {
-        PagedWork w;
-        w.valid = 1, w.b = b, w.hk = hk, w.t0 = q * 2 * p.tile_tokens, w.n_live = row.n, w.start = (int)row.start;
-        item_keys(p, row, q, w.key_lo, w.key_hi);
-        const int blk_lo = w.key_lo / kBKV, blk_n = (w.key_hi + kBKV - 1) / kBKV - blk_lo;
-        const int64_t weight = blk_n + kItemCost;
-        // this run's part of the item's blocks: its first kItemCost units stand for the fixed cost
-        const int64_t u0 = (c0 > x ? c0 - x : 0) - kItemCost, u1 = (c1 < x + weight ? c1 - x : weight) - kItemCost;
-        const int from = u0 > 0 ? (int)u0 : 0, to = u1 > 0 ? (int)u1 : 0;
-        if (to > from) {
-          w.part = from == 0 && to == blk_n ? -1 : from == 0 ? 1 : 0;
-          if (w.part == 1) split = SplitItem{1, b, hk, w.t0, row.n, (int)((x + weight - 1) / quota)};
-          auto range = [&](int t) {
-            Range r{0, 0};
-            if (t >= row.n) return r;
-            const int t_last = min(t + p.tile_tokens, row.n) - 1;
-            const int lo = first_key(a, row.start + t) / kBKV;
-            const int hi = (last_key(a, row.start + t_last, row.start + row.n) + kBKV - 1) / kBKV;
-            const int y = max(lo, blk_lo + from), z = min(hi, blk_lo + to);
-            if (z > y) r.lo = y, r.hi = z;
-            return r;
-          };
-          w.r0 = range(w.t0);
-          w.r1 = range(w.t0 + p.tile_tokens);
-          const bool live0 = w.r0.hi > w.r0.lo, live1 = w.r1.hi > w.r1.lo;
-          w.u_lo = w.u_hi = 0;
-          if (live0 && live1) {
-            w.u_lo = w.r0.lo < w.r1.lo ? w.r0.lo : w.r1.lo;
-            w.u_hi = w.r0.hi > w.r1.hi ? w.r0.hi : w.r1.hi;
-          } else if (live0) {
-            w.u_lo = w.r0.lo, w.u_hi = w.r0.hi;
-          } else if (live1) {
-            w.u_lo = w.r1.lo, w.u_hi = w.r1.hi;
-          }
-          const int slot = (int)(n_it & 1);
-          ok = wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1);
-          if (!ok) break;
-          if (lane == 0) {
-            item_ring[slot] = w;
-            __threadfence_block();
-            mbar_arrive(&item_full[slot]);
-          }
-          ++n_it;
-          ok = load_blocks(w, 0, pos);
-        }
-        // the next item
-        x += weight;
-        if (++q == live_items(p, row)) {
-          q = 0;
-          if (++hk == a.c.kv_heads) {
-            hk = 0;
-            do row = ++b < batch ? fetch_row(b) : Row{0, 0, false};
-            while (b < batch && row.n == 0);
-            if (b >= batch) break;
-          }
-        }
+        walk_run(p, run, batch, a.c.kv_heads, b, x, weight, fetch_row, take);
       }
       if (lane == 0) {
         int* h = p.heads_of_split + (int64_t)blockIdx.x * kSplitInts;

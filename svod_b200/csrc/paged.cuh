@@ -16,17 +16,10 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "paged_split.cuh"
 
 namespace svodb {
 namespace paged {
-
-// What a row of the batch holds: its first `n` chunk tokens are real and stand at positions
-// `start` and on, the last key at start + n - 1.
-struct Row {
-  int64_t start;
-  int n;
-  bool bad;  // a start below zero or keys past the table: the row is taken as empty and the status word says so
-};
 
 __device__ __forceinline__ Row row_of(const int32_t* start, const int32_t* lens, int64_t b, int64_t t, int64_t capacity) {
   Row r;
