@@ -974,6 +974,11 @@ int chunk_rows(const char* OP, const char* name, const svodb_tensor* t, int64_t 
   return SVODB_OK;
 }
 
+uint32_t* bad_index_word() {
+  uint32_t* w = device_status_word();
+  return w == nullptr ? nullptr : w + kBadIndexWord;
+}
+
 // No two elements of a written tensor in one place, by strides that leave no room for it.
 bool apart(const svodb_tensor* t) {
   int64_t reach[SVODB_MAX_RANK], step[SVODB_MAX_RANK];
@@ -1059,7 +1064,7 @@ int svodb_cache_write(const svodb_tensor* k, const svodb_tensor* v, const svodb_
   a.batch = B, a.t = T, a.dtype = k->dtype;
   a.start = (const int32_t*)start->data;
   a.lens = lens != nullptr ? (const int32_t*)lens->data : nullptr;
-  a.status = device_status_word();
+  a.bad_index = bad_index_word();
   const int vec = launch_cache_write(a, (cudaStream_t)stream);
   if (vec) chose_kernel(OP, "cache_write", a.c.dtype == SVODB_E4M3 ? "{e4m3}" : "{copy}");
   else chose_graph(OP, "shape");
@@ -1095,7 +1100,7 @@ int svodb_cache_read(const svodb_paged_cache* cache, const svodb_tensor* lens, s
   a.v_sb = v->stride[0], a.v_st = v->stride[1], a.v_sh = v->stride[2];
   a.batch = B, a.len = T, a.dtype = k->dtype;
   a.lens = (const int32_t*)lens->data;
-  a.status = device_status_word();
+  a.bad_index = bad_index_word();
   const int vec = launch_cache_read(a, (cudaStream_t)stream);
   if (vec) chose_kernel(OP, "cache_read", a.c.dtype == SVODB_E4M3 ? "{e4m3}" : "{copy}");
   else chose_graph(OP, "shape");
@@ -1176,6 +1181,7 @@ int svodb_attention_paged(const svodb_tensor* q, const svodb_paged_cache* cache,
   a.lens = lens != nullptr ? (const int32_t*)lens->data : nullptr;
   a.lse = opts->lse ? (float*)opts->lse->data : nullptr;
   a.status = device_status_word();
+  a.bad_index = bad_index_word();
   char cfg[128];
   if (config_lookup("attention|exact") == 0 && attention_paged_decode_covers(a)) {
     const int rc = launch_attention_paged_decode(a, (cudaStream_t)stream, cfg, sizeof cfg);

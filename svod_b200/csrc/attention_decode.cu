@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreadsDec, (DecCfg<D, NQ>::kPerSm))
   }
   if (bad_row) {  // an entry outside the cache: nothing is read, zeros, and the status word says so
     kv_row = 0, len64 = 0, seen = 0;
-    if (tid == 0 && rank == 0) report_bad_index(p.status);
+    if (tid == 0 && rank == 0) report_bad_index(p.status + kBadIndexWord);
   }
   const int len = (int)len64;
   const int cached = (len + kKeys - 1) / kKeys;

@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreadsF, D == 64 ? 2 : 1) attention_f32_kern
   const bool bad_row = kv_row < 0 || kv_row >= a.kv_rows;
   if (bad_row) {  // an entry outside the cache: nothing is read, the lane sees no key, the status word says so
     kv_row = 0;
-    if (tid == 0 && a.status != nullptr) report_bad_index(a.status);
+    if (tid == 0 && a.status != nullptr) report_bad_index(a.status + kBadIndexWord);
   }
   const float* q = (const float*)a.q + b * a.q_sb + h * a.q_sh;
   const float* k = (const float*)a.k + kv_row * a.k_sb + hk * a.k_sh;

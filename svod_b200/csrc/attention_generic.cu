@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(256) attention_generic_kernel(const AttnArgs a
   const bool bad_row = kv_row < 0 || kv_row >= a.kv_rows;
   if (bad_row) {
     kv_row = 0;
-    if (tid == 0 && a.status != nullptr) report_bad_index(a.status);
+    if (tid == 0 && a.status != nullptr) report_bad_index(a.status + kBadIndexWord);
   }
   const T* k = (const T*)a.k + kv_row * a.k_sb + hk * a.k_sh;
   const T* v = (const T*)a.v + kv_row * a.v_sb + hk * a.v_sh;

@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
   const int64_t capacity = a.c.width * a.c.page_size;
   if (p.longest_first) b = longest_first_row(a, b, capacity, p_s);
   const Row r = row_of(a.start, a.lens, b, a.t, capacity);
-  if (r.bad && tid == 0 && rank == 0 && hk == 0) report_bad_index(a.status);
+  if (r.bad && tid == 0 && rank == 0 && hk == 0) report_bad_index(a.bad_index);
   auto first_of = [&](int t) { return first_seen(a, r, t); };
   auto last_of = [&](int t) { return last_seen(a, r, t); };
   const int lo = r.n > 0 ? first_of(0) : 0, hi = r.n > 0 ? last_of(r.n - 1) : 0;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
     slot_in_page = j - (int)(page * p.page_size.d);
     const int id = table[page];
     if (id < 0 || id >= a.c.pages) {
-      report_bad_index(a.status);
+      report_bad_index(a.bad_index);
       return (int)a.c.pages;
     }
     return id;
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(kThreadsDec, (PagedDecCfg<T, Q8, D>::kPerSm))
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       // (65504 in f16 is 65536 as the pages hold it)
       auto pair = [&](float x, float y) {
-        if constexpr (Q8 && std::is_same<T, __half>::value) return Elem<T>::pack(in_range<T>(x * inv), in_range<T>(y * inv));
+        if constexpr (Q8 && std::is_same<T, __half>::value) return pack_in_range<T>(x * inv, y * inv);
         else return Elem<T>::pack(x * inv, y * inv);
       };
       stg128((T*)a.o + (int64_t)b * a.o_sb + tq * a.o_st + (int64_t)h * a.o_sh + d0,

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         at = j - (int)(page * p.page_size.d);
         const int id = table[page];
         if (id < 0 || id >= a.c.pages) {
-          report_bad_index(a.status);
+          report_bad_index(a.bad_index);
           return (int)a.c.pages;
         }
         return id;
@@ -270,11 +270,11 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
       // lane l keeps row l: a batch of up to 32 rows is read and weighed once
       const Row my_row = lane < batch ? row_at(lane) : Row{0, 0, false};
       const int64_t my_weight = row_weight(p, my_row);
-      if (my_row.bad && blockIdx.x == 0) report_bad_index(a.status);
+      if (my_row.bad && blockIdx.x == 0) report_bad_index(a.bad_index);
       int64_t total = my_weight;
       for (int b = lane + 32; b < batch; b += 32) {
         const Row r = row_at(b);
-        if (r.bad && blockIdx.x == 0) report_bad_index(a.status);
+        if (r.bad && blockIdx.x == 0) report_bad_index(a.bad_index);
         total += row_weight(p, r);
       }
 #pragma unroll
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
               const uint32_t wa = i & 1 ? in.z : in.x, wb = i & 1 ? in.w : in.y;
               const float2 x = from_e4m3x2(wa & 0xffffu), y = from_e4m3x2(wa >> 16);
               const float2 z = from_e4m3x2(wb & 0xffffu), u = from_e4m3x2(wb >> 16);
-              auto pair = [&](float2 v) { return Elem<T>::pack(in_range<T>(v.x * scale), in_range<T>(v.y * scale)); };
+              auto pair = [&](float2 v) { return pack_in_range<T>(v.x * scale, v.y * scale); };
               sts128((dst + (i >> 3) * KBOX) ^ (uint32_t)((i & 7) << 4), pair(x), pair(y), pair(z), pair(u));
             }
           }
@@ -866,7 +866,10 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
           const unsigned long long mine = row_ok ? (unsigned long long)orow : 0ull;
           T* const row_even = (T*)__shfl_sync(0xffffffffu, mine, lane & 30);
           T* const row_odd = (T*)__shfl_sync(0xffffffffu, mine, lane | 1);
-          auto result = [](float x) { return Q8 && std::is_same<T, __half>::value ? in_range<T>(x) : x; };
+          auto pair = [](float x, float y) {
+            if constexpr (Q8 && std::is_same<T, __half>::value) return pack_in_range<T>(x, y);
+            else return Elem<T>::pack(x, y);
+          };
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t orr[16], o[8];
@@ -874,7 +877,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              o[e] = l_run == 0.f ? 0u : Elem<T>::pack(result(__uint_as_float(orr[2 * e]) * inv), result(__uint_as_float(orr[2 * e + 1]) * inv));
+              o[e] = l_run == 0.f ? 0u : pair(__uint_as_float(orr[2 * e]) * inv, __uint_as_float(orr[2 * e + 1]) * inv);
             // two lanes change halves and write 32 bytes of either row side by side, whole sectors
             const bool odd = (lane & 1) != 0;
 #pragma unroll
@@ -971,14 +974,14 @@ __global__ void __launch_bounds__(256) attention_paged_merge_kernel(const __grid
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   const bool q8 = a.c.dtype == SVODB_E4M3;
-  auto result = [&](float x) { return std::is_same<T, __half>::value && q8 ? in_range<T>(x) : x; };
+  auto pair = [&](float x, float y) { return std::is_same<T, __half>::value && q8 ? pack_in_range<T>(x, y) : Elem<T>::pack(x, y); };
   T* o = (T*)a.o + (int64_t)b * a.o_sb + (int64_t)t_row * a.o_st + (int64_t)head * a.o_sh + d0;
 #pragma unroll
   for (int v = 0; v < kMergeCols / 8; ++v) {
     if (d0 + v * 8 >= a.c.d) break;  // padded head dim
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack(result(acc[v * 8 + 2 * e] * inv), result(acc[v * 8 + 2 * e + 1] * inv));
+    for (int e = 0; e < 4; ++e) w[e] = pair(acc[v * 8 + 2 * e] * inv, acc[v * 8 + 2 * e + 1] * inv);
     stg128(o + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
   }
   if (a.lse != nullptr && d0 == 0)

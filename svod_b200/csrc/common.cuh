@@ -23,7 +23,8 @@ enum : uint32_t {
 
 // A device-side index out of range, into the word behind the one that waits report into and look
 // at: rows beside a bad one, and calls before anybody reads the report, wait as long as ever.
-__device__ __forceinline__ void report_bad_index(uint32_t* status) { atomicExch(status + 1, (uint32_t)kStatusBadIndex); }
+constexpr int kBadIndexWord = 1;
+__device__ __forceinline__ void report_bad_index(uint32_t* word) { atomicExch(word, (uint32_t)kStatusBadIndex); }
 
 // ---- dtype traits ----------------------------------------------------------
 template <typename T>

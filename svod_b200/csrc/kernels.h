@@ -245,7 +245,7 @@ struct CacheWriteArgs {
   int dtype;
   const int32_t* start;
   const int32_t* lens;  // nullable
-  uint32_t* status;
+  uint32_t* bad_index;  // the word that says a table entry or a position was out of range
 };
 // Returns 1 when the vector kernel ran, 0 when the one for every width and alignment did.
 int launch_cache_write(const CacheWriteArgs& a, cudaStream_t s);
@@ -257,7 +257,7 @@ struct CacheReadArgs {
   int64_t batch, len;
   int dtype;
   const int32_t* lens;
-  uint32_t* status;
+  uint32_t* bad_index;  // the word that says a table entry or a position was out of range
 };
 int launch_cache_read(const CacheReadArgs& a, cudaStream_t s);
 struct PagedAttnArgs {
@@ -276,6 +276,7 @@ struct PagedAttnArgs {
   const int32_t* lens;  // nullable
   float* lse;           // [B, H, T], nullable
   uint32_t* status;
+  uint32_t* bad_index;
   void* workspace;      // what the kernel that takes the call wants of it
 };
 // Every float type, head width up to 256, page size and alignment.

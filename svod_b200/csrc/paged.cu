@@ -29,10 +29,10 @@ using namespace paged;
 constexpr int kThreadsPaged = 256;
 
 // The slot of position `pos` of row b: {page, slot}; page < 0 when the table's entry is none.
-__device__ __forceinline__ int64_t page_of(const PagedCache& c, int64_t b, int64_t page, uint32_t* status) {
+__device__ __forceinline__ int64_t page_of(const PagedCache& c, int64_t b, int64_t page, uint32_t* bad_index) {
   const int32_t id = c.table[b * c.table_sb + page];
   if (id < 0 || id >= c.pages) {
-    report_bad_index(status);
+    report_bad_index(bad_index);
     return -1;
   }
   return id;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_kernel(const CacheW
   const bool is_v = blockIdx.y != 0;
   const int b = blockIdx.z, sub = threadIdx.x % LPR;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) report_bad_index(a.status);
+  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) report_bad_index(a.bad_index);
   const uint32_t rows = (uint32_t)r.n * a.c.kv_heads;  // of this sequence's chunk
   const uint32_t row0 = blockIdx.x * (kThreadsPaged / LPR * N) + threadIdx.x / LPR;
   if (blockIdx.x * (kThreadsPaged / LPR * N) >= rows) return;  // the whole block: shuffles stay whole
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_kernel(const CacheW
       for (int e = 0; e < E / 8; ++e) u[k][e] = ldg128(src + i * src_t + head[k] * src_h + sub * E + e * 8);
       const uint32_t pos = (uint32_t)r.start + i, at = page_size.div(pos);
       slot[k] = pos - at * page_size.d;
-      page[k] = page_of(a.c, b, at, a.status);
+      page[k] = page_of(a.c, b, at, a.bad_index);
     }
   }
 #pragma unroll
@@ -143,11 +143,11 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_any_kernel(const Ca
   const int h = (int)(row % a.c.kv_heads);
   const int64_t b = token / a.t, i = token % a.t;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (r.bad && i == 0 && lane == 0) report_bad_index(a.status);
+  if (r.bad && i == 0 && lane == 0) report_bad_index(a.bad_index);
   if (i >= r.n) return;
   const int64_t pos = r.start + i, at = pos / a.c.page_size;
   const int slot = (int)(pos - at * a.c.page_size);
-  const int64_t page = page_of(a.c, b, at, a.status);
+  const int64_t page = page_of(a.c, b, at, a.bad_index);
   if (page < 0) return;
   const T* src = is_v ? (const T*)a.v + b * a.v_sb + i * a.v_st + h * a.v_sh : (const T*)a.k + b * a.k_sb + i * a.k_st + h * a.k_sh;
   const int64_t to = is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh;
@@ -170,19 +170,12 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_write_any_kernel(const Ca
   }
 }
 
-// Eight e4m3 values times their scale, rounded to the stream type.
+// Eight e4m3 values times their scale, rounded to the stream type and kept in its range.
 template <typename T>
-__device__ __forceinline__ uint4 widen_e4m3(uint2 u, uint32_t code) {
-  const float scale = scale_value(code);
-  float2 v[4] = {from_e4m3x2(u.x & 0xffffu), from_e4m3x2(u.x >> 16), from_e4m3x2(u.y & 0xffffu), from_e4m3x2(u.y >> 16)};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i].x *= scale, v[i].y *= scale;
-  if (code >= kCodeOutOfRange<T>) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i].x = in_range<T>(v[i].x), v[i].y = in_range<T>(v[i].y);
-  }
-  return make_uint4(Elem<T>::pack(v[0].x, v[0].y), Elem<T>::pack(v[1].x, v[1].y), Elem<T>::pack(v[2].x, v[2].y),
-                    Elem<T>::pack(v[3].x, v[3].y));
+__device__ __forceinline__ uint4 widen_e4m3(uint2 u, float scale) {
+  const float2 a = from_e4m3x2(u.x & 0xffffu), b = from_e4m3x2(u.x >> 16), c = from_e4m3x2(u.y & 0xffffu), d = from_e4m3x2(u.y >> 16);
+  return make_uint4(pack_in_range<T>(a.x * scale, a.y * scale), pack_in_range<T>(b.x * scale, b.y * scale),
+                    pack_in_range<T>(c.x * scale, c.y * scale), pack_in_range<T>(d.x * scale, d.y * scale));
 }
 
 __device__ __forceinline__ uint2 ldg64(const void* p) {
@@ -200,7 +193,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheRe
   const bool is_v = blockIdx.y != 0;
   const int b = blockIdx.z, sub = threadIdx.x % LPR;
   const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
-  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) report_bad_index(a.status);
+  if (r.bad && blockIdx.x == 0 && threadIdx.x == 0) report_bad_index(a.bad_index);
   const uint32_t rows = (uint32_t)a.len * a.c.kv_heads;
   const uint32_t row0 = blockIdx.x * (kThreadsPaged / LPR * N) + threadIdx.x / LPR;
   const int64_t sp = is_v ? a.c.v_sp : a.c.k_sp, ss = is_v ? a.c.v_ss : a.c.k_ss, sh = is_v ? a.c.v_sh : a.c.k_sh;
@@ -217,7 +210,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheRe
     u[k] = {};
     if (row < rows && token[k] < (uint32_t)r.n) {
       const uint32_t at = page_size.div(token[k]), slot = token[k] - at * page_size.d;
-      const int64_t page = page_of(a.c, b, at, a.status);
+      const int64_t page = page_of(a.c, b, at, a.bad_index);
       if (page >= 0) {
         const int64_t from = page * sp + slot * ss + head[k] * sh + sub * 8;
         if constexpr (Q8) {
@@ -234,7 +227,7 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_kernel(const CacheRe
   for (int k = 0; k < N; ++k) {
     if (row0 + k * (kThreadsPaged / LPR) >= rows) continue;
     T* dst = out + token[k] * out_t + head[k] * out_h + sub * 8;
-    if constexpr (Q8) stg128(dst, widen_e4m3<T>(u[k], code[k]));
+    if constexpr (Q8) stg128(dst, widen_e4m3<T>(u[k], scale_value(code[k])));
     else stg128(dst, u[k]);
   }
 }
@@ -251,13 +244,13 @@ __global__ void __launch_bounds__(kThreadsPaged) cache_read_any_kernel(const Cac
   const int h = (int)(row % a.c.kv_heads);
   const int64_t b = token / a.len, pos = token % a.len;
   const Row r = row_of(nullptr, a.lens, b, a.len, a.c.width * a.c.page_size);
-  if (r.bad && pos == 0 && lane == 0) report_bad_index(a.status);
+  if (r.bad && pos == 0 && lane == 0) report_bad_index(a.bad_index);
   int64_t page = -1, from = 0;
   float scale = 0.f;
   if (pos < r.n) {
     const int64_t at = pos / a.c.page_size;
     const int slot = (int)(pos - at * a.c.page_size);
-    page = page_of(a.c, b, at, a.status);
+    page = page_of(a.c, b, at, a.bad_index);
     if (page >= 0) {
       from = is_v ? page * a.c.v_sp + slot * a.c.v_ss + h * a.c.v_sh : page * a.c.k_sp + slot * a.c.k_ss + h * a.c.k_sh;
       if constexpr (Q8) scale = scale_value(is_v ? a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + slot] : a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + slot]);
@@ -288,7 +281,7 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
   const int64_t i = item / a.heads % a.t, b = item / a.heads / a.t;
   const int hk = h / (a.heads / a.c.kv_heads), d = a.c.d;
   const Row r = row_of(a.start, a.lens, b, a.t, a.c.width * a.c.page_size);
-  if (r.bad && i == 0 && h == 0 && threadIdx.x == 0) report_bad_index(a.status);
+  if (r.bad && i == 0 && h == 0 && threadIdx.x == 0) report_bad_index(a.bad_index);
   const int64_t pos = r.start + i;
   int64_t lo = 0, hi = r.start + r.n;
   if (a.causal && pos + 1 < hi) hi = pos + 1;
@@ -308,7 +301,7 @@ __global__ void __launch_bounds__(128) attention_paged_exact_kernel(const PagedA
   for (int64_t j = lo + warp; j < hi; j += kWarps) {
     const int64_t at = j / a.c.page_size;
     const int slot = (int)(j - at * a.c.page_size);
-    const int64_t page = page_of(a.c, b, at, a.status);
+    const int64_t page = page_of(a.c, b, at, a.bad_index);
     const bool there = page >= 0;  // where no page is, a key and a value of zeros, as reading gives
     const int64_t fk = page * a.c.k_sp + slot * a.c.k_ss + hk * a.c.k_sh, fv = page * a.c.v_sp + slot * a.c.v_ss + hk * a.c.v_sh;
     float ks = 1.f, vs = 1.f;

@@ -63,12 +63,18 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t u) {
 // that was finite reads back finite, half a step off at most. NaN stays.
 template <typename T>
 constexpr float kLargest = std::is_same<T, __half>::value ? 65504.f : std::is_same<T, float>::value ? FLT_MAX : 0x1.fep127f;
-// The least scale code whose values (up to 448 * 2^(code - 127)) leave that range.
-template <typename T>
-constexpr uint32_t kCodeOutOfRange = std::is_same<T, __half>::value ? 135u : 247u;
 template <typename T>
 __device__ __forceinline__ float in_range(float x) {
   return fabsf(x) > kLargest<T> ? copysignf(kLargest<T>, x) : x;
+}
+
+// The same for a pair on its way into the type, in the conversion itself.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_in_range(float lo, float hi) {
+  uint32_t u;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+  return u;
 }
 
 // n / d for 0 <= n < 2^31 without a division: (floor(n m / 2^32) + n) >> shift with

@@ -54,10 +54,13 @@ def test_integers_of_64_bits_are_not_cut():
 def test_an_index_out_of_range_is_no_reason_to_stop_waiting():
     """Waits give up early when their own word is set; the reports of bad indexes go to another."""
     csrc = Path(ops.__file__).resolve().parent / "csrc"
-    for f in sorted(csrc.glob("*.cu*")):
-        for line in f.read_text().splitlines():
-            if "kStatusBadIndex" in line and "atomicExch" in line:
-                assert "status + 1" in line, (f.name, line)
+    calls = [(f.name, call) for f in sorted(csrc.glob("*.cu*")) for call in re.findall(r"report_bad_index\(([^)]*)\)", f.read_text())]
+    assert len(calls) > 10
+    for name, word in calls:
+        assert "bad_index" in word or "kBadIndexWord" in word or word == "uint32_t* word", (name, word)
+    for f in csrc.glob("*.cu*"):
+        stores = [line for line in f.read_text().splitlines() if "kStatusBadIndex" in line and "atomicExch" in line]
+        assert f.name == "common.cuh" or not stores
 
 
 @pytest.mark.parametrize("q8", [False, True])
