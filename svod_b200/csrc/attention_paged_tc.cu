@@ -26,9 +26,10 @@
 // 8-bit pages: a fourth warpgroup widens each block from a ring of raw e4m3 blocks into the
 // 16-bit rings, value * 2^e, exact in bf16 (a value is 4 bits) and rounded once in f16's
 // subnormals and at its top (`in_range`; weights rounded to f16 could carry an average of its
-// largest values past it, so such results are kept in range too). A thread moves a key's row: the e4m3 fields are shifted to where the 16-bit
-// type has them and one packed multiply puts exponent bias and scale right, 5 instructions a
-// pair of values (a conversion through f32 is 6, on slower pipes).
+// largest values past it, so such results are kept in range too). A thread moves a key's row:
+// the e4m3 fields are shifted to where the 16-bit type has them and one packed multiply puts
+// exponent bias and scale right, 5 instructions a pair of values (a conversion through f32 is 6,
+// on slower pipes).
 //
 // Every mbarrier wait is bounded; a warp that gave up walks on as in attention_tc_p.cu.
 #include <cuda.h>
@@ -280,7 +281,8 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       total *= a.c.kv_heads;
-      const Run run = run_of(total, (int)blockIdx.x, (int)gridDim.x);
+      const Run run = run_of(total, blockIdx.x, gridDim.x);
+      const int64_t c0 = run.c0, c1 = run.c1;
       // Row b for the whole warp.
       auto fetch_row = [&](int b) {
         if (b >= 32) return row_at(b);
@@ -290,55 +292,13 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         r.bad = false;
         return r;
       };
-      SplitItem split{0, 0, 0, 0, 0, 0};
-      uint32_t pos = 0;
-      bool ok = true;
-      uint32_t n_it = 0;
-      auto take = [&](const Row& row, const Share& sh) {
-        PagedWork w;
-        w.valid = 1, w.b = sh.b, w.hk = sh.hk, w.t0 = sh.q * 2 * p.tile_tokens, w.n_live = row.n, w.start = (int)row.start;
-        item_keys(p, row, sh.q, w.key_lo, w.key_hi);
-        const int blk_lo = w.key_lo / kBKV;
-        w.part = sh.part;
-        if (w.part == 1) split = SplitItem{1, sh.b, sh.hk, w.t0, row.n, sh.last_cta};
-        auto range = [&](int t) {
-          Range r{0, 0};
-          if (t >= row.n) return r;
-          const int t_last = min(t + p.tile_tokens, row.n) - 1;
-          const int lo = first_key(a, row.start + t) / kBKV;
-          const int hi = (last_key(a, row.start + t_last, row.start + row.n) + kBKV - 1) / kBKV;
-          const int y = max(lo, blk_lo + sh.from), z = min(hi, blk_lo + sh.to);
-          if (z > y) r.lo = y, r.hi = z;
-          return r;
-        };
-        w.r0 = range(w.t0);
-        w.r1 = range(w.t0 + p.tile_tokens);
-        const bool live0 = w.r0.hi > w.r0.lo, live1 = w.r1.hi > w.r1.lo;
-        w.u_lo = w.u_hi = 0;
-        if (live0 && live1) {
-          w.u_lo = w.r0.lo < w.r1.lo ? w.r0.lo : w.r1.lo;
-          w.u_hi = w.r0.hi > w.r1.hi ? w.r0.hi : w.r1.hi;
-        } else if (live0) {
-          w.u_lo = w.r0.lo, w.u_hi = w.r0.hi;
-        } else if (live1) {
-          w.u_lo = w.r1.lo, w.u_hi = w.r1.hi;
-        }
-        const int slot = (int)(n_it & 1);
-        ok = wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1);
-        if (!ok) return false;
-        if (lane == 0) {
-          item_ring[slot] = w;
-          __threadfence_block();
-          mbar_arrive(&item_full[slot]);
-        }
-        ++n_it;
-        ok = load_blocks(w, 0, pos);
-        return ok;
-      };
-      if (run.c0 < run.c1) {
-        // the row in which the run begins; its work begins at x
-        int b = 0;
-        int64_t x = 0, weight = 1, base = 0;
+      // Where the run begins: row b, KV head hk, item q, whose weight lies at [x, x + weight).
+      int b = 0, hk = 0, q = 0;
+      int64_t x = 0;
+      Row row{0, 0, false};
+      int64_t weight_of_row = 0;
+      if (c0 < c1) {
+        int64_t base = 0;
         for (int b0 = 0; b0 < batch; b0 += 32) {
           const int64_t w = (b0 == 0 ? my_weight : b0 + lane < batch ? row_weight(p, row_at(b0 + lane)) : 0) * a.c.kv_heads;
           int64_t upto = w;
@@ -347,17 +307,79 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
             const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += y;
           }
-          const uint32_t past = __ballot_sync(0xffffffffu, base + upto > run.c0);
+          const uint32_t past = __ballot_sync(0xffffffffu, base + upto > c0);
           if (past != 0u) {
             const int l = __ffs((int)past) - 1;
             b = b0 + l;
-            weight = __shfl_sync(0xffffffffu, w, l) / a.c.kv_heads;
+            weight_of_row = __shfl_sync(0xffffffffu, w, l) / a.c.kv_heads;
             x = base + __shfl_sync(0xffffffffu, upto - w, l);
             break;
           }
           base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        walk_run(p, run, batch, a.c.kv_heads, b, x, weight, fetch_row, take);
+        row = fetch_row(b);
+        find_item(p, run, row, weight_of_row, x, hk, q);
+      }
+      SplitItem split{0, 0, 0, 0, 0, 0};
+      uint32_t pos = 0;
+      bool ok = true;
+      uint32_t n_it = 0;
+      // (a CTA whose run would begin behind the last item has none)
+      while (c0 < c1 && x < c1 && ok) {
+        PagedWork w;
+        w.valid = 1, w.b = b, w.hk = hk, w.t0 = q * 2 * p.tile_tokens, w.n_live = row.n, w.start = (int)row.start;
+        item_keys(p, row, q, w.key_lo, w.key_hi);
+        const int blk_lo = w.key_lo / kBKV, blk_n = (w.key_hi + kBKV - 1) / kBKV - blk_lo;
+        const int64_t weight = blk_n + kItemCost;
+        // this run's part of the item's blocks: its first kItemCost units stand for the fixed cost
+        const int from = share_from(c0, x), to = share_to(c1, x, weight);
+        if (to > from) {
+          w.part = part_of(from, to, blk_n);
+          if (w.part == 1) split = SplitItem{1, b, hk, w.t0, row.n, last_cta(x, weight, run.quota)};
+          auto range = [&](int t) {
+            Range r{0, 0};
+            if (t >= row.n) return r;
+            const int t_last = min(t + p.tile_tokens, row.n) - 1;
+            const int lo = first_key(a, row.start + t) / kBKV;
+            const int hi = (last_key(a, row.start + t_last, row.start + row.n) + kBKV - 1) / kBKV;
+            const int y = max(lo, blk_lo + from), z = min(hi, blk_lo + to);
+            if (z > y) r.lo = y, r.hi = z;
+            return r;
+          };
+          w.r0 = range(w.t0);
+          w.r1 = range(w.t0 + p.tile_tokens);
+          const bool live0 = w.r0.hi > w.r0.lo, live1 = w.r1.hi > w.r1.lo;
+          w.u_lo = w.u_hi = 0;
+          if (live0 && live1) {
+            w.u_lo = w.r0.lo < w.r1.lo ? w.r0.lo : w.r1.lo;
+            w.u_hi = w.r0.hi > w.r1.hi ? w.r0.hi : w.r1.hi;
+          } else if (live0) {
+            w.u_lo = w.r0.lo, w.u_hi = w.r0.hi;
+          } else if (live1) {
+            w.u_lo = w.r1.lo, w.u_hi = w.r1.hi;
+          }
+          const int slot = (int)(n_it & 1);
+          ok = wait_by_lane0(&item_empty[slot], ((n_it >> 1) & 1) ^ 1);
+          if (!ok) break;
+          if (lane == 0) {
+            item_ring[slot] = w;
+            __threadfence_block();
+            mbar_arrive(&item_full[slot]);
+          }
+          ++n_it;
+          ok = load_blocks(w, 0, pos);
+        }
+        // the next item
+        x += weight;
+        if (++q == live_items(p, row)) {
+          q = 0;
+          if (++hk == a.c.kv_heads) {
+            hk = 0;
+            do row = ++b < batch ? fetch_row(b) : Row{0, 0, false};
+            while (b < batch && row.n == 0);
+            if (b >= batch) break;
+          }
+        }
       }
       if (lane == 0) {
         int* h = p.heads_of_split + (int64_t)blockIdx.x * kSplitInts;

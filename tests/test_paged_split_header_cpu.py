@@ -17,8 +17,8 @@ using namespace svodb::paged;
 struct Seen { int causal, has_window; int64_t win_left, win_right; };
 struct Params { Seen a; int tile_tokens; };
 extern "C" int constants(int* out) { out[0] = kItemCost, out[1] = kLeastShare, out[2] = kBlockKeys; return 0; }
-// The shares of a CTA, eight numbers each; the row in which its run begins is found one row after
-// the other, where the kernel's warp adds up 32 at a time.
+// The shares of a CTA, seven numbers each. The steps from item to item are the kernel's; the row in
+// which the run begins is found one row after the other, where its warp adds up 32 at a time.
 extern "C" int walk(int rows, const int* start, const int* n, int kv, int tile_tokens, int causal, int window, int left, int right,
                     int ctas, int cta, int* out, int room) {
   const Params p{{causal, window, left, right}, tile_tokens};
@@ -26,18 +26,31 @@ extern "C" int walk(int rows, const int* start, const int* n, int kv, int tile_t
   int64_t total = 0;
   for (int b = 0; b < rows; ++b) total += row_weight(p, row_at(b)) * kv;
   const Run run = run_of(total, cta, ctas);
-  int count = 0;
+  int count = 0, b = 0, hk, q;
   if (run.c0 >= run.c1) return 0;
   int64_t x = 0;
-  int b = 0;
   while (x + row_weight(p, row_at(b)) * kv <= run.c0) x += row_weight(p, row_at(b++)) * kv;
-  walk_run(p, run, rows, kv, b, x, row_weight(p, row_at(b)), row_at, [&](const Row& row, const Share& s) {
-    int lo, hi;
-    item_keys(p, row, s.q, lo, hi);
-    const int all[8] = {s.b, s.hk, s.q, s.from, s.to, s.part, s.last_cta, s.blocks == (hi + kBlockKeys - 1) / kBlockKeys - lo / kBlockKeys};
-    for (int i = 0; i < 8; ++i) out[count * 8 + i] = all[i];
-    return ++count < room;
-  });
+  Row row = row_at(b);
+  find_item(p, run, row, row_weight(p, row), x, hk, q);
+  while (x < run.c1) {
+    const int blocks = item_blocks(p, row, q), weight = blocks + kItemCost;
+    const int from = share_from(run.c0, x), to = share_to(run.c1, x, weight);
+    if (to > from) {
+      if (count == room) return -1;
+      const int all[7] = {b, hk, q, from, to, part_of(from, to, blocks), last_cta(x, weight, run.quota)};
+      for (int i = 0; i < 7; ++i) out[count * 7 + i] = all[i];
+      ++count;
+    }
+    x += weight;
+    if (++q < live_items(p, row)) continue;
+    q = 0;
+    if (++hk < kv) continue;
+    hk = 0;
+    do {
+      if (++b >= rows) return count;
+      row = row_at(b);
+    } while (row.n == 0);
+  }
   return count;
 }
 """
@@ -70,11 +83,11 @@ def test_the_kernels_shares_are_the_walks(host, seed):
         rows = [(7, 0)] + rows + [(0, 0), (90, 0)]
     plan = Plan(rows, kv, step, causal, window, ctas)
     ints = lambda xs: (C.c_int * len(xs))(*xs)
-    starts, ns, out = ints([r[0] for r in rows]), ints([r[1] for r in rows]), (C.c_int * (8 * 40000))()
+    starts, ns, out = ints([r[0] for r in rows]), ints([r[1] for r in rows]), (C.c_int * (7 * 40000))()
     for cta in range(ctas):
         n = host.walk(len(rows), starts, ns, kv, step // 2, causal, window is not None, *(window or (0, 0)), ctas, cta, out, 40000)
-        got = [tuple(out[8 * k:8 * k + 8]) for k in range(n)]
+        got = [tuple(out[7 * k:7 * k + 7]) for k in range(n)]
         want, split = plan.walk(cta)
-        assert [s[:6] for s in got] == want and all(s[7] == 1 for s in got)
+        assert [s[:6] for s in got] == want
         first = [(*s[:3], s[6]) for s in got if s[5] == 1]
         assert first == ([split] if split else [])
