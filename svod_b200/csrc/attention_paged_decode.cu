@@ -114,21 +114,50 @@ __device__ __forceinline__ int last_seen(const PagedAttnArgs& a, const Row& r, i
   return (int)x;
 }
 
-// A row's class of length: its blocks of visible keys to three bits behind the first, so rows
-// of one class differ by an eighth at most. 0 for a row without keys, 200 at most.
-__device__ __forceinline__ int length_class(const PagedAttnArgs& a, const Row& r) {
+// A row's blocks of visible keys, and their class, 0 to 254: their number where they are few, from
+// 16 on to four bits behind the first, so rows of one class differ by a sixteenth at most.
+__device__ __forceinline__ int row_keys(const PagedAttnArgs& a, int64_t b, int64_t capacity, int unit) {
+  const Row r = row_of(a.start, a.lens, b, a.t, capacity);
   if (r.n <= 0) return 0;
-  const int blocks = (last_seen(a, r, r.n - 1) + kKeys - 1) / kKeys - first_seen(a, r, 0) / kKeys;
-  return blocks <= 0 ? 0 : (int)(__float_as_uint((float)blocks) >> 20) - (127 << 3) + 1;
+  const int n = (last_seen(a, r, r.n - 1) + unit - 1) / unit - first_seen(a, r, 0) / unit;
+  return n < 0 ? 0 : n;
+}
+__device__ __forceinline__ int length_class(int blocks) {
+  return blocks < 16 ? blocks : min((int)(__float_as_uint((float)blocks) >> 19) - (131 << 4) + 16, kClasses - 2);
 }
 
-// The row that comes `at`-th when the batch is put in order, longest classes first and rows of
-// one class as they lie: the chip takes the long rows first, the short ones fill its last places.
-// Work in proportion to the batch: every row's class is counted, every warp finds from the counts
-// which class holds the place and from the classes which of its rows that is. `mem` (2 KB) is
-// free again when the call returns.
+// The row that comes `at`-th when the batch is put in order, longest first and rows of one length
+// (or class) as they lie: the chip takes the long rows first, the short ones fill its last places.
+// Up to kRankedRows rows are compared with each other. More would take work that grows with the
+// square of the batch in each of its CTAs (1024 rows of 100..1000 keys x 8 KV heads: 3317 us, 543
+// by classes); by classes it is in proportion: every row's class is counted, every warp finds from
+// the counts which class holds the place and from the classes which of its rows that is. By
+// comparison | by classes, 8 KV heads, us: 16 rows of 8000..32767 keys in e4m3 118.8 | 120.4, 64
+// of 64..4095 56.9 | 57.6, 128 of them 104.9 | 104.0; 96 in bf16 137.8 | 137.2; 300 rows of
+// 16..200 x 2 KV heads 45 | 29. `mem` (2 KB) is free again when the call returns.
+constexpr int kRankedRows = 64;
 __device__ __forceinline__ int longest_first_row(const PagedAttnArgs& a, int at, int64_t capacity, uint8_t* mem) {
   const int tid = threadIdx.x, lane = tid & 31, batch = (int)a.batch;
+  if (batch <= kRankedRows) {
+    int* keys = reinterpret_cast<int*>(mem);  // [padded], then the row
+    const int padded = (batch + 3) & ~3;
+    if (tid < padded) keys[tid] = tid < batch ? row_keys(a, tid, capacity, 1) : -1;
+    __syncthreads();
+    if (tid < batch) {
+      const int mine = keys[tid];
+      int rank = 0;
+      for (int o = 0; o < padded; o += 4) {
+        const int4 n = *reinterpret_cast<const int4*>(keys + o);
+        rank += (n.x > mine || (n.x == mine && o < tid)) + (n.y > mine || (n.y == mine && o + 1 < tid)) +
+                (n.z > mine || (n.z == mine && o + 2 < tid)) + (n.w > mine || (n.w == mine && o + 3 < tid));
+      }
+      if (rank == at) keys[padded] = tid;
+    }
+    __syncthreads();
+    const int row = keys[padded];
+    __syncthreads();  // before anything is written over it
+    return row;
+  }
   int* counts = reinterpret_cast<int*>(mem);  // [kClasses]
   uint8_t* classes = mem + kClasses * 4;      // [32 lanes][per]
   const int per = (batch + 127) / 128 * 4;    // rows that a lane looks through
@@ -137,7 +166,7 @@ __device__ __forceinline__ int longest_first_row(const PagedAttnArgs& a, int at,
   for (int k = tid; k < 32 * per; k += kThreadsDec) {
     int c = kClasses - 1;  // no row's
     if (k < batch) {
-      c = length_class(a, row_of(a.start, a.lens, k, a.t, capacity));
+      c = length_class(row_keys(a, k, capacity, kKeys));
       atomicAdd(&counts[c], 1);
     }
     classes[k] = (uint8_t)c;

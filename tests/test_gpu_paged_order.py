@@ -17,7 +17,7 @@ def i32(x):
 
 
 @pytest.mark.parametrize("dtype,quantized", TYPES)
-@pytest.mark.parametrize("batch,kv", [(64, 8), (150, 4), (1023, 1), (1024, 1)])
+@pytest.mark.parametrize("batch,kv", [(64, 8), (65, 8), (150, 4), (1023, 1), (1024, 1)])
 @pytest.mark.parametrize("lengths", ["equal", "ragged", "rising"])
 def test_every_row_of_a_wide_batch(dtype, quantized, batch, kv, lengths):
     """Rows of one length, of many (some without a token, one past its table), and longer row by
