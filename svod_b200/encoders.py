@@ -253,6 +253,7 @@ class Qwen3Embedder:
         if len(caches) != c.num_hidden_layers:
             raise ValueError(f"extend: {len(caches)} caches for {c.num_hidden_layers} layers")
         B, T = ids.shape
+        ids = ids.contiguous()  # a chunk is a slice of a document's ids
         start = ops._i32(start)
         last = torch.full_like(start, T) if lens is None else ops._i32(lens)
         at = start[:, None] + torch.arange(T, dtype=torch.int32, device=start.device)

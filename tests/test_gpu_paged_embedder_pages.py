@@ -80,3 +80,16 @@ def test_a_shared_instruction_and_chunks_over_the_pages_they_wrote(quantized):
             assert (plain - want).norm() >= 2 * TOL  # so the bound above tells the pages apart
         else:
             assert (plain - want).norm() <= TOL
+
+
+def test_chunks_are_slices_of_a_documents_ids():
+    p, rng = T.weights(), np.random.default_rng(19)
+    m = T.model(p)
+    ids, table = T.i32(rng.integers(0, T.V, (2, 90))), T.i32([[0, 1], [3, 2]])
+    whole = m.extend(ids, m.paged_caches(4, 64), table, T.i32([0, 0]))
+    for kind in (torch.int32, torch.int64):
+        caches = m.paged_caches(4, 64)
+        for lo, hi in ((0, 50), (50, 89), (89, 90)):
+            got = m.extend(ids.to(kind)[:, lo:hi], caches, table, T.i32([lo, lo]))
+        ops.device_status()
+        assert ((got - whole).double().norm(dim=-1) <= 2 * TOL).all()
