@@ -41,8 +41,8 @@
 //
 // Every mbarrier wait is bounded; a timeout records a status code and the CTA
 // drains and frees its TMEM. Named barriers have no timeout, so a warp that
-// gave up never waits on one again: it only arrives, once per remaining turn of
-// its partner, which is thereby released whether or not it gave up too.
+// gave up walks its remaining turns, waits and arrivals, as if it computed: its
+// partner is released turn by turn, whether or not it gave up too.
 #include <cuda.h>
 #include <math.h>
 #include <stdio.h>
@@ -553,9 +553,10 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
       if (lane == 0) mbar_arrive(&p_full[i * 2 + buf]);
     }
     if (!ok) {
+      // the remaining turns, each waited for as ever: arrivals one after the other would complete
+      // the barrier between them, and the partner's wait has no limit
       for (int m = turns_done; m < n_paired; ++m) {
-        // arrivals only: the partner is released at each of its remaining turns and
-        // this warp never waits on a barrier without a limit again
+        if (i == 1 || m > 0) named_barrier(my_turn, 64);
         if (i == 0 || m + 1 < n_paired) named_barrier_arrive(other_turn, 64);
       }
     }
