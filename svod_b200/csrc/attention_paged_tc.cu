@@ -132,6 +132,23 @@ __device__ __forceinline__ uint32_t widen_factor(uint32_t code) {
   return h | (h << 16);
 }
 
+// A softmax warp that no item came to within the limit, which the status word says: the loader's
+// next wait ends, but what it published until then the warp's partner may have caught, and both
+// have to walk the same turns. So it takes what has come after a while longer.
+__device__ __noinline__ void walk_late_items(uint64_t* item_full, uint64_t* item_empty, const PagedWork* ring, uint32_t n_it, int i,
+                                             uint32_t turns, int my_turn, int other_turn) {
+  for (; mbar_arrives(&item_full[n_it & 1], (n_it >> 1) & 1, kWaitLimit / 64); ++n_it) {
+    const int n_paired = ring[n_it & 1].valid ? paired_blocks(ring[n_it & 1].r0, ring[n_it & 1].r1) : -1;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&item_empty[n_it & 1]);
+    if (n_paired < 0) break;
+    for (int m = 0; m < n_paired; ++m, ++turns) {
+      if (i == 1 || turns > 0) named_barrier(my_turn, 64);
+      named_barrier_arrive(other_turn, 64);
+    }
+  }
+}
+
 template <typename T, bool Q8, int D>
 __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
     attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -676,10 +693,12 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
     // CTA's first excepted, and a warp whose bounded wait ran out walks all turns on.
     uint32_t turns = 0;       // of all earlier items and this one
     bool ok = true;           // false once a bounded wait ran out: nothing is computed from then on
-    for (uint32_t n_it = 0;; ++n_it) {
+    bool late = false;        // no item came within the limit
+    uint32_t n_it = 0;
+    for (;; ++n_it) {
       const int slot = (int)(n_it & 1);
       if (!mbar_wait_patient(&item_full[slot], (n_it >> 1) & 1, a.status)) {
-        for (int64_t m = 0; m < 2 * (capacity / kBKV + 2); ++m) named_barrier_arrive(other_turn, 64);
+        late = true;
         break;
       }
       const PagedWork w = item_ring[slot];
@@ -929,6 +948,7 @@ __global__ void __launch_bounds__((PagedTcCfg<Q8, D>::kThreads), 1)
         a.lse[((int64_t)w.b * a.heads + head) * a.t + t_row] = l_run == 0.f ? -INFINITY : kLn2F * (m_run + log2f(l_run));
       }
     }
+    if (late) walk_late_items(item_full, item_empty, item_ring, n_it, i, turns, my_turn, other_turn);
   }
 
   tc_fence_before();

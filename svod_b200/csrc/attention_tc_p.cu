@@ -535,17 +535,16 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
     // is left unanswered. Both leave when the queue ends or stops being fed.
     bool turned = false;  // the CTA has had a turn
     bool ok = true;
-    for (uint32_t n_it = 0;; ++n_it) {
+    bool late = false;  // no item came within the limit
+    uint32_t n_it = 0;
+    for (;; ++n_it) {
       const int slot = (int)(n_it & 1);
       // Both warps of a MUFU pair must take the same items: this wait ignores a
       // status word that is already set (it would let one partner leave while the
       // other still receives the item and then waits on a named barrier for good)
       // and ends only with the item or with its own limit, which both reach together.
       if (!mbar_wait_patient(&item_full[slot], (n_it >> 1) & 1, p.status)) {
-        // No item within the limit: the queue is dead. Should the partner have
-        // caught an item in the instant between the two limits (the loader can be
-        // at most two items ahead), it is released through every turn it may take.
-        for (int64_t m = 0; m < 2 * (p.tk / kBKV + 2); ++m) named_barrier_arrive(other_turn, 64);
+        late = true;
         break;
       }
       const Work w = item_ring[slot];
@@ -828,6 +827,23 @@ __global__ void __launch_bounds__(kThreadsFa, 1)
       }
       if (p.lse != nullptr && row_ok)
         p.lse[(b * p.heads + h) * p.t + row] = l_run == 0.f ? -INFINITY : kLn2F * (m_run + log2f(l_run));
+    }
+    // No item within the limit, and the status word says so: the loader's next wait ends, but what
+    // it published until then the partner may have caught, and both have to walk the same turns.
+    // So this warp takes what has come after a while longer.
+    for (; late && mbar_arrives(&item_full[n_it & 1], (n_it >> 1) & 1, kWaitLimit / 64); ++n_it) {
+      const int n_paired = item_ring[n_it & 1].valid ? paired_blocks(item_ring[n_it & 1].r0, item_ring[n_it & 1].r1) : -1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[n_it & 1]);
+      if (n_paired < 0) break;
+      if (i == 0 && n_paired > 0) {
+        if (turned) named_barrier(my_turn, 64);
+        turned = true;
+      }
+      for (int m = 0; m < n_paired; ++m) {
+        if (i == 1 || m > 0) named_barrier(my_turn, 64);
+        named_barrier_arrive(other_turn, 64);
+      }
     }
     if (lane == 0) tma_store_wait_all();  // the slab stays put until its last store has read it
   }

@@ -243,6 +243,12 @@ __device__ __forceinline__ bool mbar_wait_patient(uint64_t* bar, uint32_t parity
   atomicExch(status, (uint32_t)kStatusWaitTimeout);
   return false;
 }
+// Whether `parity` comes on `bar` within `limit` polls; nothing is reported.
+__device__ __forceinline__ bool mbar_arrives(uint64_t* bar, uint32_t parity, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
 
 // ---- TMA (non-multicast only) ----------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {

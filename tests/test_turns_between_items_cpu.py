@@ -15,12 +15,11 @@ ONE_ITEM = "attention_tc.cu"  # an item a CTA: its last turn is nobody's to wait
 
 
 def rules(name, call):
-    """The conditions under which the kernel makes `call`, as Python; those of its loops that
-    only run when no more items come are left out."""
+    """The conditions under which the kernel makes `call`, as Python."""
     lines = [line for line in (CSRC / name).read_text().splitlines() if not line.strip().startswith("//")]
     found = []
     for k, line in enumerate(lines):
-        if call not in line or "for (" in line:
+        if call not in line:
             continue
         conds = re.findall(r"if \((.*)\)", line.split("named_barrier")[0])
         if re.search(r"if \(.*[{)]$", lines[k - 1]):  # the block it stands in, or the line it goes with
@@ -35,7 +34,7 @@ def test_no_warp_arrives_twice_before_its_partner_waits(name, seed):
     g = random.Random(seed)
     items = [g.choice([0, 1, 1, 2, 3, 7]) for _ in range(1 if name == ONE_ITEM else g.randint(2, 25))]
     waits, passes = rules(name, "named_barrier(my_turn"), rules(name, "named_barrier_arrive(other_turn")
-    border = [w for w in waits if "turned" in w]  # once an item
+    border = {w for w in waits if "turned" in w}  # once an item
     waits = [w for w in waits if w not in border]  # once a turn: in the block loop, and where a warp has given up
     assert waits and len(border) <= 1
     assert len(waits) == len(passes), "a place that passes turns on without waiting for its own"
@@ -44,7 +43,7 @@ def test_no_warp_arrives_twice_before_its_partner_waits(name, seed):
         turns = 0
         for n_paired in items:
             env = dict(i=i, n_paired=n_paired, pairs=n_paired, turned=turns > 0)
-            if border and eval(border[0], {}, env):
+            if any(eval(b, {}, env) for b in border):
                 yield "wait"
             for n in range(n_paired):
                 env.update(n=n, m=n, turns=turns)
