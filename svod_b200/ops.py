@@ -510,7 +510,8 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, lengt
     """`(k, v)` `[B, length, kv_heads, D]` of the sequences under `table`: the first
     `lens[b]` positions of row `b`, zeros behind them. `length` defaults to what the table
     reaches; `dtype` is the pages' own, for 8-bit pages any float type (bf16 by default;
-    value times scale, rounded once)."""
+    value times scale, rounded once, its largest number for what is beyond it). Positions
+    whose table entry is no page are zeros too, and `device_status()` raises."""
     global launches
     if dtype is None:
         dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
