@@ -1118,6 +1118,7 @@ size_t svodb_attention_paged_workspace_bytes(const svodb_tensor* q, const svodb_
   a.q_sb = a.o_sb = q->stride[0], a.q_st = a.o_st = q->stride[1], a.q_sh = a.o_sh = q->stride[2];
   a.scale = 1.f;
   // the few-row kernel merges on the chip, the exact one has nothing to merge
+  if (config_lookup("attention|exact") != 0) return 0;
   return attention_paged_few_rows(a) || !attention_paged_tc_covers(a) ? 0 : attention_paged_tc_workspace(a);
 }
 

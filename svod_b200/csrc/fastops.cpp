@@ -22,6 +22,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+
 #include "svodb.h"
 
 namespace {
@@ -443,7 +445,9 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   at::Tensor out = at::empty(qt.sizes(), qt.options()), lse, ws;
   desc_of(out, y, q.dtype);
   if (want) lse = lse_for(qt, q.shape[0], q.shape[2], q.shape[1], o, ak);
-  const size_t need = p_attention_paged_workspace_bytes(&q, &c);
+  // (a scale that is not positive is the exact kernel's, which wants none)
+  const bool tiles = !o.has_scale || (o.scale > 0.f && std::isfinite(o.scale));
+  const size_t need = tiles ? p_attention_paged_workspace_bytes(&q, &c) : 0;
   if (need > 0) {
     ws = at::empty({(int64_t)need}, qt.options().dtype(at::kByte));
     o.workspace = ws.data_ptr(), o.workspace_bytes = need;

@@ -570,7 +570,9 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, sta
         o, lse = _attn_opts(opts, q.shape, q.dtype, q.device, keep)
         qd, sd, ld, od = _desc(q), _desc(start), _desc(lens), _desc(out)
         lib = L.load()
-        need = lib.svodb_attention_paged_workspace_bytes(_p(qd), C.byref(c))
+        # (a scale that is not positive is the exact kernel's, which wants none)
+        tiles = not o.has_scale or 0 < o.scale < float("inf")
+        need = lib.svodb_attention_paged_workspace_bytes(_p(qd), C.byref(c)) if tiles else 0
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             keep.append(ws)

@@ -162,6 +162,17 @@ def test_a_bad_row_does_not_shorten_the_waits_beside_it():
     ops.device_status()
 
 
+def test_one_launch_is_counted_where_the_exact_kernel_takes_the_call():
+    q, start, table = torch.randn(2, 40, 4, 64, device="cuda").to(BF16), i32([0, 0]), i32([[0, 1, 2], [3, 4, 5]])
+    cache = ops.PagedCache.empty(12, 16, 2, 64)
+    for scale, want in ((None, 2), (0.3, 2), (0.0, 1), (-0.5, 1)):
+        for lens in (None, torch.tensor([40, 3], device="cuda")):  # the compiled call path and the general one
+            before = ops.launches
+            ops.attention_paged(q, cache, table, start, lens, ops.Attn(causal=True, scale=scale))
+            assert ops.launches - before == want and ops.chosen().startswith("attention_paged: graph") == (want == 1)
+    ops.device_status()
+
+
 def test_a_timeout_is_told_before_a_bad_index():
     cache = ops.PagedCache.empty(2, 16, 1, 64)
     x = torch.zeros(1, 1, 1, 64, dtype=BF16, device="cuda")
