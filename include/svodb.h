@@ -100,9 +100,10 @@ int svodb_config_set(const char* key, int32_t value);
 int32_t svodb_config_get(const char* key);
 void svodb_config_clear(void);
 
-/* Reads and clears the device status word bounded waits report into
- * (0 = ok). Synchronises `stream`. Returns SVODB_ERR_TIMEOUT when a wait ran
- * out since the last call. */
+/* Reads and clears what kernels reported on the device since the last call:
+ * SVODB_ERR_TIMEOUT when a bounded wait ran out, else SVODB_ERR_SHAPE when an
+ * index in device memory was out of range (a cache row map or page table entry,
+ * a position past the table). Synchronises `stream`. */
 int svodb_device_status(void* stream);
 
 /* Self-tests of the failure paths; none of them hangs or faults the device.

@@ -114,8 +114,9 @@ __device__ __forceinline__ int last_seen(const PagedAttnArgs& a, const Row& r, i
   return (int)x;
 }
 
-// A row's blocks of visible keys, and their class, 0 to 254: their number where they are few, from
-// 16 on to four bits behind the first, so rows of one class differ by a sixteenth at most.
+// A row's visible keys in blocks of `unit`; and the class of a number of blocks, 0 to 254: itself
+// where they are few, from 16 on to four bits behind the first, so rows of one class differ by a
+// sixteenth at most.
 __device__ __forceinline__ int row_keys(const PagedAttnArgs& a, int64_t b, int64_t capacity, int unit) {
   const Row r = row_of(a.start, a.lens, b, a.t, capacity);
   if (r.n <= 0) return 0;
