@@ -217,7 +217,8 @@ def chosen() -> Optional[str]:
 
 
 def device_status() -> None:
-    """Raises if a bounded device-side wait ran out since the last check."""
+    """Raises if a bounded device-side wait ran out since the last check, or an index in device
+    memory (a cache row map or page table entry, a position past the table) was out of range."""
     _check(L.load().svodb_device_status(_stream()), 0)
 
 
