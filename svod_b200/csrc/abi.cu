@@ -164,6 +164,9 @@ int no_alias(const char* op, const svodb_tensor* out, std::initializer_list<cons
   return SVODB_OK;
 }
 
+// A vector that kernels read element after element.
+bool is_vector(const svodb_tensor* t, int64_t n) { return t->rank == 1 && t->shape[0] == n && contiguous(t); }
+
 bool same_shape(const svodb_tensor* a, const svodb_tensor* b) {
   if (a->rank != b->rank) return false;
   for (int i = 0; i < a->rank; ++i)
@@ -355,7 +358,7 @@ int svodb_linear(const svodb_tensor* x, const svodb_tensor* w, const svodb_linea
   }
   if (opts->bias != nullptr) {
     TRY(realized(OP, "bias", opts->bias));
-    if (opts->bias->rank != 1 || opts->bias->shape[0] != w->shape[0]) return shape_err(OP, "bias", opts->bias, "[N]");
+    if (!is_vector(opts->bias, w->shape[0])) return shape_err(OP, "bias", opts->bias, "[N], contiguous");
     if (opts->bias->dtype != x->dtype) return dtype_err(OP, "bias", opts->bias->dtype, x->dtype);
   }
   // out shape = lead..., N
@@ -617,7 +620,7 @@ int attend(const char* OP, const svodb_tensor* q, const svodb_tensor* k, const s
     if (mapped) {
       TRY(realized(OP, "row map", opts->cache_row_map));
       const svodb_tensor* m = opts->cache_row_map;
-      if (m->rank != 1 || m->shape[0] != B) return shape_err(OP, "row map", m, "[B]");
+      if (!is_vector(m, B)) return shape_err(OP, "row map", m, "[B], contiguous");
       if (m->dtype != SVODB_I32) return dtype_err(OP, "row map", m->dtype, SVODB_I32);
     }
     if ((opts->cache_app_k != nullptr) != (opts->cache_app_v != nullptr))
@@ -639,7 +642,7 @@ int attend(const char* OP, const svodb_tensor* q, const svodb_tensor* k, const s
     if (opts->cache_app_lens != nullptr) {
       TRY(realized(OP, "appended lens", opts->cache_app_lens));
       const svodb_tensor* t = opts->cache_app_lens;
-      if (n_app == 0 || t->rank != 1 || t->shape[0] != B) return shape_err(OP, "appended lens", t, "[B] with appended rows");
+      if (n_app == 0 || !is_vector(t, B)) return shape_err(OP, "appended lens", t, "[B] with appended rows, contiguous");
       if (t->dtype != SVODB_I32) return dtype_err(OP, "appended lens", t->dtype, SVODB_I32);
     }
   }
@@ -647,7 +650,7 @@ int attend(const char* OP, const svodb_tensor* q, const svodb_tensor* k, const s
     return fail(SVODB_ERR_GRAPH, "%s: key lengths and a key mask are alternatives (KeyMask)", OP);
   if (opts->key_lens != nullptr) {
     TRY(realized(OP, "key lens", opts->key_lens));
-    if (opts->key_lens->rank != 1 || opts->key_lens->shape[0] != B) return shape_err(OP, "key lens", opts->key_lens, "[B]");
+    if (!is_vector(opts->key_lens, B)) return shape_err(OP, "key lens", opts->key_lens, "[B], contiguous");
     if (opts->key_lens->dtype != SVODB_I32) return dtype_err(OP, "key lens", opts->key_lens->dtype, SVODB_I32);
   }
   if (opts->key_mask != nullptr) {
@@ -1284,7 +1287,7 @@ int svodb_heads(const svodb_tensor* qkv, const svodb_qkv_opts* opts, svodb_tenso
   for (int i = 0; i < 2; ++i) {
     if (norms[i] == nullptr) continue;
     TRY(realized(OP, nnames[i], norms[i]));
-    if (norms[i]->rank != 1 || norms[i]->shape[0] != d) return shape_err(OP, nnames[i], norms[i], "[head_dim]");
+    if (!is_vector(norms[i], d)) return shape_err(OP, nnames[i], norms[i], "[head_dim], contiguous");
     if (norms[i]->dtype != qkv->dtype) return dtype_err(OP, nnames[i], norms[i]->dtype, qkv->dtype);
   }
   const int64_t B = qkv->shape[0], T = qkv->shape[1];
@@ -1343,11 +1346,11 @@ int norm_op(const char* OP, int layer, const svodb_tensor* x, const svodb_tensor
   if (x->rank < 1) return shape_err(OP, "x", x, "[..., D]");
   const int64_t d = x->shape[x->rank - 1];
   if (!is_float(x->dtype)) return fail(SVODB_ERR_GRAPH, "%s: x is not a float type", OP);
-  if (w->rank != 1 || w->shape[0] != d) return shape_err(OP, "w", w, "[D]");
+  if (!is_vector(w, d)) return shape_err(OP, "w", w, "[D], contiguous");
   if (w->dtype != x->dtype) return dtype_err(OP, "w", w->dtype, x->dtype);
   if (b != nullptr) {
     TRY(realized(OP, "b", b));
-    if (b->rank != 1 || b->shape[0] != d) return shape_err(OP, "b", b, "[D]");
+    if (!is_vector(b, d)) return shape_err(OP, "b", b, "[D], contiguous");
     if (b->dtype != x->dtype) return dtype_err(OP, "b", b->dtype, x->dtype);
   }
   if (residual != nullptr) {
@@ -1528,7 +1531,7 @@ int pool_impl(const char* OP, const svodb_tensor* hidden, const svodb_tensor* no
     if (aux->dtype != SVODB_U8 && aux->dtype != SVODB_I32) return dtype_err(OP, "mask", aux->dtype, SVODB_U8);
   } else if (mode == 2) {
     TRY(realized(OP, "lengths", aux));
-    if (aux->rank != 1 || aux->shape[0] != B) return shape_err(OP, "lengths", aux, "[B]");
+    if (!is_vector(aux, B)) return shape_err(OP, "lengths", aux, "[B], contiguous");
     if (aux->dtype != SVODB_I32) return dtype_err(OP, "lengths", aux->dtype, SVODB_I32);
   }
   if (L == 0) return shape_err(OP, "hidden", hidden, "[B, L >= 1, D]");

@@ -291,7 +291,7 @@ def _attn_opts(opts: Attn, q_shape, dtype, device, keep: list):
     o.causal = int(opts.causal)
     if opts.keys is not None and opts.keys.lens is not None:
         t = opts.keys.lens
-        t = t if t.dtype == torch.int32 else t.to(torch.int32)
+        t = (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
         keep.append(_desc(t)), keep.append(t)
         o.key_lens = C.pointer(keep[-2])
     if opts.keys is not None and opts.keys.mask is not None:
@@ -761,8 +761,8 @@ def norm_pool(hidden, norm_w=None, norm_b=None, eps: float = 1e-5, layer: bool =
     elif out is None:
         rows = B * aux.shape[1] if mode == POOL_GATHER else B
         out = torch.empty(rows, D, dtype=torch.float32, device=hidden.device)
-    if aux is not None and aux.dtype not in (torch.bool, torch.uint8, torch.int32):
-        aux = aux.to(torch.int32)
+    if aux is not None:
+        aux = (aux if aux.dtype in (torch.bool, torch.uint8, torch.int32) else aux.to(torch.int32)).contiguous()
     a, b, c, w, bb = _desc(hidden), _desc(aux), _desc(out), _desc(norm_w), _desc(norm_b)
     lib = L.load()
 
@@ -790,8 +790,8 @@ def pool(hidden, aux=None, mode: int = POOL_CLS, normalize: bool = True, out=Non
     if out is None:
         rows = B * aux.shape[1] if mode == POOL_GATHER else B
         out = torch.empty(rows, D, dtype=torch.float32, device=hidden.device)
-    if aux is not None and aux.dtype not in (torch.bool, torch.uint8, torch.int32):
-        aux = aux.to(torch.int32)
+    if aux is not None:
+        aux = (aux if aux.dtype in (torch.bool, torch.uint8, torch.int32) else aux.to(torch.int32)).contiguous()
     a, b, c = _desc(hidden), _desc(aux), _desc(out)
     _check(L.load().svodb_pool(_p(a), _p(b), int(mode), int(normalize), _p(c), _stream()), 2 if normalize else 1)
     return out
